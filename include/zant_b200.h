@@ -87,7 +87,11 @@ typedef enum zant_dtype {
     ZANT_F32 = 0,
     ZANT_I8 = 1,
     ZANT_U8 = 2,
-    ZANT_I32 = 3
+    ZANT_I32 = 3,
+    /* Taken by the operators that name them (quantize_rows, qmatmul_scaled, qmatmul_grouped, token_logprobs); all others
+     * return ZANT_E_INPUT_ARRAY_WRONG_TYPE. */
+    ZANT_F16 = 4,
+    ZANT_BF16 = 5
 } zant_dtype;
 
 /* AutoPadType of src/Core/Tensor/TensorMath/op_pooling.zig:9-14 (same ordinal values). */
@@ -555,6 +559,61 @@ int32_t zant_b200_maxpool_q8(zant_ctx* ctx, int32_t dtype,
  * (unsigned view of the byte): y[i] = lut[(uint8_t)x[i]].  Used for LeakyReLU / ReLU /
  * rescale between QDQ tensors, where the table is built on the host from the pinned formula. */
 int32_t zant_b200_lut_q8(zant_ctx* ctx, const void* x, const uint8_t lut[256], void* y, size_t n);
+
+/* ------------------------------------------------------------------------------------------
+ * Operators of language models on the int8 path: activations are quantized as they come, with one scale for each row
+ * (token); weights are int8 [out, in] with one scale for each output channel.  No counterpart in the reference tree.
+ * They differ from the operators above in three points: F16 and BF16 take part, rows may lie further apart than they are
+ * long, and a call with no rows does nothing.
+ *   - *_stride is the distance between rows in elements, 0 for dense rows; less than a row is WrongStride.
+ *   - Device pointers must be aligned to their element (InvalidInput).  Rows of int8 operands that start at multiples of 16
+ *     bytes (pointer and stride) are read by the tensor memory accelerator; others take a slower kernel, same results.
+ *   - All calls with device pointers may be captured into a CUDA graph; they use no workspace.
+ *   - Arrays of a call must not overlap its outputs.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Symmetric int8 codes with one scale for each row of x [x_rows, cols] (F32, F16 or BF16):
+ *   scale[r] = max |x[r, :]| / 127                 (fp32 division)
+ *   q[r, c]  = the integer nearest to x[r, c] / scale[r], ties to even, at most 127 in magnitude
+ * The quotient is the exact one: where an fp32 division would round onto a tie, the codes may differ from QuantizeLinear's.
+ * A row of zeros (or one whose scale underflows to zero) has scale 0 and codes 0.  A row that holds a NaN or an infinity has
+ * scale NaN and codes 0, so that its products are NaN and no other row's are.
+ * `index` (int32, `rows` entries, may be NULL): row r of the result is row index[r] of x, as tokens are put in the order of
+ * their experts; an index outside [0, x_rows), -1 by custom, gives scale 0 and codes 0.  NULL: rows must equal x_rows. */
+int32_t zant_b200_quantize_rows(zant_ctx* ctx, int32_t x_dtype, const void* x, size_t x_rows, size_t cols, size_t x_stride,
+                                const int32_t* index, size_t rows,
+                                int8_t* q, size_t q_stride, float* scale);
+
+/* Matrix product of int8 operands with a scale for each row of either:
+ *   y[m, n] = float(sum over k of a[m, k] * w[n, k]) * a_scale[m] * w_scale[n] + bias[n]
+ * a [rows, k], w [n, k], exact int32 sums (k <= 131071, else TooLarge), then fp32 in the order written, one rounding to
+ * y_dtype (F32, F16 or BF16) at the end.  a_scale holds `rows` values, w_scale and bias `n`; bias may be NULL. */
+int32_t zant_b200_qmatmul_scaled(zant_ctx* ctx, const int8_t* a, size_t rows, size_t k, size_t a_stride, const float* a_scale,
+                                 const int8_t* w, size_t n, size_t w_stride, const float* w_scale, const float* bias,
+                                 int32_t y_dtype, void* y, size_t y_stride);
+
+/* The same product where groups of rows have weights of their own (the experts of a mixture): rows offsets[g] to
+ * offsets[g + 1] - 1 of a are multiplied with w[g].  w is [groups, n, k] (group g starts g * n * w_stride elements into it),
+ * w_scale and bias are [groups, n].  `offsets` holds groups + 1 int32 values (at most 1024 groups, else TooLarge); with a
+ * device pointer they are read on the device, when the kernel runs.  Rows that belong to no group are left as they were in y.
+ * Offsets do not decrease; what breaks that is not an error: values are taken as clamped to [0, rows], a group that ends
+ * before it begins is empty, and a row in several groups holds the result of one of them. */
+int32_t zant_b200_qmatmul_grouped(zant_ctx* ctx, const int8_t* a, size_t rows, size_t k, size_t a_stride, const float* a_scale,
+                                  const int8_t* w, size_t groups, size_t n, size_t w_stride, const float* w_scale, const float* bias,
+                                  const int32_t* offsets, int32_t y_dtype, void* y, size_t y_stride);
+
+/* What a model's logits [rows, vocab] (F32, F16 or BF16) say of given tokens, per row, in one pass over the logits; with
+ * p = softmax(logits):
+ *   logprob[r]  = log p[tokens[r]];  0 where tokens[r] is negative (padding), NaN where it is >= vocab
+ *   entropy[r]  = -sum over v of p[v] log p[v]
+ *   top_ids[r, i], top_logprobs[r, i], i < top: the i-th likeliest id (equal logits: the lower id first) and its log p
+ * Sums are fp32.  `tokens` and `logprob` may both be NULL, and so may `entropy`; top is 0 to 32 and at most vocab (else
+ * InvalidInput), with 0 top_ids and top_logprobs may be NULL.  Logits of minus infinity have log p of minus infinity and add
+ * nothing to the entropy; a row of nothing else has log p of minus infinity throughout and entropy 0.  A row with a NaN or
+ * plus infinity has NaN for every log p and the entropy; a NaN ranks before every number. */
+int32_t zant_b200_token_logprobs(zant_ctx* ctx, int32_t dtype, const void* logits, size_t rows, size_t vocab, size_t stride,
+                                 const int32_t* tokens, float* logprob, float* entropy,
+                                 int32_t top, int32_t* top_ids, float* top_logprobs);
 
 /* ------------------------------------------------------------------------------------------
  * Plan: the run-time form of a generated predict() (src/codeGen/predict.zig:23-70).  One

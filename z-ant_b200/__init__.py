@@ -22,6 +22,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libzant_b200.so")
 
 F32, I8, U8, I32 = 0, 1, 2, 3
+F16, BF16 = 4, 5        # quantize_rows, qmatmul_scaled, qmatmul_grouped and token_logprobs only
 NP_DTYPE = {F32: np.float32, I8: np.int8, U8: np.uint8, I32: np.int32}
 DTYPE_OF = {np.dtype(np.float32): F32, np.dtype(np.int8): I8, np.dtype(np.uint8): U8, np.dtype(np.int32): I32}
 AUTO_PAD = {"NOTSET": 0, "SAME_UPPER": 1, "SAME_LOWER": 2, "VALID": 3}
@@ -29,6 +30,7 @@ QACT = {None: 0, "none": 0, "relu": 1, "relu6": 2}
 COORD_MODE = {"half_pixel": 0, "align_corners": 1, "asymmetric": 2}
 SIZE_MAX = (1 << 64) - 1
 _TORCH_DTYPE = {}       # torch dtype -> code, filled when the first tensor is seen
+_ROW_DTYPE = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.int8): I8, np.dtype(np.int32): I32}     # the same with F16 and BF16; torch's too
 
 OP = dict(Conv=1, MatMul=2, Gemm=3, MaxPool=4, Relu=5, LeakyRelu=6, Add=7, Concat=8, Resize=9, ReduceMean=10,
           Reshape=11, Clip=12, Sigmoid=13, Softmax=14, Tanh=15, Ceil=16, Mul=17, Div=18, Transpose=19, Slice=27, Gather=28,
@@ -87,6 +89,8 @@ _SIGNATURES = {
     "sum_tensors_f32": "p ppz ppz ppz", "quantize_linear": "p p z f i i p", "dequantize_linear": "p i p z f i p",
     "qlinearconv": "p i ppz f i ppz pp z f i p z i ppz pz pz pz z i i", "qlinearconv_nhwc": "p i ppz f i ppz pp z f i p z i ppz pz pz pz z i i",
     "qlinearmatmul": "p i ppz f i ppz pp z f i p z i ppz i", "qlinearadd": "p i p f i p f i f i p z i", "plan_run": "p pp",
+    "quantize_rows": "p i pzzz pz pzp", "qmatmul_scaled": "p pzzzp pzzpp ipz", "qmatmul_grouped": "p pzzzp pzzzpp p ipz",
+    "token_logprobs": "p i pzzz ppp ipp",
 }
 _CTYPE = {"p": C.c_void_p, "z": C.c_size_t, "i": C.c_int32, "f": C.c_float}
 
@@ -191,6 +195,82 @@ def _dtype_code(a):
             _TORCH_DTYPE.update({torch.float32: F32, torch.int8: I8, torch.uint8: U8, torch.int32: I32})
         return _TORCH_DTYPE[a.dtype]
     return DTYPE_OF[a.dtype]
+
+
+def _row_code(dtype):
+    """Code of an element type of the row operators (numpy or torch), None for others."""
+    code = _ROW_DTYPE.get(dtype)
+    if code is None and not isinstance(dtype, np.dtype) and "torch" not in _ROW_DTYPE:
+        import torch
+        _ROW_DTYPE.update({"torch": -1, torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8, torch.int32: I32})
+        code = _ROW_DTYPE.get(dtype)
+    return code
+
+
+def _rows(a, what, rank=2):
+    """(array to keep, address, shape, distance between rows in elements, type code) of an operand of `rank` dimensions whose
+    last dimension is dense and whose leading ones follow each other in equal rows."""
+    if hasattr(a, "data_ptr"):
+        shape = a.shape
+        if len(shape) != rank:
+            raise ZantError(-59, "InvalidRank", f"{what} has {len(shape)} dimensions, not {rank}")
+        strides, ptr = a.stride(), a.data_ptr()
+    else:
+        a = np.asarray(a)
+        shape = a.shape
+        if len(shape) != rank:
+            raise ZantError(-59, "InvalidRank", f"{what} has {len(shape)} dimensions, not {rank}")
+        if not a.flags.c_contiguous:
+            a = np.ascontiguousarray(a)
+        strides = None
+        ptr = a.__array_interface__["data"][0]
+    code = _row_code(a.dtype)
+    if code is None:
+        raise ZantError(-34, "InputArrayWrongType", f"{what} is {a.dtype}")
+    cols = shape[-1]
+    if strides is None:
+        return a, ptr, shape, cols, code
+    row = strides[-2] if shape[-2] > 1 else cols
+    if (cols > 1 and strides[-1] != 1) or row < cols:
+        raise ZantError(-9, "WrongStride", f"{what} has strides {tuple(strides)}: rows must be dense and apart")
+    if rank == 3:
+        if shape[-2] == 1 and shape[0] > 1:
+            row = strides[0]
+        if row < cols or (shape[0] > 1 and strides[0] != shape[1] * row):
+            raise ZantError(-9, "WrongStride", f"{what} has strides {tuple(strides)}: its matrices must follow each other")
+    return a, ptr, shape, row, code
+
+
+def _values(a, n, code, what):
+    """(array to keep, address) of `n` dense values of type `code`; numpy arrays are cast."""
+    if hasattr(a, "data_ptr"):
+        if _row_code(a.dtype) != code:
+            raise ZantError(-34, "InputArrayWrongType", f"{what} is {a.dtype}")
+        if a.numel() != n:
+            raise ZantError(-35, "InputArrayWrongSize", f"{what} holds {a.numel()} values, not {n}")
+        if not a.is_contiguous():
+            raise ZantError(-9, "WrongStride", f"{what} is not dense")
+        return a, a.data_ptr()
+    a = np.ascontiguousarray(a, dtype=NP_DTYPE[code])
+    if a.size != n:
+        raise ZantError(-35, "InputArrayWrongSize", f"{what} holds {a.size} values, not {n}")
+    return a, a.__array_interface__["data"][0]
+
+
+def _result(a, n, code, what):
+    """The same for an output: numpy arrays must be what they are said to be."""
+    if not hasattr(a, "data_ptr") and (not isinstance(a, np.ndarray) or _row_code(a.dtype) != code or not a.flags.c_contiguous):
+        raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array of its type")
+    return _values(a, n, code, what)
+
+
+def _result_rows(a, rows, cols, what):
+    if not hasattr(a, "data_ptr") and (not isinstance(a, np.ndarray) or not a.flags.c_contiguous):
+        raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array")
+    a, ptr, shape, stride, code = _rows(a, what)
+    if shape[0] != rows or shape[1] != cols:
+        raise ZantError(-6, "OutputTensorDifferentSize", f"{what} is {tuple(shape)}, not {(rows, cols)}")
+    return ptr, stride, code
 
 
 def _shape_list(shapes):
@@ -724,6 +804,84 @@ class Context:
         check(lib().zant_b200_qlinear_global_avgpool(self._h, C.c_int32(dt), _ptr(x), xs, C.c_size_t(xr), C.c_float(x_scale),
                                                      C.c_int32(x_zp), C.c_float(y_scale), C.c_int32(y_zp), _ptr(y)))
         return y
+
+    # -- operators of language models (F32, F16 and BF16 rows, which may lie apart)
+    def quantize_rows(self, x, index=None, out=None, out_scale=None):
+        """int8 codes of the rows of x [rows, cols] and one scale for each: (q, scale), x ~ q * scale[:, None].  `index`
+        (int32) gathers: row r of the result is row index[r] of x, zeros where that is outside x."""
+        x, xp, (x_rows, cols), stride, code = _rows(x, "x")
+        rows, ip = x_rows, None
+        if index is not None:
+            rows = len(index)
+            index, ip = _values(index, rows, I32, "index")
+        if out is None:
+            out = np.zeros((rows, cols), np.int8)
+        if out_scale is None:
+            out_scale = np.zeros(rows, np.float32)
+        qp, q_stride, q_code = _result_rows(out, rows, cols, "out")
+        if q_code != I8:
+            raise ZantError(-34, "InputArrayWrongType", "codes are int8")
+        check(lib().zant_b200_quantize_rows(self._h, code, xp, x_rows, cols, stride, ip, rows, qp, q_stride, _result(out_scale, rows, F32, "out_scale")[1]))
+        return out, out_scale
+
+    def _scaled(self, a, a_scale, w, w_scale, bias, y_dtype, out, offsets):
+        a, ap, (rows, k), a_stride, a_code = _rows(a, "a")
+        w, wp, w_shape, w_stride, w_code = _rows(w, "w", 2 if offsets is None else 3)
+        if a_code != I8 or w_code != I8:
+            raise ZantError(-34, "InputArrayWrongType", "both operands are int8")
+        n = w_shape[-2]
+        if w_shape[-1] != k:
+            raise ZantError(-5, "InputTensorsWrongShape", f"a has rows of {k}, w of {w_shape[-1]}")
+        groups = 1 if offsets is None else w_shape[0]
+        a_scale, asp = _values(a_scale, rows, F32, "a_scale")
+        w_scale, wsp = _values(w_scale, groups * n, F32, "w_scale")
+        bp = None
+        if bias is not None:
+            bias, bp = _values(bias, groups * n, F32, "bias")
+        if out is None:
+            if y_dtype not in (F32, F16):
+                raise ZantError(-34, "InputArrayWrongType", "numpy results are F32 or F16: give `out`")
+            out = np.zeros((rows, n), np.float32 if y_dtype == F32 else np.float16)
+        yp, y_stride, y_code = _result_rows(out, rows, n, "out")
+        if offsets is None:
+            check(lib().zant_b200_qmatmul_scaled(self._h, ap, rows, k, a_stride, asp, wp, n, w_stride, wsp, bp, y_code, yp, y_stride))
+        else:
+            offsets, op = _values(offsets, groups + 1, I32, "offsets")
+            check(lib().zant_b200_qmatmul_grouped(self._h, ap, rows, k, a_stride, asp, wp, groups, n, w_stride, wsp, bp, op, y_code, yp, y_stride))
+        return out
+
+    def qmatmul_scaled(self, a, a_scale, w, w_scale, bias=None, y_dtype=F32, out=None):
+        """a [rows, k] int8 times w [n, k] int8, transposed: y[m, n] = sum * a_scale[m] * w_scale[n] + bias[n] in F32, F16 or
+        BF16 (the type of `out` where that is given)."""
+        return self._scaled(a, a_scale, w, w_scale, bias, y_dtype, out, None)
+
+    def qmatmul_grouped(self, a, a_scale, w, w_scale, offsets, bias=None, y_dtype=F32, out=None):
+        """The same with weights for each group of rows (experts): rows offsets[g] to offsets[g + 1] - 1 of a times w[g] of
+        [groups, n, k].  Rows in no group are left as they were in `out`."""
+        if offsets is None:
+            raise ZantError(-102, "NullPointer", "offsets")
+        return self._scaled(a, a_scale, w, w_scale, bias, y_dtype, out, offsets)
+
+    def token_logprobs(self, logits, tokens=None, top=0, out=None):
+        """(logprob, entropy, top_ids, top_logprobs) of logits [rows, vocab]: log probability of tokens[r] (int32; negative:
+        0), entropy of the row, the `top` likeliest ids and their log probabilities.  `out` takes the four arrays, with
+        logprob None where there are no tokens, and entropy None where it is not wanted."""
+        x, xp, (rows, vocab), stride, code = _rows(logits, "logits")
+        tp = None
+        if tokens is not None:
+            tokens, tp = _values(tokens, rows, I32, "tokens")
+        if out is None:
+            if not 0 <= top <= 32:
+                raise ZantError(-55, "InvalidInput", f"top {top}: 0 to 32")
+            out = (None if tokens is None else np.zeros(rows, np.float32), np.zeros(rows, np.float32), np.zeros((rows, top), np.int32), np.zeros((rows, top), np.float32))
+        logprob, entropy, ids, likely = out
+        if (logprob is None) != (tokens is None):
+            raise ZantError(-102, "NullPointer", "tokens and logprob come together")
+        check(lib().zant_b200_token_logprobs(self._h, code, xp, rows, vocab, stride, tp, None if logprob is None else _result(logprob, rows, F32, "logprob")[1],
+                                             None if entropy is None else _result(entropy, rows, F32, "entropy")[1], top,
+                                             _result(ids, rows * top, I32, "top_ids")[1] if top else None,
+                                             _result(likely, rows * top, F32, "top_logprobs")[1] if top else None))
+        return out
 
     def lut_q8(self, x, lut, out=None):
         x = _host(x); lut = np.ascontiguousarray(lut, np.uint8)

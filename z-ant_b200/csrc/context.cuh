@@ -272,6 +272,12 @@ class Stager {
 
     int in(const void* p, size_t bytes) { return add(p, nullptr, bytes, true); }
     int out(void* p, size_t bytes) { return add(nullptr, p, bytes, false); }
+    // An output of which the kernel may leave parts as they were.
+    int inout(void* p, size_t bytes) {
+        const int i = add(nullptr, p, bytes, false);
+        if (slots_[i].staged) slots_[i].host_in = p;
+        return i;
+    }
     // Weights: large ones in pageable memory go by the context's upload lane, between start_early and end_early of this call, if it has one and may
     // allocate; everything else as with `in`.  One per call.
     int in_early(const void* p, size_t bytes) {

@@ -4,3 +4,4 @@
 #include "plan.cu"
 #include "noalloc.cu"
 #include "multi.cu"
+#include "token_ops.cu"
