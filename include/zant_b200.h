@@ -596,8 +596,8 @@ int32_t zant_b200_qmatmul_scaled(zant_ctx* ctx, const int8_t* a, size_t rows, si
  * offsets[g + 1] - 1 of a are multiplied with w[g].  w is [groups, n, k] (group g starts g * n * w_stride elements into it),
  * w_scale and bias are [groups, n].  `offsets` holds groups + 1 int32 values (at most 1024 groups, else TooLarge); with a
  * device pointer they are read on the device, when the kernel runs.  Rows that belong to no group are left as they were in y.
- * Offsets do not decrease; what breaks that is not an error: values are taken as clamped to [0, rows], a group that ends
- * before it begins is empty, and a row in several groups holds the result of one of them. */
+ * Offsets do not decrease; what breaks that is not an error: each is taken as clamped to [0, rows] and as the largest of
+ * those up to it, so that a group which ends before it begins is empty and no row is in two. */
 int32_t zant_b200_qmatmul_grouped(zant_ctx* ctx, const int8_t* a, size_t rows, size_t k, size_t a_stride, const float* a_scale,
                                   const int8_t* w, size_t groups, size_t n, size_t w_stride, const float* w_scale, const float* bias,
                                   const int32_t* offsets, int32_t y_dtype, void* y, size_t y_stride);
