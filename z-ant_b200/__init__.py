@@ -197,80 +197,89 @@ def _dtype_code(a):
     return DTYPE_OF[a.dtype]
 
 
-def _row_code(dtype):
-    """Code of an element type of the row operators (numpy or torch), None for others."""
+def _row_code(dtype, what):
+    """Code of an element type of the row operators (numpy or torch)."""
     code = _ROW_DTYPE.get(dtype)
     if code is None and not isinstance(dtype, np.dtype) and "torch" not in _ROW_DTYPE:
         import torch
         _ROW_DTYPE.update({"torch": -1, torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8, torch.int32: I32})
         code = _ROW_DTYPE.get(dtype)
+    if code is None:
+        raise ZantError(-34, "InputArrayWrongType", f"{what} is {dtype}")
     return code
 
 
-def _rows(a, what, rank=2):
-    """(array to keep, address, shape, distance between rows in elements, type code) of an operand of `rank` dimensions whose
-    last dimension is dense and whose leading ones follow each other in equal rows."""
-    if hasattr(a, "data_ptr"):
-        shape = a.shape
-        if len(shape) != rank:
-            raise ZantError(-59, "InvalidRank", f"{what} has {len(shape)} dimensions, not {rank}")
-        strides, ptr = a.stride(), a.data_ptr()
-    else:
+def _strides_refused(what, strides):
+    return ZantError(-9, "WrongStride", f"{what} has strides {tuple(strides)}: rows must be dense and apart, matrices must follow each other")
+
+
+def _rows(a, what, result=False):
+    """(array to keep, address, rows, their length, distance between them in elements, type code) of a matrix whose rows are dense.
+    An array for a result must be dense itself (numpy) or have dense rows (tensors)."""
+    try:
+        ptr = a.data_ptr()
+    except AttributeError:
+        if result and (not isinstance(a, np.ndarray) or not a.flags.c_contiguous):
+            raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array") from None
         a = np.asarray(a)
-        shape = a.shape
-        if len(shape) != rank:
-            raise ZantError(-59, "InvalidRank", f"{what} has {len(shape)} dimensions, not {rank}")
+        if a.ndim != 2:
+            raise ZantError(-59, "InvalidRank", f"{what} has {a.ndim} dimensions, not 2") from None
         if not a.flags.c_contiguous:
             a = np.ascontiguousarray(a)
-        strides = None
-        ptr = a.__array_interface__["data"][0]
-    code = _row_code(a.dtype)
+        return a, a.__array_interface__["data"][0], a.shape[0], a.shape[1], a.shape[1], _row_code(a.dtype, what)
+    strides = a.stride()
+    if len(strides) != 2:
+        raise ZantError(-59, "InvalidRank", f"{what} has {len(strides)} dimensions, not 2")
+    row, col = strides
+    rows, cols = a.shape
+    code = _ROW_DTYPE.get(a.dtype)
     if code is None:
+        code = _row_code(a.dtype, what)
+    if rows <= 1:
+        row = cols
+    if row < cols or (col != 1 and cols > 1):
+        raise _strides_refused(what, strides)
+    return a, ptr, rows, cols, row, code
+
+
+def _matrices(a, what):
+    """(array to keep, address, matrices, rows, their length, distance between them in elements, type code) of matrices that follow each
+    other in equal rows."""
+    if not hasattr(a, "data_ptr"):
+        a = np.ascontiguousarray(a)
+        if a.ndim != 3:
+            raise ZantError(-59, "InvalidRank", f"{what} has {a.ndim} dimensions, not 3")
+        return (a, a.__array_interface__["data"][0]) + a.shape + (a.shape[2], _row_code(a.dtype, what))
+    strides = a.stride()
+    if len(strides) != 3:
+        raise ZantError(-59, "InvalidRank", f"{what} has {len(strides)} dimensions, not 3")
+    n, rows, cols = a.shape
+    row = strides[1]
+    if rows <= 1:
+        row = strides[0] if n > 1 else cols
+    if row < cols or (strides[2] != 1 and cols > 1) or (n > 1 and strides[0] != rows * row):
+        raise _strides_refused(what, strides)
+    return a, a.data_ptr(), n, rows, cols, row, _row_code(a.dtype, what)
+
+
+def _values(a, n, code, what, result=False):
+    """(array to keep, address) of `n` dense values of type `code`; numpy arrays are cast, those for a result must be what they are said to be."""
+    try:
+        ptr = a.data_ptr()
+    except AttributeError:
+        if result and (not isinstance(a, np.ndarray) or _ROW_DTYPE.get(a.dtype) != code or not a.flags.c_contiguous):
+            raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array of its type") from None
+        a = np.ascontiguousarray(a, dtype=NP_DTYPE[code])
+        if a.size != n:
+            raise ZantError(-35, "InputArrayWrongSize", f"{what} holds {a.size} values, not {n}") from None
+        return a, a.__array_interface__["data"][0]
+    if _ROW_DTYPE.get(a.dtype) != code and _row_code(a.dtype, what) != code:
         raise ZantError(-34, "InputArrayWrongType", f"{what} is {a.dtype}")
-    cols = shape[-1]
-    if strides is None:
-        return a, ptr, shape, cols, code
-    row = strides[-2] if shape[-2] > 1 else cols
-    if (cols > 1 and strides[-1] != 1) or row < cols:
-        raise ZantError(-9, "WrongStride", f"{what} has strides {tuple(strides)}: rows must be dense and apart")
-    if rank == 3:
-        if shape[-2] == 1 and shape[0] > 1:
-            row = strides[0]
-        if row < cols or (shape[0] > 1 and strides[0] != shape[1] * row):
-            raise ZantError(-9, "WrongStride", f"{what} has strides {tuple(strides)}: its matrices must follow each other")
-    return a, ptr, shape, row, code
-
-
-def _values(a, n, code, what):
-    """(array to keep, address) of `n` dense values of type `code`; numpy arrays are cast."""
-    if hasattr(a, "data_ptr"):
-        if _row_code(a.dtype) != code:
-            raise ZantError(-34, "InputArrayWrongType", f"{what} is {a.dtype}")
-        if a.numel() != n:
-            raise ZantError(-35, "InputArrayWrongSize", f"{what} holds {a.numel()} values, not {n}")
-        if not a.is_contiguous():
-            raise ZantError(-9, "WrongStride", f"{what} is not dense")
-        return a, a.data_ptr()
-    a = np.ascontiguousarray(a, dtype=NP_DTYPE[code])
-    if a.size != n:
-        raise ZantError(-35, "InputArrayWrongSize", f"{what} holds {a.size} values, not {n}")
-    return a, a.__array_interface__["data"][0]
-
-
-def _result(a, n, code, what):
-    """The same for an output: numpy arrays must be what they are said to be."""
-    if not hasattr(a, "data_ptr") and (not isinstance(a, np.ndarray) or _row_code(a.dtype) != code or not a.flags.c_contiguous):
-        raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array of its type")
-    return _values(a, n, code, what)
-
-
-def _result_rows(a, rows, cols, what):
-    if not hasattr(a, "data_ptr") and (not isinstance(a, np.ndarray) or not a.flags.c_contiguous):
-        raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array")
-    a, ptr, shape, stride, code = _rows(a, what)
-    if shape[0] != rows or shape[1] != cols:
-        raise ZantError(-6, "OutputTensorDifferentSize", f"{what} is {tuple(shape)}, not {(rows, cols)}")
-    return ptr, stride, code
+    if a.numel() != n:
+        raise ZantError(-35, "InputArrayWrongSize", f"{what} holds {a.numel()} values, not {n}")
+    if not a.is_contiguous():
+        raise ZantError(-9, "WrongStride", f"{what} is not dense")
+    return a, ptr
 
 
 def _shape_list(shapes):
@@ -809,7 +818,7 @@ class Context:
     def quantize_rows(self, x, index=None, out=None, out_scale=None):
         """int8 codes of the rows of x [rows, cols] and one scale for each: (q, scale), x ~ q * scale[:, None].  `index`
         (int32) gathers: row r of the result is row index[r] of x, zeros where that is outside x."""
-        x, xp, (x_rows, cols), stride, code = _rows(x, "x")
+        x, xp, x_rows, cols, stride, code = _rows(x, "x")
         rows, ip = x_rows, None
         if index is not None:
             rows = len(index)
@@ -818,31 +827,38 @@ class Context:
             out = np.zeros((rows, cols), np.int8)
         if out_scale is None:
             out_scale = np.zeros(rows, np.float32)
-        qp, q_stride, q_code = _result_rows(out, rows, cols, "out")
+        _, qp, q_rows, q_cols, q_stride, q_code = _rows(out, "out", True)
         if q_code != I8:
             raise ZantError(-34, "InputArrayWrongType", "codes are int8")
-        check(lib().zant_b200_quantize_rows(self._h, code, xp, x_rows, cols, stride, ip, rows, qp, q_stride, _result(out_scale, rows, F32, "out_scale")[1]))
+        if q_rows != rows or q_cols != cols:
+            raise ZantError(-6, "OutputTensorDifferentSize", f"out is {q_rows} x {q_cols}, not {rows} x {cols}")
+        check(lib().zant_b200_quantize_rows(self._h, code, xp, x_rows, cols, stride, ip, rows, qp, q_stride, _values(out_scale, rows, F32, "out_scale", True)[1]))
         return out, out_scale
 
     def _scaled(self, a, a_scale, w, w_scale, bias, y_dtype, out, offsets):
-        a, ap, (rows, k), a_stride, a_code = _rows(a, "a")
-        w, wp, w_shape, w_stride, w_code = _rows(w, "w", 2 if offsets is None else 3)
+        a, ap, rows, k, a_stride, a_code = _rows(a, "a")
+        if offsets is None:
+            w, wp, n, w_k, w_stride, w_code = _rows(w, "w")
+            groups, wide = 1, n
+        else:
+            w, wp, groups, n, w_k, w_stride, w_code = _matrices(w, "w")
+            wide = groups * n
         if a_code != I8 or w_code != I8:
             raise ZantError(-34, "InputArrayWrongType", "both operands are int8")
-        n = w_shape[-2]
-        if w_shape[-1] != k:
-            raise ZantError(-5, "InputTensorsWrongShape", f"a has rows of {k}, w of {w_shape[-1]}")
-        groups = 1 if offsets is None else w_shape[0]
+        if w_k != k:
+            raise ZantError(-5, "InputTensorsWrongShape", f"a has rows of {k}, w of {w_k}")
         a_scale, asp = _values(a_scale, rows, F32, "a_scale")
-        w_scale, wsp = _values(w_scale, groups * n, F32, "w_scale")
+        w_scale, wsp = _values(w_scale, wide, F32, "w_scale")
         bp = None
         if bias is not None:
-            bias, bp = _values(bias, groups * n, F32, "bias")
+            bias, bp = _values(bias, wide, F32, "bias")
         if out is None:
             if y_dtype not in (F32, F16):
                 raise ZantError(-34, "InputArrayWrongType", "numpy results are F32 or F16: give `out`")
             out = np.zeros((rows, n), np.float32 if y_dtype == F32 else np.float16)
-        yp, y_stride, y_code = _result_rows(out, rows, n, "out")
+        _, yp, y_rows, y_cols, y_stride, y_code = _rows(out, "out", True)
+        if y_rows != rows or y_cols != n:
+            raise ZantError(-6, "OutputTensorDifferentSize", f"out is {y_rows} x {y_cols}, not {rows} x {n}")
         if offsets is None:
             check(lib().zant_b200_qmatmul_scaled(self._h, ap, rows, k, a_stride, asp, wp, n, w_stride, wsp, bp, y_code, yp, y_stride))
         else:
@@ -866,7 +882,7 @@ class Context:
         """(logprob, entropy, top_ids, top_logprobs) of logits [rows, vocab]: log probability of tokens[r] (int32; negative:
         0), entropy of the row, the `top` likeliest ids and their log probabilities.  `out` takes the four arrays, with
         logprob None where there are no tokens, and entropy None where it is not wanted."""
-        x, xp, (rows, vocab), stride, code = _rows(logits, "logits")
+        x, xp, rows, vocab, stride, code = _rows(logits, "logits")
         tp = None
         if tokens is not None:
             tokens, tp = _values(tokens, rows, I32, "tokens")
@@ -877,10 +893,12 @@ class Context:
         logprob, entropy, ids, likely = out
         if (logprob is None) != (tokens is None):
             raise ZantError(-102, "NullPointer", "tokens and logprob come together")
-        check(lib().zant_b200_token_logprobs(self._h, code, xp, rows, vocab, stride, tp, None if logprob is None else _result(logprob, rows, F32, "logprob")[1],
-                                             None if entropy is None else _result(entropy, rows, F32, "entropy")[1], top,
-                                             _result(ids, rows * top, I32, "top_ids")[1] if top else None,
-                                             _result(likely, rows * top, F32, "top_logprobs")[1] if top else None))
+        lp = None if logprob is None else _values(logprob, rows, F32, "logprob", True)[1]
+        ep = None if entropy is None else _values(entropy, rows, F32, "entropy", True)[1]
+        idp = lkp = None
+        if top:
+            idp, lkp = _values(ids, rows * top, I32, "top_ids", True)[1], _values(likely, rows * top, F32, "top_logprobs", True)[1]
+        check(lib().zant_b200_token_logprobs(self._h, code, xp, rows, vocab, stride, tp, lp, ep, top, idp, lkp))
         return out
 
     def lut_q8(self, x, lut, out=None):

@@ -83,12 +83,6 @@ template <> struct Logits<__half> {
     }
 };
 
-// Two floats in a register pair: one instruction for both.
-__device__ __forceinline__ unsigned long long pack2(float a, float b) { unsigned long long r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ float2 unpack2(unsigned long long v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) { unsigned long long r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) { unsigned long long r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) { unsigned long long r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -229,7 +223,7 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
         const float top = L::max1(best);
         seen = fmaxf(seen, top);
         if (top > s.m) s.raise(top);
-        const unsigned long long minus_m = pack2(-s.m, -s.m), log2e = pack2(kLog2e, kLog2e);
+        const unsigned long long minus_m = ptx::pack2(-s.m, -s.m), log2e = ptx::pack2(kLog2e, kLog2e);
         unsigned long long S2 = 0, W2 = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -239,14 +233,14 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
                 float2 p;
                 if constexpr (N == 8) p = L::pair(L::floored2(w[k]));
                 else p = make_float2(L::floored(w[2 * k]), L::floored(w[2 * k + 1]));
-                const unsigned long long d = add2(pack2(p.x, p.y), minus_m);
-                const float2 t = unpack2(mul2(d, log2e));
-                const unsigned long long e = pack2(ex2(t.x), ex2(t.y));
-                S2 = add2(S2, e);
-                W2 = fma2(e, d, W2);
+                const unsigned long long d = ptx::add2(ptx::pack2(p.x, p.y), minus_m);
+                const float2 t = ptx::unpack2(ptx::mul2(d, log2e));
+                const unsigned long long e = ptx::pack2(ex2(t.x), ex2(t.y));
+                S2 = ptx::add2(S2, e);
+                W2 = ptx::fma2(e, d, W2);
             }
         }
-        const float2 S = unpack2(S2), W = unpack2(W2);
+        const float2 S = ptx::unpack2(S2), W = ptx::unpack2(W2);
         s.S += S.x + S.y;
         s.W += W.x + W.y;
     }
