@@ -2,14 +2,16 @@
 //   m = max x, S = sum exp(x - m), W = sum (x - m) exp(x - m):   log p(t) = x_t - m - log S,   entropy = log S - W / S
 //
 // One pass over the logits.  A thread keeps its own maximum, S and W, four 16-byte vectors at a time, and rescales when a batch raises its
-// maximum; the parts are joined at the end.  Logits of minus infinity are taken as a lowest value that no other term sees (a product of
-// zero and infinity would spoil W); rows for which that is not so (their maximum is about as low), and rows with a NaN or plus
-// infinity, go through a plain second form, one pass a result.
+// maximum; the parts are joined at the end.  Everything is in units of log 2: d = x log2(e) - m log2(e) is one fused operation for two
+// logits, and the rounding of m log2(e), which all terms of a sum share, cancels in log p and the entropy because the token's own d is
+// taken the same way.  Logits of minus infinity are taken as a lowest value that no other term sees (a product of zero and infinity would
+// spoil W); rows for which that is not so (their maximum is about as low), rows about as large as their type can be, and rows with a NaN
+// or plus infinity go through a plain second form, one pass a result.
 //
 // The alternatives: tau, the n-th largest of the threads' maxima, is a lower bound of the n-th largest logit, and only threads whose maximum
-// reaches it have seen a logit that does.  About n threads do; their vectors (V / 512 logits each) are read again, from L2, what reaches tau
-// is collected, and each candidate's rank among them is its place in the result.  Equal logits rank by id; where hundreds of them equal
-// tau (a mask that leaves fewer than n tokens), the row is read from its start for the lowest ids.
+// reaches it have seen a logit that does.  About n threads do; their vectors (V / threads logits each) are read again, from L2, what
+// reaches tau is collected, and each candidate's rank among them is its place in the result.  Equal logits rank by id; where hundreds of
+// them equal tau (a mask that leaves fewer than n tokens), the row is read from its start for the lowest ids.
 //
 // Few rows: a cluster of 2, 4 or 8 CTAs shares a row; the first joins the sums and the lists, which come by distributed shared memory.
 #pragma once
@@ -43,11 +45,11 @@ __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_flo
 __device__ __forceinline__ unsigned long long key_of(uint32_t order, int id) { return ((unsigned long long)order << 32) | (uint32_t)~id; }
 
 // 16 bytes of logits.  LOW: bits of a float that its values leave 0; FLOOR: what stands for minus infinity; LEAST: a maximum that FLOOR is
-// far enough below to add nothing.
+// far enough below to add nothing; MOST: one whose product with log2(e) is finite.
 template <typename T> struct Logits;
 template <> struct Logits<float> {
     static constexpr int N = 4, LOW = 0;
-    static constexpr float FLOOR = -1e30f, LEAST = -0.9e30f;
+    static constexpr float FLOOR = -1e30f, LEAST = -0.9e30f, MOST = 1e38f;
     static constexpr uint32_t NONE = 0xff800000u;
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
     static __device__ __forceinline__ float max1(uint32_t a) { return __uint_as_float(a); }
@@ -56,7 +58,7 @@ template <> struct Logits<float> {
 };
 template <> struct Logits<__nv_bfloat16> {
     static constexpr int N = 8, LOW = 16;
-    static constexpr float FLOOR = -1e30f, LEAST = -0.9e30f;
+    static constexpr float FLOOR = -1e30f, LEAST = -0.9e30f, MOST = 1e38f;
     static constexpr uint32_t NONE = 0xff80ff80u, FLOOR2 = 0xf14af14au;       // -1.0002e30
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t r; asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
     static __device__ __forceinline__ uint32_t floored2(uint32_t a) { uint32_t r; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(FLOOR2)); return r; }
@@ -70,7 +72,7 @@ template <> struct Logits<__nv_bfloat16> {
 };
 template <> struct Logits<__half> {
     static constexpr int N = 8, LOW = 13;
-    static constexpr float FLOOR = -65504.0f, LEAST = -65304.0f;
+    static constexpr float FLOOR = -65504.0f, LEAST = -65304.0f, MOST = INFINITY;
     static constexpr uint32_t NONE = 0xfc00fc00u, FLOOR2 = 0xfbfffbffu;
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t r; asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
     static __device__ __forceinline__ uint32_t floored2(uint32_t a) { uint32_t r; asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(FLOOR2)); return r; }
@@ -84,35 +86,40 @@ template <> struct Logits<__half> {
 };
 
 __device__ __forceinline__ float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// m, S and W of what a thread has seen.
+// m log2(e), S and W (in log 2) of what a thread has seen.
 struct ExpSums {
     float m, S, W;
     // To a greater maximum.
     __device__ __forceinline__ void raise(float to) {
-        const float d = m - to, f = ex2(d * kLog2e);
+        const float d = m - to, f = ex2(d);
         W = f > 0.0f ? (W + S * d) * f : 0.0f;         // (d may be so great that S d is infinite)
         S *= f;
         m = to;
     }
-    __device__ __forceinline__ void join(ExpSums o) {
-        const float to = fmaxf(m, o.m);
-        raise(to); o.raise(to);
-        S += o.S; W += o.W;
+    // The sums of a warp's lanes, in every lane.
+    __device__ __forceinline__ void join_lanes(int lanes) {
+        float top = m;
+        for (int d = lanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        raise(top);
+        for (int d = lanes / 2; d; d >>= 1) { S += __shfl_xor_sync(0xffffffffu, S, d); W += __shfl_xor_sync(0xffffffffu, W, d); }
     }
 };
 
+template <int T>
 struct TokenLogprobsShared {
-    static constexpr int THREADS = 512, WARPS = THREADS / 32, CAP = 1024;
+    static constexpr int THREADS = T, WARPS = THREADS / 32, CAP = 1024;
     ExpSums sums[WARPS];
     float top[WARPS];
+    uint32_t seen[THREADS];                            // the threads' maxima, as orders (0: none)
     unsigned long long over[CAP], equal[CAP];          // candidates above tau and at it
     unsigned long long lists[8][kTopMax];              // of the CTAs of a row, in the first of them
     ExpSums part_sums[8];
     float part_top[8];
     int part_odd[8];
     short seen_by[THREADS];
+    uint32_t tau;
     int n_seen, n_over, n_equal, odd;
     unsigned long long key_part[WARPS];
     float part[WARPS];
@@ -131,8 +138,8 @@ __device__ __forceinline__ V block_reduce(V v, V* part, F f) {
 }
 
 // The plain form, one CTA, a pass for the maximum, one for the sums and one for each alternative.
-template <typename T>
-__device__ __noinline__ void token_logprobs_plain(const TokenLogprobsArgs& a, long long r, TokenLogprobsShared& sh) {
+template <typename T, typename Sh>
+__device__ __noinline__ void token_logprobs_plain(const TokenLogprobsArgs& a, long long r, Sh& sh) {
     const T* x = static_cast<const T*>(a.x) + r * a.stride;
     const int step = blockDim.x;
     float m = -INFINITY;
@@ -184,16 +191,38 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* a, int na, c
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprobs_kernel(const TokenLogprobsArgs a) {
+// tau of a warp that holds R maxima a lane: the largest value that `top` of all reach, in the bits that values have (0: fewer than `top` threads
+// have seen a logit).  Bit by bit below what the largest and the least of them have in common.
+template <int R, int LOW>
+__device__ __forceinline__ uint32_t nth_largest(const uint32_t (&v)[R], int top) {
+    uint32_t hi = v[0], lo = v[0];
+#pragma unroll
+    for (int i = 1; i < R; ++i) { hi = max(hi, v[i]); lo = min(lo, v[i]); }
+    hi = __reduce_max_sync(0xffffffffu, hi); lo = __reduce_min_sync(0xffffffffu, lo);
+    if (top == 1) return hi;
+    if (hi == lo) return lo;
+    const int first = 31 - __clz(hi ^ lo);
+    uint32_t tau = first == 31 ? 0u : hi & ~((2u << first) - 1u);
+    for (int bit = first; bit >= LOW; --bit) {
+        const uint32_t at = tau | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) n += v[i] >= at;
+        if ((int)__reduce_add_sync(0xffffffffu, (unsigned)n) >= top) tau = at;
+    }
+    return tau;
+}
+
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const TokenLogprobsArgs a) {
     using L = Logits<T>;
-    using Sh = TokenLogprobsShared;
-    constexpr int THREADS = Sh::THREADS, U = 4, N = L::N;
+    using Sh = TokenLogprobsShared<THREADS>;
+    constexpr int U = 4, N = L::N;
     __shared__ Sh sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, P = a.parts;
     const int part = P > 1 ? (int)ptx::cluster_rank() : 0;
     const long long r = (long long)blockIdx.x / P;
-    if (tid == 0) { sh.n_seen = sh.n_over = sh.n_equal = 0; sh.odd = 0; }
+    if (tid == 0) sh.n_seen = sh.n_over = sh.n_equal = 0;
     if (P > 1) ptx::cluster_arrive();                 // its shared memory may be written to
     ptx::grid_start();
     const T* row = static_cast<const T*>(a.x) + r * a.stride;
@@ -211,7 +240,8 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
         if (token >= 0 && token < a.vocab) given = as_float(row[token]);
     }
 
-    ExpSums s{L::FLOOR, 0.0f, 0.0f};
+    ExpSums s{L::FLOOR * kLog2e, 0.0f, 0.0f};
+    float m = L::FLOOR;
     float seen = -INFINITY;                           // the largest of the thread's vectors
     for (int i = tid; i < nv; i += THREADS * U) {
         uint4 v[U];
@@ -222,7 +252,7 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
         for (int u = 1; u < U; ++u) best = L::max2(best, L::max2(L::max2(v[u].x, v[u].y), L::max2(v[u].z, v[u].w)));
         const float top = L::max1(best);
         seen = fmaxf(seen, top);
-        if (top > s.m) s.raise(top);
+        if (top > m) { m = top; s.raise(m * kLog2e); }
         const unsigned long long minus_m = ptx::pack2(-s.m, -s.m), log2e = ptx::pack2(kLog2e, kLog2e);
         unsigned long long S2 = 0, W2 = 0;
 #pragma unroll
@@ -233,8 +263,8 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
                 float2 p;
                 if constexpr (N == 8) p = L::pair(L::floored2(w[k]));
                 else p = make_float2(L::floored(w[2 * k]), L::floored(w[2 * k + 1]));
-                const unsigned long long d = ptx::add2(ptx::pack2(p.x, p.y), minus_m);
-                const float2 t = ptx::unpack2(ptx::mul2(d, log2e));
+                const unsigned long long d = ptx::fma2(ptx::pack2(p.x, p.y), log2e, minus_m);
+                const float2 t = ptx::unpack2(d);
                 const unsigned long long e = ptx::pack2(ex2(t.x), ex2(t.y));
                 S2 = ptx::add2(S2, e);
                 W2 = ptx::fma2(e, d, W2);
@@ -249,8 +279,8 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
         float v = as_float(x[single_at(tid)]);
         highest = fmaxf(highest, v);
         if (v != v || v > L::FLOOR) {
-            if (v > s.m) s.raise(v);
-            const float d = v - s.m, e = ex2(d * kLog2e);
+            if (v > m) s.raise(v * kLog2e);
+            const float d = fmaf(v, kLog2e, -s.m), e = ex2(d);
             s.S += e;
             s.W += e * d;
         }
@@ -258,21 +288,34 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
 
     // one S and W for the CTA
     ExpSums c = s;
+    c.join_lanes(32);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, d));
-        c.join(ExpSums{__shfl_xor_sync(0xffffffffu, c.m, d), __shfl_xor_sync(0xffffffffu, c.S, d), __shfl_xor_sync(0xffffffffu, c.W, d)});
-    }
+    for (int d = 16; d; d >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, d));
     if (lane == 0) { sh.sums[warp] = c; sh.top[warp] = highest; }
+    const uint32_t mine = tid < nv ? order_of(seen) : 0u;
+    if (a.top > 0) sh.seen[tid] = mine;
+    __syncthreads();
+    if (warp == 0) {
+        const bool in = lane < Sh::WARPS;
+        ExpSums t = in ? sh.sums[lane] : ExpSums{L::FLOOR * kLog2e, 0.0f, 0.0f};
+        float h = in ? sh.top[lane] : -INFINITY;
+        t.join_lanes(Sh::WARPS);
+#pragma unroll
+        for (int d = Sh::WARPS / 2; d; d >>= 1) h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, d));
+        if (lane == 0) { sh.part_sums[part] = t; sh.part_top[part] = h; sh.part_odd[part] = 0; }
+        if (a.top > 0) {
+            uint32_t v[Sh::WARPS];
+#pragma unroll
+            for (int i = 0; i < Sh::WARPS; ++i) v[i] = sh.seen[i * 32 + lane];
+            uint32_t tau = nth_largest<Sh::WARPS, L::LOW>(v, a.top);
+            if (L::LOW && !(tau & 0x80000000u)) tau |= (1u << L::LOW) - 1u;      // of negative numbers these bits are set
+            if (lane == 0) sh.tau = tau;
+        }
+    }
     __syncthreads();
 
     if (a.top > 0) {
-        // tau: the largest value that `top` threads reach (0: every logit does)
-        const uint32_t mine = tid < nv ? order_of(seen) : 0u;
-        uint32_t tau = 0;
-        for (int bit = 31; bit >= L::LOW; --bit)
-            if (__syncthreads_count(mine >= (tau | (1u << bit))) >= a.top) tau |= 1u << bit;
-        if (L::LOW && !(tau & 0x80000000u)) tau |= (1u << L::LOW) - 1u;          // of negative numbers these bits are set
+        const uint32_t tau = sh.tau;
         auto offer = [&](float v, int id) {
             const uint32_t o = order_of(v);
             if (o < tau) return;
@@ -295,7 +338,7 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
         __syncthreads();
         const int n_over = sh.n_over;
         int n_equal = sh.n_equal;
-        if (n_over > Sh::CAP) { if (tid == 0) sh.odd = 1; }
+        if (n_over > Sh::CAP) { if (tid == 0) sh.part_odd[part] = 1; }
         else {
             if (n_over >= a.top) n_equal = 0;
             else if (n_equal > Sh::CAP - THREADS) {    // the lowest ids among them
@@ -315,18 +358,7 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
         __syncthreads();
     }
 
-    if (warp == 0) {
-        ExpSums t = lane < Sh::WARPS ? sh.sums[lane] : ExpSums{L::FLOOR, 0.0f, 0.0f};
-        float h = lane < Sh::WARPS ? sh.top[lane] : -INFINITY;
-#pragma unroll
-        for (int d = 8; d; d >>= 1) {
-            h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, d));
-            t.join(ExpSums{__shfl_xor_sync(0xffffffffu, t.m, d), __shfl_xor_sync(0xffffffffu, t.S, d), __shfl_xor_sync(0xffffffffu, t.W, d)});
-        }
-        if (lane == 0) { sh.part_sums[part] = t; sh.part_top[part] = h; sh.part_odd[part] = sh.odd; }
-    }
     if (P > 1) {
-        __syncthreads();
         ptx::cluster_wait();                          // the first CTA has started
         auto send = [&](const void* p) { ptx::st_cluster_u32(ptx::cluster_addr(ptx::smem_u32(p), 0), *static_cast<const uint32_t*>(p)); };
         if (part > 0) {
@@ -347,34 +379,53 @@ __global__ void __launch_bounds__(TokenLogprobsShared::THREADS, 2) token_logprob
     ExpSums t = sh.part_sums[0];
     float h = sh.part_top[0];
     int odd = sh.part_odd[0];
-    for (int i = 1; i < P; ++i) { t.join(sh.part_sums[i]); h = fmaxf(h, sh.part_top[i]); odd |= sh.part_odd[i]; }
-    const bool plain = odd || !(t.S < INFINITY) || !(h > L::LEAST);
-    if (plain) { token_logprobs_plain<T>(a, r, sh); return; }
-    const float ls = logf(t.S);
+    for (int i = 1; i < P; ++i) {
+        ExpSums o = sh.part_sums[i];
+        const float to = fmaxf(t.m, o.m);
+        t.raise(to); o.raise(to);
+        t.S += o.S; t.W += o.W;
+        h = fmaxf(h, sh.part_top[i]);
+        odd |= sh.part_odd[i];
+    }
+    if (odd || !(t.S < INFINITY) || !(h > L::LEAST) || !(h < L::MOST)) { token_logprobs_plain<T>(a, r, sh); return; }
+    const float ls = log2f(t.S);
+    auto logp = [&](float v) {
+        const float p = (fmaf(v, kLog2e, -t.m) - ls) * kLn2;
+        return p > -INFINITY ? p : v - t.m * kLn2;    // (about the lowest value of the type: its product with log2(e) is infinite)
+    };
     if (tid == 0) {
-        if (a.logprob) a.logprob[r] = token < 0 ? 0.0f : (token >= a.vocab ? __uint_as_float(0x7fffffffu) : given - t.m - ls);
-        if (a.entropy) a.entropy[r] = ls - t.W / t.S;
+        if (a.logprob) a.logprob[r] = token < 0 ? 0.0f : (token >= a.vocab ? __uint_as_float(0x7fffffffu) : logp(given));
+        if (a.entropy) a.entropy[r] = (ls - t.W / t.S) * kLn2;
     }
     if (tid < a.top) {
         const unsigned long long k = sh.lists[0][tid];
         a.top_ids[r * a.top + tid] = (int)~(uint32_t)k;
-        a.top_logprobs[r * a.top + tid] = value_of((uint32_t)(k >> 32)) - t.m - ls;
+        a.top_logprobs[r * a.top + tid] = logp(value_of((uint32_t)(k >> 32)));
     }
 }
 
-inline int32_t run_token_logprobs(zant_ctx* ctx, int32_t dtype, TokenLogprobsArgs a) {
-    // Two CTAs fit an SM.  A row is shared while that leaves nobody idle and each part has a batch of vectors for every thread.
-    const int batch = TokenLogprobsShared::THREADS * (dtype == ZANT_F32 ? 4 : 8);
-    a.parts = 1;
-    while (a.parts < 8 && a.rows * a.parts * 2 <= 2LL * ctx->sm_count && a.vocab / (a.parts * 2) >= batch) a.parts *= 2;
-    const dim3 grid((unsigned)(a.rows * a.parts));
+template <int THREADS>
+inline int32_t launch_token_logprobs(zant_ctx* ctx, int32_t dtype, TokenLogprobsArgs a, int parts) {
+    a.parts = parts;
     auto go = [&](auto kernel) {
-        launch_cluster(ctx, kernel, grid, TokenLogprobsShared::THREADS, 0, (unsigned)a.parts, a);
+        launch_cluster(ctx, kernel, dim3((unsigned)(a.rows * parts)), THREADS, 0, (unsigned)parts, a);
         return check_launch(ctx, "token_logprobs_kernel");
     };
-    if (dtype == ZANT_F32) return go(token_logprobs_kernel<float>);
-    if (dtype == ZANT_F16) return go(token_logprobs_kernel<__half>);
-    return go(token_logprobs_kernel<__nv_bfloat16>);
+    if (dtype == ZANT_F32) return go(token_logprobs_kernel<float, THREADS>);
+    if (dtype == ZANT_F16) return go(token_logprobs_kernel<__half, THREADS>);
+    return go(token_logprobs_kernel<__nv_bfloat16, THREADS>);
+}
+
+inline int32_t run_token_logprobs(zant_ctx* ctx, int32_t dtype, const TokenLogprobsArgs& a) {
+    const int vectors = a.vocab / (dtype == ZANT_F32 ? 4 : 8);
+    // Many rows: small CTAs, whose ends (about 3 us after the last logit) overlap with other rows (1000 x 5000 bf16: 8.8, 13.0, 25.5 us with
+    // 128, 256, 512 threads), but not so small that tau lets much through (4096 x 65536, 20 alternatives: 158, 134, 160).
+    if (a.rows > 2LL * ctx->sm_count) return vectors <= 4096 ? launch_token_logprobs<128>(ctx, dtype, a, 1) : launch_token_logprobs<256>(ctx, dtype, a, 1);
+    // Few rows: two large CTAs an SM; a row is shared while that leaves nobody idle and a thread has 7 vectors (64 x 128000 bf16: 17.6, 14.1,
+    // 12.6, 25.6 us with 1, 2, 4, 8 CTAs a row; 64 x 32000: 5.3, 5.6, 7.1).
+    int parts = 1;
+    while (parts < 8 && a.rows * parts * 2 <= 2LL * ctx->sm_count && vectors / (parts * 2) >= 7 * 512) parts *= 2;
+    return launch_token_logprobs<512>(ctx, dtype, a, parts);
 }
 
 }  // namespace zb
