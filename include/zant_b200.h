@@ -566,9 +566,12 @@ int32_t zant_b200_lut_q8(zant_ctx* ctx, const void* x, const uint8_t lut[256], v
  * They differ from the operators above in three points: F16 and BF16 take part, rows may lie further apart than they are
  * long, and a call with no rows does nothing.
  *   - *_stride is the distance between rows in elements, 0 for dense rows; less than a row is WrongStride.
- *   - Device pointers must be aligned to their element (InvalidInput).  Rows of int8 operands that start at multiples of 16
- *     bytes (pointer and stride) are read by the tensor memory accelerator; others take a slower kernel, same results.
- *   - All calls with device pointers may be captured into a CUDA graph; they use no workspace.
+ *   - Device pointers must be aligned to their element (InvalidInput).  Any other address will do; rows of int8 operands
+ *     that start at multiples of 16 bytes (pointer and stride) are read by the tensor memory accelerator, and a program that
+ *     can choose lays its weights and codes out like that: products of more than 32 tokens with other rows take about twice
+ *     as long.
+ *   - Calls with device pointers may be captured into a CUDA graph.  Outside a capture, products whose operands' rows start
+ *     at other addresses lay them out in the context's arena first, if it is large enough as it is.
  *   - Arrays of a call must not overlap its outputs.
  * ---------------------------------------------------------------------------------------- */
 

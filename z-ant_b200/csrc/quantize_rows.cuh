@@ -193,7 +193,7 @@ __device__ __forceinline__ void row_chunk(const char* row, int sh, I bytes, I at
 #pragma unroll
         for (int i = 0; i < 5; ++i) e[i] = (sh & 4) ? e[i + 1] : e[i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = sizeof(T) == 2 ? __funnelshift_r(e[i], e[i + 1], (sh & 2) * 8) : e[i];
+        for (int i = 0; i < 4; ++i) e[i] = sizeof(T) < 4 ? __funnelshift_r(e[i], e[i + 1], (sh & 3) * 8) : e[i];
         cur = make_uint4(e[0], e[1], e[2], e[3]);
     }
     if (left < 16 && left + (SHIFT ? sh : 0) > 0) cur = first_bytes(cur, (int)left);
