@@ -81,7 +81,7 @@ class NodeAttrs(C.Structure):
 
 # Argument types of the entry points that are called per operator or per pass: with them ctypes converts Python integers and
 # addresses itself (a conv call spent half of its 9 us on the host wrapping 22 arguments one by one).
-# p pointer, z size_t, i int32, f float.
+# p pointer, z size_t, i int32, f float; n: a size_t that is not negative, converted as a pointer (a third of the time).
 _SIGNATURES = {
     "conv_f32": "p ppz ppz pz ppz pz pz pz z pz", "mat_mul_f32": "p ppz ppz ppz", "gemm_lean_f32": "p ppz ppz ppz ffii ppz", "gemm_f32": "p ppz ppz ppz ffii ppz",
     "maxpool_f32": "p ppz ppz pz pz pz pz i", "maxpool_q8": "p i ppz ppz pz pz pz pz i", "relu_f32": "p pp z", "leaky_relu_f32": "p p f p z",
@@ -89,10 +89,10 @@ _SIGNATURES = {
     "sum_tensors_f32": "p ppz ppz ppz", "quantize_linear": "p p z f i i p", "dequantize_linear": "p i p z f i p",
     "qlinearconv": "p i ppz f i ppz pp z f i p z i ppz pz pz pz z i i", "qlinearconv_nhwc": "p i ppz f i ppz pp z f i p z i ppz pz pz pz z i i",
     "qlinearmatmul": "p i ppz f i ppz pp z f i p z i ppz i", "qlinearadd": "p i p f i p f i f i p z i", "plan_run": "p pp",
-    "quantize_rows": "p i pzzz pz pzp", "qmatmul_scaled": "p pzzzp pzzpp ipz", "qmatmul_grouped": "p pzzzp pzzzpp p ipz",
-    "token_logprobs": "p i pzzz ppp ipp",
+    "quantize_rows": "p i pnnn pn pnp", "qmatmul_scaled": "p pnnnp pnnpp ipn", "qmatmul_grouped": "p pnnnp pnnnpp p ipn",
+    "token_logprobs": "p i pnnn ppp ipp",
 }
-_CTYPE = {"p": C.c_void_p, "z": C.c_size_t, "i": C.c_int32, "f": C.c_float}
+_CTYPE = {"p": C.c_void_p, "z": C.c_size_t, "i": C.c_int32, "f": C.c_float, "n": C.c_void_p}
 
 _lib = None
 

@@ -261,7 +261,7 @@ struct UploadLane {
 // declared (plan phase) before the first is materialised so the arena can grow once.
 class Stager {
   public:
-    explicit Stager(zant_ctx* c) : ctx_(c) {}
+    explicit Stager(zant_ctx* c) : ctx_(c) { slots_.reserve(12); }
     ~Stager() {
         if (!ctx_) return;
         if (early_ == 2) end_early();

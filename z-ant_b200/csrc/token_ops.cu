@@ -65,17 +65,14 @@ inline int32_t scaled_gemm_entry(zant_ctx* ctx, const int8_t* a, size_t rows, si
     ScaledGemmArgs p{};
     p.a = a; p.a_stride = (long long)a_stride; p.w = w; p.w_stride = (long long)w_stride; p.y_stride = (long long)y_stride;
     p.rows = (int)rows; p.n = (int)n; p.k = (int)k; p.groups = (int)groups;
-    // Rows that the TMA cannot read are laid out in the arena, if it holds them as it is and the call is not captured.  (Host rows
-    // are staged at a multiple of 256 bytes.)
-    if (!is_device_ptr(a)) p.a = nullptr;
-    if (!is_device_ptr(w)) p.w = nullptr;
-    const size_t align_a = scaled_align_bytes(p, false), align_w = scaled_align_bytes(p, true);
-    const bool lay_out = (align_a || align_w) && !stream_capturing(ctx) && align_a + align_w + 2 * kArenaAlign <= ctx->arena_bytes && p.a && p.w;
+    // Device rows that the TMA cannot read are laid out in the arena, if it holds them as it is and the call is not captured.
+    size_t align_a = scaled_align_bytes(p, false), align_w = scaled_align_bytes(p, true);
+    if ((align_a || align_w) && (align_a + align_w + 2 * kArenaAlign > ctx->arena_bytes || stream_capturing(ctx) || !is_device_ptr(a) || !is_device_ptr(w))) align_a = align_w = 0;
     Stager s(ctx);
     const int ia = s.in(a, a_bytes), ias = s.in(a_scale, rows * 4), iw = s.in(w, w_bytes), iws = s.in(w_scale, groups * n * 4), ib = s.in(bias, groups * n * 4);
     const int io = s.in(grouped ? offsets : nullptr, (groups + 1) * 4);
     const int iy = grouped || y_stride != n ? s.inout(y, y_bytes) : s.out(y, y_bytes);
-    const int ila = lay_out && align_a ? s.scratch(align_a) : -1, ilw = lay_out && align_w ? s.scratch(align_w) : -1;
+    const int ila = align_a ? s.scratch(align_a) : -1, ilw = align_w ? s.scratch(align_w) : -1;
     ZB_TRY(s.commit());
     p.a = s.ptr<int8_t>(ia); p.a_scale = s.ptr<float>(ias); p.w = s.ptr<int8_t>(iw); p.w_scale = s.ptr<float>(iws);
     p.bias = s.ptr<float>(ib); p.y = s.ptr<void>(iy); p.offsets = s.ptr<int32_t>(io);

@@ -468,3 +468,61 @@ pub fn qlinear_activation_lean(comptime T: type, input: *Tensor(T), x_scale: f32
     }
     try check(zant_b200_lut_q8(context(), input.data.ptr, &lut, output.data.ptr, input.size));
 }
+
+// ------------------------------------------------------------------------------------------
+// Operators of language models: activations quantized as they come, one scale for each row.  No reference counterpart;
+// zant_b200.h states them.  Rows are dense here, elements f32 or f16.
+// ------------------------------------------------------------------------------------------
+extern fn zant_b200_quantize_rows(ctx: ?*Ctx, x_dtype: i32, x: *const anyopaque, x_rows: usize, cols: usize, x_stride: usize, index: ?[*]const i32, rows: usize, q: [*]i8, q_stride: usize, scale: [*]f32) i32;
+extern fn zant_b200_qmatmul_scaled(ctx: ?*Ctx, a: [*]const i8, rows: usize, k: usize, a_stride: usize, a_scale: [*]const f32, w: [*]const i8, n: usize, w_stride: usize, w_scale: [*]const f32, bias: ?[*]const f32, y_dtype: i32, y: *anyopaque, y_stride: usize) i32;
+extern fn zant_b200_qmatmul_grouped(ctx: ?*Ctx, a: [*]const i8, rows: usize, k: usize, a_stride: usize, a_scale: [*]const f32, w: [*]const i8, groups: usize, n: usize, w_stride: usize, w_scale: [*]const f32, bias: ?[*]const f32, offsets: [*]const i32, y_dtype: i32, y: *anyopaque, y_stride: usize) i32;
+extern fn zant_b200_token_logprobs(ctx: ?*Ctx, dtype: i32, logits: *const anyopaque, rows: usize, vocab: usize, stride: usize, tokens: ?[*]const i32, logprob: ?[*]f32, entropy: ?[*]f32, top: i32, top_ids: ?[*]i32, top_logprobs: ?[*]f32) i32;
+
+fn rowTypeOf(comptime T: type) i32 {
+    return switch (T) {
+        f32 => 0,
+        f16 => 4,
+        else => @compileError("zant_b200: rows are f32 or f16"),
+    };
+}
+
+/// x [rows, cols] (or the rows that `index` names) -> codes q and one scale for each row.
+pub fn quantize_rows_lean(comptime T: type, x: *const Tensor(T), index: ?*const Tensor(i32), q: *Tensor(i8), scale: *Tensor(f32)) !void {
+    if (x.shape.len != 2 or q.shape.len != 2) return TensorError.InvalidRank;
+    if (q.shape[1] != x.shape[1] or scale.size != q.shape[0]) return TensorMathError.OutputTensorDifferentSize;
+    if (index) |i| if (i.size != q.shape[0]) return TensorMathError.InputTensorDifferentSize;
+    try check(zant_b200_quantize_rows(context(), rowTypeOf(T), x.data.ptr, x.shape[0], x.shape[1], 0, if (index) |i| i.data.ptr else null, q.shape[0], q.data.ptr, 0, scale.data.ptr));
+}
+
+/// y [rows, n] = a [rows, k] times the transpose of w [n, k], with a scale for each row of either and an optional bias [n].
+pub fn qmatmul_scaled_lean(comptime YT: type, a: *const Tensor(i8), a_scale: *const Tensor(f32), w: *const Tensor(i8), w_scale: *const Tensor(f32), bias: ?*const Tensor(f32), y: *Tensor(YT)) !void {
+    if (a.shape.len != 2 or w.shape.len != 2 or y.shape.len != 2) return TensorError.InvalidRank;
+    if (a.shape[1] != w.shape[1] or a_scale.size != a.shape[0] or w_scale.size != w.shape[0]) return TensorMathError.InputTensorsWrongShape;
+    if (bias) |b| if (b.size != w.shape[0]) return TensorMathError.InputTensorsWrongShape;
+    if (y.shape[0] != a.shape[0] or y.shape[1] != w.shape[0]) return TensorMathError.OutputTensorDifferentSize;
+    try check(zant_b200_qmatmul_scaled(context(), a.data.ptr, a.shape[0], a.shape[1], 0, a_scale.data.ptr, w.data.ptr, w.shape[0], 0, w_scale.data.ptr, if (bias) |b| b.data.ptr else null, rowTypeOf(YT), y.data.ptr, 0));
+}
+
+/// The same with weights w [groups, n, k] for the rows offsets[g] .. offsets[g + 1] - 1; rows in no group are left as they were.
+pub fn qmatmul_grouped_lean(comptime YT: type, a: *const Tensor(i8), a_scale: *const Tensor(f32), w: *const Tensor(i8), w_scale: *const Tensor(f32), offsets: *const Tensor(i32), bias: ?*const Tensor(f32), y: *Tensor(YT)) !void {
+    if (a.shape.len != 2 or w.shape.len != 3 or y.shape.len != 2) return TensorError.InvalidRank;
+    if (a.shape[1] != w.shape[2] or a_scale.size != a.shape[0] or w_scale.size != w.shape[0] * w.shape[1] or offsets.size != w.shape[0] + 1) return TensorMathError.InputTensorsWrongShape;
+    if (bias) |b| if (b.size != w_scale.size) return TensorMathError.InputTensorsWrongShape;
+    if (y.shape[0] != a.shape[0] or y.shape[1] != w.shape[1]) return TensorMathError.OutputTensorDifferentSize;
+    try check(zant_b200_qmatmul_grouped(context(), a.data.ptr, a.shape[0], a.shape[1], 0, a_scale.data.ptr, w.data.ptr, w.shape[0], w.shape[1], 0, w_scale.data.ptr, if (bias) |b| b.data.ptr else null, offsets.data.ptr, rowTypeOf(YT), y.data.ptr, 0));
+}
+
+/// Log probabilities of `tokens` [rows] under logits [rows, vocab], the rows' entropies, and the likeliest ids [rows, top] with their
+/// log probabilities (both null for none).
+pub fn token_logprobs_lean(comptime T: type, logits: *const Tensor(T), tokens: *const Tensor(i32), logprob: *Tensor(f32), entropy: *Tensor(f32), top_ids: ?*Tensor(i32), top_logprobs: ?*Tensor(f32)) !void {
+    if (logits.shape.len != 2) return TensorError.InvalidRank;
+    const rows = logits.shape[0];
+    if (tokens.size != rows or logprob.size != rows or entropy.size != rows) return TensorMathError.InputTensorDifferentSize;
+    var top: usize = 0;
+    if (top_ids) |ids| {
+        if (top_logprobs == null) return B200Error.NullPointer;
+        if (rows == 0 or ids.size % rows != 0 or ids.size / rows > 32 or top_logprobs.?.size != ids.size) return TensorMathError.OutputTensorDifferentSize;
+        top = ids.size / rows;
+    }
+    try check(zant_b200_token_logprobs(context(), rowTypeOf(T), logits.data.ptr, rows, logits.shape[1], 0, tokens.data.ptr, logprob.data.ptr, entropy.data.ptr, @intCast(top), if (top_ids) |t| t.data.ptr else null, if (top_logprobs) |t| t.data.ptr else null));
+}
