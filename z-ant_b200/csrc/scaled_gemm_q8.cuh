@@ -2,11 +2,13 @@
 //   y[m, n] = float(sum over k of a[m, k] w[n, k]) * a_scale[m] * w_scale[n] + bias[n]
 // The sums are exact (int32), so neither their order nor a split of k changes a result.
 //
-// Three kernels, chosen by the tokens of a group and by the operands' addresses:
+// Chosen by the tokens of a group, the tiles that there are, and the operands' addresses:
 //
-//   scaled_few_kernel    up to 32 tokens: warp-level MMAs on operands straight from global memory
-//   scaled_gemm_kernel   tcgen05, operands by TMA: rows that start at multiples of 16 bytes
-//   scaled_any_kernel    tcgen05, rows that start anywhere
+//   scaled_few_kernel    few tokens: warp-level MMAs on operands straight from global memory
+//   scaled_gemm_kernel   tcgen05, 128 channels x 64, 128 or 256 tokens, operands by TMA
+//   scaled_pair_kernel   tcgen05 on pairs of CTAs, 256 channels x 256 tokens
+//   scaled_any_kernel    tcgen05, 128 x 128, rows that the TMA cannot read: calls that may not use the arena
+//   scaled_align_kernel  lays such rows out in the arena for the kernels above
 //
 // On tcgen05 (kind::i8) the weights are the MMA's A operand: 128 output channels on the lanes of an accumulator, NT tokens in its
 // columns.  A warp that reads one column then holds 32 neighbouring channels of one token and stores them as one line, w_scale and bias
@@ -26,10 +28,9 @@
 
 #include "context.cuh"
 #include "fused_cnn.cuh"
+#include "irb_band.cuh"
 #include "ptx_sm100.cuh"
 #include "quantize_rows.cuh"
-#include "quantize_rows.cuh"
-#include "irb_band.cuh"
 #include "tc_conv_nhwc.cuh"
 
 namespace zb {
@@ -448,8 +449,9 @@ __global__ void __launch_bounds__(ScaledAny::THREADS, 1) scaled_any_kernel(const
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// Pairs of CTAs: tiles of 256 channels x 256 tokens, each CTA loads half of either operand (32 KB for 512 clocks of MMA, where one CTA with 128
-// x 256 loads 48 KB: an SM gets about 64 bytes a clock from L2, which held that kernel at 3170 of 4570 TOPS).
+// Pairs of CTAs: tiles of 256 channels x 256 tokens, each CTA loads half of either operand.  What bounds both forms is shared memory, 128 bytes a
+// clock: for 512 clocks of MMA a CTA of a pair takes 32 KB in and 32 KB out to the tensor core, one CTA with 128 x 256 takes 48 KB each way
+// (8192 x 8192 x 8192: 334 us, 3300 TOPS, against 371; the tensor pipe is active 80 % of a tile's time).
 template <int NT>
 __global__ void __launch_bounds__(ScaledCfg<NT>::THREADS, 1) scaled_pair_kernel(const __grid_constant__ ScaledGemmArgs a, const __grid_constant__ CUtensorMap w_map,
                                                                                 const __grid_constant__ CUtensorMap a_map) {
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(ScaledCfg<NT>::THREADS, 1) scaled_pair_kernel(
 // Up to 32 tokens a tile.  Bound by the weights' bytes, and by latency where they are few: no shared memory in front of the MMAs, no barriers but
 // one.  A CTA has 16 MT channels; its 8 warps share k, 128 bytes at a time, and their sums meet in shared memory.  A lane reads 16
 // neighbouring bytes of a row; as operands of m16n8k32 these stand for other k than the instruction's order says, but for the same ones in both
-// operands, and the order of a sum is free.
+// operands, and the order of a sum is free.  One token, 4096 x 4096: 4.9 us, 3.4 TB/s; 8192 x 8192: 14.5 us, 4.6 TB/s.
 template <int NTL, int MT>
 struct ScaledFew {
     static constexpr int TOK = 8 * NTL, CH = 16 * MT, THREADS = 256;
@@ -577,14 +579,14 @@ __global__ void __launch_bounds__(256, 2) scaled_few_kernel(const __grid_constan
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int k = c * 128 + h * 64, valid = all ? 16 : a.k - k - q * 16;
-                auto get = [&](const int8_t* p) {
+                auto get = [&](const int8_t* p, bool once) {
                     if constexpr (ANY) return load16_any(p + k, min(valid, 16));
-                    else return all || valid >= 16 ? __ldg(reinterpret_cast<const uint4*>(p + k)) : load16_any(p + k, valid);
+                    else return all || valid >= 16 ? (once ? ptx::ld_global_once(reinterpret_cast<const uint4*>(p + k)) : __ldg(reinterpret_cast<const uint4*>(p + k))) : load16_any(p + k, valid);
                 };
 #pragma unroll
-                for (int m = 0; m < MT; ++m) { wv[h][m][0] = get(w[m][0]); wv[h][m][1] = get(w[m][1]); }
+                for (int m = 0; m < MT; ++m) { wv[h][m][0] = get(w[m][0], true); wv[h][m][1] = get(w[m][1], true); }
 #pragma unroll
-                for (int i = 0; i < NTL; ++i) xv[h][i] = get(x[i]);
+                for (int i = 0; i < NTL; ++i) xv[h][i] = get(x[i], false);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(256, 2) scaled_few_kernel(const __grid_constan
                     }
         };
         int c = warp;
-#pragma unroll 2
+#pragma unroll (ANY ? 2 : 4)
         for (; c < whole; c += 8) step(c, true);
         if (c * 128 < a.k) step(c, false);
         __syncthreads();                              // the sums of the tile before have been read
@@ -777,8 +779,8 @@ inline int32_t run_scaled_gemm(zant_ctx* ctx, int32_t y_dtype, ScaledGemmArgs a)
     // (the narrowest tiles of any kernel; fewer than an int holds unless y is larger than any memory)
     if (((long long)a.rows / 8 + a.groups) * ((a.n + 15LL) / 16) > 0x7fffffffLL) return fail(ZANT_E_TOO_LARGE, "%d rows in %d groups and %d columns", a.rows, a.groups, a.n);
     const bool tma = a.a_tma && a.w_tma;
-    // Few tokens, and so few tiles of 128 channels that they leave half of the SMs idle (1 x 4096 x 4096: 5.2 us, as tiles 9.9; 1 x 8192 x 8192: 15,
-    // 20; but 16 x 2048 x 12288: 10, 8.4, and 64 experts of one or two rows: 38, 20).  Rows at odd addresses: up to 32 tokens always
+    // Few tokens, and so few tiles of 128 channels that they leave half of the SMs idle (1 x 4096 x 4096: 4.9 us, as tiles 9.9; 1 x 8192 x 8192: 15,
+    // 20; but 16 x 2048 x 12288: 10, 8.2, and 64 experts of one or two rows: 38, 20).  Rows at odd addresses: up to 32 tokens always
     // (1 x 4095 x 4096: 8.3 us, as tiles 16).
     if (tma ? per <= 16 && scaled_row_tiles(a, 64) * ((a.n + 127) / 128) <= ctx->sm_count / 2 : per <= kScaledFewAny) {
         if (per <= 8) return launch_scaled_few<1, 1>(ctx, a);
