@@ -91,6 +91,19 @@ def test_masks(ctx, t, vocab):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(3, 70000), (260, 1819), (200, 31910)])
+@pytest.mark.parametrize("share", [0.5, 0.9, 0.999])
+def test_most_places_masked(ctx, t, rows, vocab, share):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (torch.randn(rows, vocab, generator=g, device="cuda") * 3).to(torch_type(torch, t))
+    x[torch.rand(rows, vocab, generator=g, device="cuda") < share] = -float("inf")
+    tokens = np.random.default_rng(rows).integers(0, vocab, rows).astype(np.int32)
+    for top in (0, 5):
+        check(run(ctx, torch, x, tokens, top), x, tokens, top)
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("vocab", [33, 5000])
 def test_nan_and_infinity(ctx, t, vocab):
     import torch

@@ -44,7 +44,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float((order & 0x80000000u) ? (order & 0x7fffffffu) : ~order); }
 __device__ __forceinline__ unsigned long long key_of(uint32_t order, int id) { return ((unsigned long long)order << 32) | (uint32_t)~id; }
 
-// 16 bytes of logits.  LOW: bits of a float that its values leave 0; FLOOR: what stands for minus infinity; LEAST: a maximum that FLOOR is
+// 16 bytes of logits.  LOW: bits of a float that its values leave 0; FLOOR: a thread's maximum before it has seen one, and about what
+// stands for minus infinity (in f32 below it: what the rounding of FLOOR log2(e) leaves of their difference would overflow); LEAST: a maximum that FLOOR is
 // far enough below to add nothing; MOST: one whose product with log2(e) is finite.
 template <typename T> struct Logits;
 template <> struct Logits<float> {
@@ -53,7 +54,7 @@ template <> struct Logits<float> {
     static constexpr uint32_t NONE = 0xff800000u;
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
     static __device__ __forceinline__ float max1(uint32_t a) { return __uint_as_float(a); }
-    static __device__ __forceinline__ float floored(uint32_t a) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(FLOOR)); return r; }
+    static __device__ __forceinline__ float floored(uint32_t a) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(2.0f * FLOOR)); return r; }
     static __device__ __forceinline__ void values(const uint4& v, float* f) { f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w); }
 };
 template <> struct Logits<__nv_bfloat16> {
