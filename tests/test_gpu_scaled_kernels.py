@@ -38,6 +38,26 @@ def test_sizes_of_each_kernel(ctx, rows, k, n, t):
     sampled(torch, product(ctx, torch, *ops, t, (0, pad), (0, pad)), ops, t)
 
 
+@pytest.mark.parametrize("rows,k,n,t", [
+    (40, 9033, 1856, "bf16"), (113, 9792, 1472, "f16"), (17, 4000, 129, "f32"), (128, 5000, 33, "bf16"),                  # few tiles with a long k
+    (777, 1040, 8191, "f16"), (420, 144, 6200, "f32"), (449, 160, 6300, "bf16"), (1116, 272, 11328, "bf16"), (300, 80, 6331, "f16"), (385, 144, 8000, "f32")])  # pairs, 224 and 192
+def test_narrower_pairs_and_long_rows(ctx, rows, k, n, t):
+    import torch
+    ops = operands(np.random.default_rng(rows), rows, k, n, bias=rows % 2 == 0)
+    pad = -k % 16
+    sampled(torch, product(ctx, torch, *ops, t, (0, pad), (0, pad)), ops, t)
+
+
+@pytest.mark.parametrize("counts", [[340, 300], [0, 900, 131, 65], [257, 5, 640]])
+@pytest.mark.parametrize("k,n,a_at,w_at", [(77, 200, (0, 0), (0, 0)), (513, 129, (0, 15), (0, 0)), (400, 300, (1, 0), (0, 0)), (400, 2900, (0, 0), (0, 0))])
+def test_longer_groups(ctx, tight, counts, k, n, a_at, w_at):
+    import torch
+    offsets = np.concatenate([[1], 1 + np.cumsum(counts)])
+    ops = operands(np.random.default_rng(k + n), int(offsets[-1]) + 3, k, n, len(counts), bias=True)
+    for c in (ctx, tight):
+        check_groups(grouped(c, torch, ops, offsets, "bf16", 2, a_at, w_at), ops, offsets, "bf16")
+
+
 @pytest.mark.parametrize("a_at,w_at", [((0, 0), (1, 0)), ((7, 0), (0, 0)), ((3, 1), (5, 2)), ((1, 4), (2, 6))])
 @pytest.mark.parametrize("rows,k,n", [(3, 700, 130), (30, 333, 257), (33, 129, 128), (129, 1001, 300), (260, 64, 129), (70, 4111, 131)])
 def test_rows_read_where_they_are(tight, rows, k, n, a_at, w_at):

@@ -284,7 +284,7 @@ inline int32_t launch_quantize_rows(zant_ctx* ctx, const QuantizeRowsArgs& a) {
     // Chunks a thread: one for latency while the GPU holds that many threads (8 x 4096 bf16: 1.6, 1.7, 2.1, 2.9 us with 1, 2, 4, 8; 512 x 4096:
     // 3.2, 3.1, 4.5, 5.5), more where there are millions, which saves the instructions that each thread spends on its row (8192 x 4096: 30,
     // 25, 20, 21; 8192 x 8192: 62, 57, 38, 36), and no more than a warp needs for a row (65536 x 1024: 68, 68, 35, 46).
-    auto many = [&](int per_thread) { return a.rows * chunks > (long long)ctx->sm_count * (per_thread == 4 ? 40960 : 3072 * per_thread); };
+    auto many = [&](int per_thread) { return a.rows * chunks > (long long)ctx->sm_count * (per_thread == 4 ? 40960 : 3000 * per_thread); };
     int per = 1;
     while (per < 8 && (warps(per) > 32 || (warps(per) > 1 && many(per)))) per *= 2;
     if (warps(per) > (per == 8 ? 16 : 32)) return go(quantize_rows_kernel<T, 4, true>, 32);
