@@ -144,6 +144,19 @@ def test_c_entries(zb):
     assert logprobs(rows=0, x=None) == "OK"
 
 
+def test_counts_next_to_an_ints_limit(zb):
+    """What the loops of the kernels could not step over is refused, a little less is not."""
+    L, p = zb.lib(), np.zeros(64, F).__array_interface__["data"][0]
+    name = lambda status: L.zant_b200_status_name(C.c_int32(status)).decode()
+    for v, want in ((0x7fffffff, "TooLarge"), (0x7fff0001, "TooLarge"), (0x7fff0000, "CudaUnavailable")):
+        assert name(L.zant_b200_quantize_rows(None, 0, p, v, 1, 0, None, v, p, 0, p)) == want
+        assert name(L.zant_b200_quantize_rows(None, 0, p, 1, v, 0, None, 1, p, 0, p)) == want
+        assert name(L.zant_b200_qmatmul_scaled(None, p, v, 1, 0, p, p, 1, 0, p, None, 0, p, 0)) == want
+        assert name(L.zant_b200_qmatmul_scaled(None, p, 1, 1, 0, p, p, v, 0, p, None, 0, p, 0)) == want
+        assert name(L.zant_b200_token_logprobs(None, 0, p, v, 1, 0, None, None, p, 0, None, None)) == want
+        assert name(L.zant_b200_token_logprobs(None, 0, p, 1, v, 0, None, None, p, 0, None, None)) == want
+
+
 def test_other_operators_refuse_the_new_types(zb):
     L = zb.lib()
     p = np.zeros(64, F).__array_interface__["data"][0]

@@ -44,9 +44,9 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float((order & 0x80000000u) ? (order & 0x7fffffffu) : ~order); }
 __device__ __forceinline__ unsigned long long key_of(uint32_t order, int id) { return ((unsigned long long)order << 32) | (uint32_t)~id; }
 
-// 16 bytes of logits.  LOW: bits of a float that its values leave 0; FLOOR: a thread's maximum before it has seen one, and about what
-// stands for minus infinity (in f32 below it: what the rounding of FLOOR log2(e) leaves of their difference would overflow); LEAST: a maximum that FLOOR is
-// far enough below to add nothing; MOST: one whose product with log2(e) is finite.
+// 16 bytes of logits.  LOW: bits of a float that its values leave 0; FLOOR: a thread's maximum before it has seen one; what stands for minus
+// infinity is FLOOR in f16, below it in the others, where the rounding of FLOOR log2(e) leaves a difference whose power would overflow;
+// LEAST: a maximum that both are far enough below to add nothing; MOST: one whose product with log2(e) is finite.
 template <typename T> struct Logits;
 template <> struct Logits<float> {
     static constexpr int N = 4, LOW = 0;

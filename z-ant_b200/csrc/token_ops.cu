@@ -31,7 +31,8 @@ inline int32_t check_aligned(const char* what, const void* p, size_t esz) {
     return (reinterpret_cast<uintptr_t>(p) & (esz - 1)) && is_device_ptr(p) ? fail(ZANT_E_INVALID_INPUT, "%s is not aligned to its elements", what) : ZANT_OK;
 }
 
-inline int32_t check_int(const char* what, size_t v) { return v > 0x7fffffffULL ? fail(ZANT_E_TOO_LARGE, "%s = %zu", what, v) : ZANT_OK; }
+// What the kernels count in an int, with room for the steps of their loops past the end.
+inline int32_t check_int(const char* what, size_t v) { return v > 0x7fff0000ULL ? fail(ZANT_E_TOO_LARGE, "%s = %zu", what, v) : ZANT_OK; }
 
 // Nothing of C++ leaves a C entry point.
 template <typename F>
