@@ -40,8 +40,8 @@ def test_sizes_of_each_kernel(ctx, rows, k, n, t):
 
 @pytest.mark.parametrize("rows,k,n,t", [
     (40, 9033, 1856, "bf16"), (113, 9792, 1472, "f16"), (17, 4000, 129, "f32"), (128, 5000, 33, "bf16"),                  # few tiles with a long k
-    (777, 1040, 8191, "f16"), (420, 144, 6200, "f32"), (449, 160, 6300, "bf16"), (1116, 272, 11328, "bf16"), (300, 80, 6331, "f16"), (385, 144, 8000, "f32")])  # pairs, 224 and 192
-def test_narrower_pairs_and_long_rows(ctx, rows, k, n, t):
+    (777, 1040, 8191, "f16"), (420, 144, 6200, "f32"), (449, 160, 6300, "bf16"), (1116, 272, 11328, "bf16"), (300, 80, 6331, "f16"), (385, 144, 8000, "f32")])  # pairs whose last tiles are short
+def test_long_rows_and_last_pairs(ctx, rows, k, n, t):
     import torch
     ops = operands(np.random.default_rng(rows), rows, k, n, bias=rows % 2 == 0)
     pad = -k % 16

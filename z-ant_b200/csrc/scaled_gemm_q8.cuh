@@ -6,7 +6,7 @@
 //
 //   scaled_few_kernel    few tokens: warp-level MMAs on operands straight from global memory
 //   scaled_gemm_kernel   tcgen05, 128 channels x 64, 128 or 256 tokens, operands by TMA
-//   scaled_pair_kernel   tcgen05 on pairs of CTAs, 256 channels x up to 256 tokens
+//   scaled_pair_kernel   tcgen05 on pairs of CTAs, 256 channels x 256 tokens
 //   scaled_any_kernel    tcgen05, 128 x 128, rows that the TMA cannot read: calls that may not use the arena
 //   scaled_align_kernel  lays such rows out in the arena for the kernels above
 //
@@ -48,7 +48,6 @@ struct ScaledGemmArgs {
     int y_dtype;
     // how it is run
     int n_tiles, k_blocks, stages;
-    int nt;                              // tokens of a pair's tile: a multiple of 32 up to 256
     int a_tma, w_tma;
     int off_scales, off_groups, off_bar;        // shared memory
     int* status;
@@ -200,7 +199,7 @@ __device__ __forceinline__ void scaled_epilogue_role(const ScaledGemmArgs& a, co
     int ti = 0;
     for (int t = t0; t < tiles; t += step, ++ti) {
         const TileAt at = tile_at(t, row_tiles, a.n_tiles);
-        const RowTile rt = row_tile_of(a, grow, gfirst, at.m, PAIR ? a.nt : NT);
+        const RowTile rt = row_tile_of(a, grow, gfirst, at.m, NT);
         const int n = (PAIR ? at.n * 256 + rank * 128 : at.n * 128) + quarter * 32 + lane, b = ti & 1;
         const bool live = n < a.n;
         const long long wat = (long long)rt.group * a.n + n;
@@ -450,14 +449,14 @@ __global__ void __launch_bounds__(ScaledAny::THREADS, 1) scaled_any_kernel(const
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// Pairs of CTAs: tiles of 256 channels x up to 256 tokens, each CTA loads half of either operand.  What bounds both forms is shared memory, 128 bytes a
+// Pairs of CTAs: tiles of 256 channels x 256 tokens, each CTA loads half of either operand.  What bounds both forms is shared memory, 128 bytes a
 // clock: for 512 clocks of MMA a CTA of a pair takes 32 KB in and 32 KB out to the tensor core, one CTA with 128 x 256 takes 48 KB each way
 // (8192 x 8192 x 8192: 334 us, 3300 TOPS, against 371; the tensor pipe is active 80 % of a tile's time).
 __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel(const __grid_constant__ ScaledGemmArgs a, const __grid_constant__ CUtensorMap w_map,
                                                                                 const __grid_constant__ CUtensorMap a_map) {
     constexpr int NT = 256;
     using Cfg = ScaledCfg<NT>;
-    const int stage = Cfg::STAGE_W + a.nt / 2 * 128;
+    constexpr int STAGE = Cfg::STAGE_W + NT / 2 * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t s0 = ptx::smem_u32(smem);
     int* grow = reinterpret_cast<int*>(smem + a.off_groups);
@@ -467,8 +466,8 @@ __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel
     const int warp = threadIdx.x >> 5, rank = (int)ptx::cluster_rank();
     const uint32_t tmem_base = scaled_setup<Cfg::TMEM_COLS, true>(smem, a, bar, 1, 2 * Cfg::EPI);
 
-    int row_tiles = (a.rows + a.nt - 1) / a.nt;
-    if (a.offsets) { group_tiles(a.offsets, a.groups, a.rows, a.nt, grow, gfirst); row_tiles = gfirst[a.groups]; }
+    int row_tiles = (a.rows + NT - 1) / NT;
+    if (a.offsets) { group_tiles(a.offsets, a.groups, a.rows, NT, grow, gfirst); row_tiles = gfirst[a.groups]; }
     const int step = (int)gridDim.x / 2, t0 = (int)blockIdx.x / 2, tiles = row_tiles * a.n_tiles;
     // columns of a tile: its tokens rounded up to 32; the first half of them are rank 0's rows of the operand, the second rank 1's
     auto half_of = [](int rows) { return ((rows + 31) & ~31) / 2; };
@@ -478,12 +477,12 @@ __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel
             int s = 0; uint32_t ph = 0;
             for (int t = t0; t < tiles; t += step) {
                 const TileAt at = tile_at(t, row_tiles, a.n_tiles);
-                const RowTile rt = row_tile_of(a, grow, gfirst, at.m, a.nt);
+                const RowTile rt = row_tile_of(a, grow, gfirst, at.m, NT);
                 const int wrow = rt.group * a.n + at.n * 256 + rank * 128, xrow = rt.row + rank * half_of(rt.rows);
                 for (int kb = 0; kb < a.k_blocks; ++kb) {
                     if (!ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag)) goto producer_done;
-                    if (rank == 0) ptx::mbar_arrive_expect_tx(bar.full(s), 2 * stage);
-                    const uint32_t dst = s0 + (uint32_t)(s * stage), full = ptx::cluster_addr(bar.full(s), 0);
+                    if (rank == 0) ptx::mbar_arrive_expect_tx(bar.full(s), 2 * STAGE);
+                    const uint32_t dst = s0 + (uint32_t)(s * STAGE), full = ptx::cluster_addr(bar.full(s), 0);
                     ptx::tma_load_2d_pair(dst, &w_map, kb * 128, wrow, full);
                     ptx::tma_load_2d_pair(dst + Cfg::STAGE_W, &a_map, kb * 128, xrow, full);
                     if (++s == a.stages) { s = 0; ph ^= 1u; }
@@ -503,13 +502,13 @@ __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel
                 ok = ptx::mbar_wait(bar.tempty(b), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag);
                 if (!ok) break;
                 ptx::tc_fence_after();
-                const RowTile rt = row_tile_of(a, grow, gfirst, tile_at(t, row_tiles, a.n_tiles).m, a.nt);
+                const RowTile rt = row_tile_of(a, grow, gfirst, tile_at(t, row_tiles, a.n_tiles).m, NT);
                 const uint32_t idesc = ptx::idesc_i8(256, 2 * half_of(rt.rows), true, true), d = tmem_base + (uint32_t)(b * NT);
                 for (int kb = 0; kb < a.k_blocks; ++kb) {
                     ok = ptx::mbar_wait(bar.full(s), ph, abort_flag);
                     if (!ok) break;
                     ptx::tc_fence_after();
-                    const uint32_t wa = lo + ((s0 + (uint32_t)(s * stage)) >> 4), ta = wa + (Cfg::STAGE_W >> 4);
+                    const uint32_t wa = lo + ((s0 + (uint32_t)(s * STAGE)) >> 4), ta = wa + (Cfg::STAGE_W >> 4);
                     const int steps = min(4, (a.k - kb * 128 + 31) >> 5);
                     for (int i = 0; i < steps; ++i) ptx::mma_i8_pair_if(leader, d, wa + 2u * i, hi, ta + 2u * i, hi, idesc, (kb | i) ? 1u : 0u);
                     ptx::mma_commit_pair_if(leader, bar.empty(s));
@@ -528,7 +527,7 @@ __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel
 // Up to 32 tokens a tile.  Bound by the weights' bytes, and by latency where they are few: no shared memory in front of the MMAs, no barriers but
 // one.  A CTA has 16 MT channels; its 8 warps share k, 128 bytes at a time, and their sums meet in shared memory.  A lane reads 16
 // neighbouring bytes of a row; as operands of m16n8k32 these stand for other k than the instruction's order says, but for the same ones in both
-// operands, and the order of a sum is free.  One token, 4096 x 4096: 4.9 us, 3.4 TB/s; 8192 x 8192: 14.5 us, 4.6 TB/s.
+// operands, and the order of a sum is free.  One token, 4096 x 4096: 4.9 us, 3.4 TB/s; 8192 x 8192: 14.5 us, 4.6 TB/s.  PER: CTAs an SM.
 template <int NTL, int MT>
 struct ScaledFew {
     static constexpr int TOK = 8 * NTL, CH = 16 * MT, THREADS = 256;
@@ -551,8 +550,8 @@ __device__ __forceinline__ uint4 load16_any(const int8_t* p, int valid) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-template <int NTL, int MT, bool ANY>
-__global__ void __launch_bounds__(256, 2) scaled_few_kernel(const __grid_constant__ ScaledGemmArgs a) {
+template <int NTL, int MT, bool ANY, int PER>
+__global__ void __launch_bounds__(256, PER) scaled_few_kernel(const __grid_constant__ ScaledGemmArgs a) {
     using F = ScaledFew<NTL, MT>;
     __shared__ int part[8][F::TOK][F::CH];
     __shared__ int grow[kScaledMaxGroups + 1], gfirst[kScaledMaxGroups + 1];
@@ -669,9 +668,20 @@ template <int NTL, int MT>
 inline int32_t launch_scaled_few(zant_ctx* ctx, ScaledGemmArgs a) {
     using F = ScaledFew<NTL, MT>;
     a.n_tiles = (a.n + F::CH - 1) / F::CH;
-    const unsigned grid = (unsigned)std::min<long long>(scaled_row_tiles(a, F::TOK) * a.n_tiles, (long long)ctx->sm_count * 16);
-    if (a.a_tma && a.w_tma) launch(ctx, scaled_few_kernel<NTL, MT, false>, dim3(grid), F::THREADS, 0, a);
-    else launch(ctx, scaled_few_kernel<NTL, MT, true>, dim3(grid), F::THREADS, 0, a);
+    const long long tiles = scaled_row_tiles(a, F::TOK) * a.n_tiles;
+    const unsigned grid = (unsigned)std::min<long long>(tiles, (long long)ctx->sm_count * 16);
+    auto go = [&](auto kernel) { launch(ctx, kernel, dim3(grid), F::THREADS, 0, a); };
+    // No more tiles than SMs: one CTA an SM with twice the registers, for loads further ahead (40 x 9040 x 1856: 12.8 us, with two 17.8; 16 x 4096 x
+    // 2048: 4.0, 5.1; 30 x 4095 x 2001: 12.2, 18.9; but 18 x 3381 x 8256, 258 tiles: 19.3, 15.1).  One token at an odd address needs no more.
+    const bool tma = a.a_tma && a.w_tma, one = tiles <= ctx->sm_count;
+    if (tma) {
+        if constexpr (NTL == 4) go(scaled_few_kernel<NTL, MT, false, 1>);         // (comes here with so few tiles only)
+        else one ? go(scaled_few_kernel<NTL, MT, false, 1>) : go(scaled_few_kernel<NTL, MT, false, 2>);
+    } else if constexpr (NTL == 1) {
+        go(scaled_few_kernel<NTL, MT, true, 2>);
+    } else {
+        one ? go(scaled_few_kernel<NTL, MT, true, 1>) : go(scaled_few_kernel<NTL, MT, true, 2>);
+    }
     return check_launch(ctx, "scaled_few_kernel");
 }
 
@@ -682,7 +692,7 @@ inline int32_t launch_scaled_tc(zant_ctx* ctx, const char* name, ScaledGemmArgs 
     constexpr int LIMIT = 232448;
     a.n_tiles = (a.n + tile_n - 1) / tile_n;
     a.k_blocks = (a.k + 127) / 128;
-    const int groups = a.offsets ? (kScaledMaxGroups + 1) * 8 : 0, scales = 2 * 256 * 4;
+    const int groups = a.offsets ? (kScaledMaxGroups + 1) * 8 : 0, scales = 2 * tile_rows * 4;
     a.stages = std::min(16, (LIMIT - scales - groups - ScaledBars::BYTES - 16) / stage);
     a.off_scales = a.stages * stage;
     a.off_groups = a.off_scales + scales;
@@ -701,7 +711,7 @@ inline int32_t launch_scaled_gemm(zant_ctx* ctx, const ScaledGemmArgs& a) {
     return launch_scaled_tc<scaled_gemm_kernel<NT>>(ctx, "scaled_gemm_kernel", a, ScaledCfg<NT>::STAGE, ScaledCfg<NT>::THREADS, NT, 128, 128, NT, 1);
 }
 inline int32_t launch_scaled_pair(zant_ctx* ctx, const ScaledGemmArgs& a) {
-    return launch_scaled_tc<scaled_pair_kernel>(ctx, "scaled_pair_kernel", a, ScaledCfg<256>::STAGE_W + a.nt / 2 * 128, ScaledCfg<256>::THREADS, a.nt, 256, 128, a.nt / 2, 2);
+    return launch_scaled_tc<scaled_pair_kernel>(ctx, "scaled_pair_kernel", a, ScaledCfg<256>::STAGE_W + 128 * 128, ScaledCfg<256>::THREADS, 256, 256, 128, 128, 2);
 }
 template <bool BOTH>
 inline int32_t launch_scaled_any(zant_ctx* ctx, const ScaledGemmArgs& a) {
@@ -737,15 +747,14 @@ inline int32_t run_scaled_align(zant_ctx* ctx, const int8_t* from, long long str
 }
 
 // Which kernel: clocks of an SM (or a pair) for 128 bytes of k of a tile, from products of 128 to 8192 rows, times the tiles that one of them gets.  They
-// are what shared memory delivers: operands in and out again, 64 tokens 24 KB each way, 128 32 KB, 256 48 KB, in a pair 24 KB for 128 to
-// 32 KB for 256.  Pairs of 224 or 192 tokens are for sizes that leave a round of tiles of 256 nearly empty (1116 x 7168 x 11328: 67 us, with 256 only
-// 71.5; 570 x 10048 x 4608: 24, 29).
-// Up to 128 tokens a group the few-token kernel wins where k is long and the tiles are few (113 x 9792 x 1472, 24 tiles: 17.9 us, as tiles 19.4; 40 x
-// 9040 x 1856: 17.8, 20.7; but 64 x 512 x 512: 4.1, 3.5): it reads 64 bytes for each k of a 32 x 32 tile, 9.5 TB/s or less.
+// are what shared memory delivers: operands in and out again, 64 tokens 24 KB each way, 128 32 KB, 256 48 KB, in a pair 32 KB.
+// Up to 128 tokens a group the few-token kernel wins where there are no more tiles of 32 x 32 than SMs (40 x 9040 x 1856: 12.8 us, as tiles of 128
+// channels 20.7; 96 x 4096 x 1024: 6.2, 9.6; 128 x 1024 x 512: 4.0, 4.4; but 113 x 9792 x 1472, 184 tiles: 23, 19.4; 128 x 512 x 512: 3.6, 3.5), at odd
+// addresses with any k (37 x 970 x 1065: 5.0 us, 7.9).
 struct ScaledChoice { int nt; bool pair, few; };
 inline ScaledChoice scaled_choice(const ScaledGemmArgs& a, int sm_count) {
     struct Kind { int nt, wide, clocks; };
-    constexpr Kind kinds[6] = {{64, 128, 370}, {128, 128, 450}, {256, 128, 720}, {256, 256, 620}, {224, 256, 580}, {192, 256, 545}};
+    constexpr Kind kinds[4] = {{64, 128, 370}, {128, 128, 450}, {256, 128, 720}, {256, 256, 620}};
     const double groups = std::min(a.rows, a.groups), per = a.rows / groups;
     ScaledChoice best{64, false, false};
     double least = 0;
@@ -755,8 +764,8 @@ inline ScaledChoice scaled_choice(const ScaledGemmArgs& a, int sm_count) {
         const double cost = (a.offsets ? std::max(1.0, tiles) : std::ceil(tiles)) * k.clocks;
         if (least == 0 || cost < least) { least = cost; best = ScaledChoice{k.nt, k.wide == 256, false}; }
     }
-    const double bytes = (double)scaled_row_tiles(a, 32) * ((a.n + 31) / 32) * 64 * a.k, us = least * ((a.k + 127) / 128) / 1750;
-    best.few = per <= 128 && a.k >= 2048 && bytes / 9.5e6 < 0.85 * us;
+    const bool tma = tma_rows(a.a, (size_t)a.rows, (size_t)a.a_stride) && tma_rows(a.w, (size_t)a.groups * a.n, (size_t)a.w_stride);
+    best.few = per <= 128 && scaled_row_tiles(a, 32) * ((a.n + 31) / 32) <= sm_count && (!tma || a.k > 512);
     return best;
 }
 
@@ -792,7 +801,6 @@ inline int32_t run_scaled_gemm(zant_ctx* ctx, int32_t y_dtype, ScaledGemmArgs a)
         return launch_scaled_few<4, 2>(ctx, a);
     }
     if (!tma) return a.a_tma || a.w_tma ? launch_scaled_any<false>(ctx, a) : launch_scaled_any<true>(ctx, a);
-    a.nt = c.nt;
     if (c.pair) return launch_scaled_pair(ctx, a);
     if (c.nt == 64) return launch_scaled_gemm<64>(ctx, a);
     if (c.nt == 128) return launch_scaled_gemm<128>(ctx, a);
