@@ -189,8 +189,9 @@ int32_t zant_b200_measure_int8_peak_sustained(zant_ctx* ctx, double seconds, dou
 int32_t zant_b200_selftest_bounded_wait(zant_ctx* ctx, uint32_t budget_us);
 
 /* Failure-path self test (no reference counterpart).  In the next launch of the kernel that runs an inverted residual
- * block of a plan on bands of rows (few images), CTA `cta`, modulo the launch's CTAs, acts as if its first bounded wait
- * had run out: it fetches no further weights and gives up later waits soon.  That run reports
+ * block of a plan on bands of rows (few images), or of a tensor-memory kernel of qmatmul_scaled and qmatmul_grouped, CTA
+ * `cta`, modulo the launch's CTAs, acts as if its first bounded wait had run out: it fetches no further weights and gives
+ * up later waits soon.  That run reports
  * ZANT_E_DEVICE_TIMEOUT as zant_b200_selftest_bounded_wait describes, and the runs after it are right again.
  * A negative `cta` disarms it. */
 int32_t zant_b200_selftest_give_up(zant_ctx* ctx, int32_t cta);

@@ -414,7 +414,8 @@ class Context:
         check(lib().zant_b200_selftest_bounded_wait(self._h, C.c_uint32(int(budget_us))))
 
     def selftest_give_up(self, cta):
-        """CTA `cta` of the next inverted residual block that runs on clusters gives up a wait; that run raises DeviceTimeout."""
+        """CTA `cta` of the next inverted residual block that runs on clusters, or of the next scaled product on tensor memory, gives up a
+        wait; that run raises DeviceTimeout."""
         check(lib().zant_b200_selftest_give_up(self._h, C.c_int32(int(cta))))
 
     def measure_int8_peak(self, iters=20000):

@@ -51,6 +51,8 @@ struct ScaledGemmArgs {
     int a_tma, w_tma;
     int off_scales, off_groups, off_bar;        // shared memory
     int* status;
+    long long wait_budget;               // clocks after which a wait gives up
+    int give_up;                         // self test: a CTA whose first wait counts as run out (-1: none)
 };
 
 __device__ __forceinline__ void store_as(float* p, float v) { *p = v; }
@@ -160,6 +162,12 @@ struct ScaledBars {
     static constexpr int SLOT = 400, FLAG = 404, BYTES = 512;       // TMEM address, abort flag
 };
 
+// A wait of a whole warp.  Its lanes leave it together and with one answer: behind it stand instructions and barriers that want all of them (tcgen05.ld,
+// shuffles, the next wait of a ring, in which a lane a phase behind the others would wait for good).
+__device__ __forceinline__ bool scaled_wait(const ScaledGemmArgs& a, uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag, a.wait_budget)) != 0;
+}
+
 // The MMA issuer (a whole warp): NT columns per tile of the walk t0, t0 + step, ..
 template <int NT>
 __device__ __forceinline__ void scaled_mma_role(const ScaledGemmArgs& a, const ScaledBars& bar, uint32_t s0, uint32_t tmem_base, const int* grow, const int* gfirst,
@@ -172,12 +180,12 @@ __device__ __forceinline__ void scaled_mma_role(const ScaledGemmArgs& a, const S
     uint32_t ph = 0;
     for (int t = t0; t < tiles; t += step, ++ti) {
         const int b = ti & 1;
-        if (!ptx::mbar_wait(bar.tempty(b), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag)) return;
+        if (!scaled_wait(a, bar.tempty(b), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag)) return;
         ptx::tc_fence_after();
         const RowTile rt = row_tile_of(a, grow, gfirst, tile_at(t, row_tiles, a.n_tiles).m, NT);
         const uint32_t idesc = ptx::idesc_i8(128, (rt.rows + 15) & ~15, true, true), d = tmem_base + (uint32_t)(b * NT);
         for (int kb = 0; kb < a.k_blocks; ++kb) {
-            if (!ptx::mbar_wait(bar.full(s), ph, abort_flag)) return;
+            if (!scaled_wait(a, bar.full(s), ph, abort_flag)) return;
             ptx::tc_fence_after();
             const uint32_t wa = lo + ((s0 + (uint32_t)(s * Cfg::STAGE)) >> 4), ta = wa + (Cfg::STAGE_W >> 4);
             const int steps = min(4, (a.k - kb * 128 + 31) >> 5);
@@ -190,13 +198,15 @@ __device__ __forceinline__ void scaled_mma_role(const ScaledGemmArgs& a, const S
 }
 
 // An epilogue warp: lane quarter `warp & 3`, the `part`-th of the tile's column ranges.  PAIR: the CTA has half `rank` of the tile's 256 channels,
-// and rank 0 is told when the accumulators are free.
+// and rank 0 is told when the accumulators are free.  A warp whose wait has given up still walks its tiles, from part barrier to part barrier: the other
+// warps of the part may have had the accumulator, and would stand there.
 template <int NT, bool PAIR>
 __device__ __forceinline__ void scaled_epilogue_role(const ScaledGemmArgs& a, const ScaledBars& bar, uint32_t tmem_base, const int* grow, const int* gfirst, int row_tiles,
                                                      int t0, int step, int quarter, int part, int rank, float* scale_ring, volatile int* abort_flag) {
     using Cfg = ScaledCfg<NT>;
     const int tiles = row_tiles * a.n_tiles, lane = threadIdx.x & 31;
     int ti = 0;
+    bool ok = true;
     for (int t = t0; t < tiles; t += step, ++ti) {
         const TileAt at = tile_at(t, row_tiles, a.n_tiles);
         const RowTile rt = row_tile_of(a, grow, gfirst, at.m, NT);
@@ -210,7 +220,8 @@ __device__ __forceinline__ void scaled_epilogue_role(const ScaledGemmArgs& a, co
         float* scales = scale_ring + b * NT + col0;
         if (lane < Cfg::COLS / 4) scales[own] = own < cols ? a.a_scale[rt.row + col0 + own] : 0.0f;
         ptx::named_barrier_sync(1 + part, 128);
-        if (!ptx::mbar_wait(bar.tfull(b), (uint32_t)(ti >> 1) & 1u, abort_flag)) return;
+        ok = ok && scaled_wait(a, bar.tfull(b), (uint32_t)(ti >> 1) & 1u, abort_flag);
+        if (!ok) continue;
         ptx::tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * NT + col0);
 #pragma unroll 1
@@ -236,7 +247,7 @@ __device__ __forceinline__ uint32_t scaled_setup(uint8_t* smem, const ScaledGemm
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) { ptx::mbar_init(bar.full(s), (uint32_t)full_arrivals); ptx::mbar_init(bar.empty(s), 1); }
         for (int b = 0; b < 2; ++b) { ptx::mbar_init(bar.tfull(b), 1); ptx::mbar_init(bar.tempty(b), (uint32_t)epilogue_warps); }
-        *reinterpret_cast<volatile int*>(smem + a.off_bar + ScaledBars::FLAG) = 0;
+        *reinterpret_cast<volatile int*>(smem + a.off_bar + ScaledBars::FLAG) = (int)blockIdx.x == a.give_up ? 1 : 0;
         ptx::mbar_fence_init();
     }
     if (threadIdx.x >> 5 == 1) {
@@ -293,7 +304,7 @@ __global__ void __launch_bounds__(ScaledCfg<NT>::THREADS, 1) scaled_gemm_kernel(
                 const RowTile rt = row_tile_of(a, grow, gfirst, at.m, NT);
                 const int wrow = rt.group * a.n + at.n * 128;
                 for (int kb = 0; kb < a.k_blocks; ++kb) {
-                    if (!ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag)) goto producer_done;
+                    if (!ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag, a.wait_budget)) goto producer_done;
                     ptx::mbar_arrive_expect_tx(bar.full(s), Cfg::STAGE);
                     const uint32_t dst = s0 + (uint32_t)(s * Cfg::STAGE);
                     ptx::tma_load_2d(dst, &w_map, kb * 128, wrow, bar.full(s));
@@ -401,7 +412,7 @@ __global__ void __launch_bounds__(ScaledAny::THREADS, 1) scaled_any_kernel(const
                 const RowTile rt = row_tile_of(a, grow, gfirst, at.m, NT);
                 const int wrow = rt.group * a.n + at.n * 128;
                 for (int kb = 0; kb < a.k_blocks; ++kb) {
-                    if (!ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag)) goto producer_done;
+                    if (!ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag, a.wait_budget)) goto producer_done;
                     ptx::mbar_arrive_expect_tx(bar.full(s), bytes);
                     const uint32_t dst = s0 + (uint32_t)(s * Cfg::STAGE);
                     if (a.w_tma) ptx::tma_load_2d(dst, &w_map, kb * 128, wrow, bar.full(s));
@@ -430,7 +441,7 @@ __global__ void __launch_bounds__(ScaledAny::THREADS, 1) scaled_any_kernel(const
             else rows.begin(a.a, rt.row + row0, a.a_stride, rt.rows - row0, a.k, lane);
             auto stage = [&](auto at_stage, int kb) {
                 if (kb >= a.k_blocks || !ok) return;
-                ok = ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag);
+                ok = scaled_wait(a, bar.empty(s), ph ^ 1u, abort_flag);
                 if (!ok) return;
                 rows.template stage<decltype(at_stage)::value>(smem + s * Cfg::STAGE + (weights ? 0 : Cfg::STAGE_W) + row0 * 128, a.k - kb * 128, lane);
                 ptx::fence_proxy_async_smem();
@@ -480,7 +491,7 @@ __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel
                 const RowTile rt = row_tile_of(a, grow, gfirst, at.m, NT);
                 const int wrow = rt.group * a.n + at.n * 256 + rank * 128, xrow = rt.row + rank * half_of(rt.rows);
                 for (int kb = 0; kb < a.k_blocks; ++kb) {
-                    if (!ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag)) goto producer_done;
+                    if (!ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag, a.wait_budget)) goto producer_done;
                     if (rank == 0) ptx::mbar_arrive_expect_tx(bar.full(s), 2 * STAGE);
                     const uint32_t dst = s0 + (uint32_t)(s * STAGE), full = ptx::cluster_addr(bar.full(s), 0);
                     ptx::tma_load_2d_pair(dst, &w_map, kb * 128, wrow, full);
@@ -499,13 +510,13 @@ __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel
             bool ok = true;
             for (int t = t0; t < tiles && ok; t += step, ++ti) {
                 const int b = ti & 1;
-                ok = ptx::mbar_wait(bar.tempty(b), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag);
+                ok = scaled_wait(a, bar.tempty(b), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 const RowTile rt = row_tile_of(a, grow, gfirst, tile_at(t, row_tiles, a.n_tiles).m, NT);
                 const uint32_t idesc = ptx::idesc_i8(256, 2 * half_of(rt.rows), true, true), d = tmem_base + (uint32_t)(b * NT);
                 for (int kb = 0; kb < a.k_blocks; ++kb) {
-                    ok = ptx::mbar_wait(bar.full(s), ph, abort_flag);
+                    ok = scaled_wait(a, bar.full(s), ph, abort_flag);
                     if (!ok) break;
                     ptx::tc_fence_after();
                     const uint32_t wa = lo + ((s0 + (uint32_t)(s * STAGE)) >> 4), ta = wa + (Cfg::STAGE_W >> 4);
@@ -703,6 +714,9 @@ inline int32_t launch_scaled_tc(zant_ctx* ctx, const char* name, ScaledGemmArgs 
     ZB_SMEM_ATTR(ctx, KERNEL, LIMIT);
     const long long tiles = std::max<long long>(1, scaled_row_tiles(a, tile_rows)) * a.n_tiles;
     const unsigned grid = (unsigned)std::min<long long>(tiles, ctx->sm_count / cluster) * (unsigned)cluster;
+    a.give_up = ctx->give_up_cta < 0 ? -1 : ctx->give_up_cta % (int)grid;
+    ctx->give_up_cta = -1;
+    a.wait_budget = a.give_up < 0 ? ptx::kWaitBudgetCycles : 4000000;       // self test: 2 ms, which the CTA's pair waits for it
     launch_cluster(ctx, KERNEL, dim3(grid), threads, (size_t)a.off_bar + ScaledBars::BYTES, (unsigned)cluster, a, w_map, a_map);
     return check_launch(ctx, name);
 }
