@@ -65,3 +65,33 @@ def test_few_token_products_have_no_such_wait(zb, tight):
     tight.selftest_give_up(-1)
     ops = operands(np.random.default_rng(4), 300, 256, 4000)
     sampled(torch, product(tight, torch, *ops, "f32"), ops, "f32")
+
+
+def test_kernels_close_behind_each_other(zb):
+    """Short products of each kernel follow each other without a pause, on barriers at the same shared memory: none is disturbed by what the one before it
+    has still under way, and none waits for long."""
+    import torch
+    c = zb.Context(0)
+    stream = torch.cuda.Stream()
+    c.set_stream(stream.cuda_stream)
+    rng = np.random.default_rng(11)
+    work = []
+    # pairs of CTAs before and behind each other kernel; k of one stage, of a few, of more than the ring holds
+    for rows, k, n in ((1000, 512, 4096), (60, 128, 3000), (1000, 128, 4096), (130, 320, 9001), (8192, 144, 512), (700, 144, 6200), (1000, 1040, 4096), (5, 256, 128)):
+        ops = operands(rng, rows, k, n)
+        dev = [torch.from_numpy(v).cuda() for v in ops[:4]]
+        want = (dev[0].double() @ dev[2].double().T).float() * dev[1][:, None] * dev[3]         # (exact sums, and the kernels' order of roundings)
+        work.append((dev, torch.empty(rows, n, device="cuda"), want))
+    torch.cuda.synchronize()
+    for turn in range(40):
+        for i in range(len(work)):
+            dev, y, _ = work[(i * (1 + 2 * (turn % 4))) % len(work)]
+            c.qmatmul_scaled(*dev, out=y)
+        if turn % 8 == 7:
+            c.synchronize()
+            for _, y, want in work:
+                assert torch.equal(y, want)
+                y.fill_(77.0)
+            torch.cuda.synchronize()
+    c.set_stream(torch.cuda.default_stream().cuda_stream)
+    c.close()

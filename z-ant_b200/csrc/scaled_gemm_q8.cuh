@@ -197,6 +197,15 @@ __device__ __forceinline__ void scaled_mma_role(const ScaledGemmArgs& a, const S
     }
 }
 
+// The end of a producer's ring: the tensor core has arrived on every stage's barrier.  Nothing else waits for the last round of these arrivals, and
+// one of them must not come when the shared memory (in a pair, the other CTA's) is the next kernel's.
+__device__ __forceinline__ void scaled_drain(const ScaledGemmArgs& a, const ScaledBars& bar, int s, uint32_t ph, volatile int* abort_flag) {
+    for (int i = 0; i < a.stages; ++i) {
+        if (!ptx::mbar_wait(bar.empty(s), ph ^ 1u, abort_flag, a.wait_budget)) return;      // (a stage that was never filled is free)
+        if (++s == a.stages) { s = 0; ph ^= 1u; }
+    }
+}
+
 // An epilogue warp: lane quarter `warp & 3`, the `part`-th of the tile's column ranges.  PAIR: the CTA has half `rank` of the tile's 256 channels,
 // and rank 0 is told when the accumulators are free.  A warp whose wait has given up still walks its tiles, from part barrier to part barrier: the other
 // warps of the part may have had the accumulator, and would stand there.
@@ -312,6 +321,7 @@ __global__ void __launch_bounds__(ScaledCfg<NT>::THREADS, 1) scaled_gemm_kernel(
                     if (++s == a.stages) { s = 0; ph ^= 1u; }
                 }
             }
+            scaled_drain(a, bar, s, ph, abort_flag);
         producer_done:;
         }
     } else if (warp == 1) {
@@ -420,6 +430,7 @@ __global__ void __launch_bounds__(ScaledAny::THREADS, 1) scaled_any_kernel(const
                     if (++s == a.stages) { s = 0; ph ^= 1u; }
                 }
             }
+            scaled_drain(a, bar, s, ph, abort_flag);
         producer_done:;
         }
     } else if (warp == 1) {
@@ -499,6 +510,7 @@ __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel
                     if (++s == a.stages) { s = 0; ph ^= 1u; }
                 }
             }
+            scaled_drain(a, bar, s, ph, abort_flag);
         producer_done:;
         }
     } else if (warp == 1) {
