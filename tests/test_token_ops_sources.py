@@ -1,0 +1,23 @@
+"""Rules of the language-model kernels whose breach shows in no result for certain: read from their sources."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "z-ant_b200", "csrc")
+
+
+def source(name):
+    """The file without its comments."""
+    with open(os.path.join(CSRC, name)) as f:
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+def test_barriers_that_other_ctas_arrive_on_are_waited_for_at_cluster_scope():
+    text = source("scaled_gemm_q8.cuh")
+    pair = text[text.index("scaled_pair_kernel(const __grid_constant__"):text.index("struct ScaledFew")]
+    remote = set(re.findall(r"mbar_arrive_cluster\(ptx::cluster_addr\(bar\.(\w+)\(", text))
+    assert remote == {"tempty"}
+    for name in remote:
+        waits = re.findall(r"(\w+(?:<\w+>)?)\((?:a, )?bar\.%s\([^;]*abort_flag" % name, pair)
+        assert waits and all(w.endswith("<true>") for w in waits), waits
+    ptx = source("ptx_sm100.cuh")
+    assert "mbarrier.try_wait.parity.acquire.cluster" in ptx and "mbarrier.arrive.release.cluster" in ptx

@@ -73,11 +73,16 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}\n" ::"r"(bar), "r"(bytes) : "memory");
 }
+// CLUSTER: other CTAs of the cluster arrive on the barrier by mbar_arrive_cluster, and what they did before is to be seen.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, P;\n\t}\n"
-        : "=r"(ok) : "r"(bar), "r"(parity), "r"(2000u) : "memory");   // may suspend the thread for up to ~2 us before reporting "not yet"
+    uint32_t ok;                                                       // may suspend the thread for up to ~2 us before reporting "not yet"
+    if (CLUSTER)
+        asm volatile("{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, P;\n\t}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(2000u) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, P;\n\t}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(2000u) : "memory");
     return ok != 0;
 }
 
@@ -87,14 +92,15 @@ constexpr long long kWaitBudgetCycles = 4000000000LL;
 // Waits for the phase with the given parity.  Returns false when the budget (in SM clock cycles) ran
 // out or when another role already raised `*abort_flag` (a shared-memory int).  The production kernels
 // use the default budget; the bounded-wait self test passes a budget of microseconds.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           long long budget_cycles = kWaitBudgetCycles) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait<CLUSTER>(bar, parity)) return true;
     const long long t0 = clock64();
     const uint32_t check_mask = budget_cycles < (1LL << 24) ? 3u : 255u;   // short budgets look at the clock more often
     uint32_t spins = 0;
     while (true) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (mbar_try_wait<CLUSTER>(bar, parity)) return true;
         if (++spins > 32) __nanosleep(40);
         if ((spins & check_mask) == 0u) {
             if (*abort_flag) return false;
@@ -341,7 +347,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 // Arrives on a barrier of any CTA of the cluster (cluster_addr); what the thread (and, behind a warp barrier, its warp) wrote to that
-// CTA's memory before is visible to whoever waits for the phase with mbar_wait_cluster.
+// CTA's memory before is visible to whoever waits for the phase with mbar_wait<true>.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }

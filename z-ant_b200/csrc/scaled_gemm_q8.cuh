@@ -164,8 +164,9 @@ struct ScaledBars {
 
 // A wait of a whole warp.  Its lanes leave it together and with one answer: behind it stand instructions and barriers that want all of them (tcgen05.ld,
 // shuffles, the next wait of a ring, in which a lane a phase behind the others would wait for good).
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool scaled_wait(const ScaledGemmArgs& a, uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag, a.wait_budget)) != 0;
+    return __all_sync(0xffffffffu, ptx::mbar_wait<CLUSTER>(bar, parity, abort_flag, a.wait_budget)) != 0;
 }
 
 // The MMA issuer (a whole warp): NT columns per tile of the walk t0, t0 + step, ..
@@ -522,7 +523,7 @@ __global__ void __launch_bounds__(ScaledCfg<256>::THREADS, 1) scaled_pair_kernel
             bool ok = true;
             for (int t = t0; t < tiles && ok; t += step, ++ti) {
                 const int b = ti & 1;
-                ok = scaled_wait(a, bar.tempty(b), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag);
+                ok = scaled_wait<true>(a, bar.tempty(b), ((uint32_t)(ti >> 1) & 1u) ^ 1u, abort_flag);       // both CTAs' epilogues have read this accumulator
                 if (!ok) break;
                 ptx::tc_fence_after();
                 const RowTile rt = row_tile_of(a, grow, gfirst, tile_at(t, row_tiles, a.n_tiles).m, NT);
