@@ -21,3 +21,14 @@ def test_barriers_that_other_ctas_arrive_on_are_waited_for_at_cluster_scope():
         assert waits and all(w.endswith("<true>") for w in waits), waits
     ptx = source("ptx_sm100.cuh")
     assert "mbarrier.try_wait.parity.acquire.cluster" in ptx and "mbarrier.arrive.release.cluster" in ptx
+
+
+def test_what_the_kernel_before_may_write_is_read_by_coherent_loads():
+    """These kernels start beside the one that writes their operands: no load among them is a non-coherent one."""
+    for name in ("quantize_rows.cuh", "scaled_gemm_q8.cuh", "token_logprobs.cuh"):
+        text = source(name)
+        assert "grid_start()" in text or "grid_wait()" in text
+        assert not re.findall(r"__ldg\(|ld_global_nc|\.nc\.", text), name
+    once = source("ptx_sm100.cuh")
+    once = once[once.index("uint4 ld_global_once("):]
+    assert "asm volatile" in once[:once.index("}")] and ".nc" not in once[:once.index("}")]

@@ -14,6 +14,9 @@
 // columns.  A warp that reads one column then holds 32 neighbouring channels of one token and stores them as one line, w_scale and bias
 // belong to the lane, and a last tile of few tokens costs few MMA clocks.  A stage is 128 bytes of k: 128 rows of weights and NT of tokens,
 // K-major operands in the 128-byte swizzle.
+//
+// The kernels start while the one before them still writes their tokens (ptx::grid_wait), so that operands are read by plain loads: the
+// non-coherent ones (__ldg) are for what nobody writes while the kernel runs, and may be moved in front of the wait.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -366,7 +369,7 @@ struct AnyRows {
     __device__ __forceinline__ void fetch(uint4 (&to)[R]) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            to[i] = end[i] > 0 ? __ldg(src[i]) : make_uint4(0, 0, 0, 0);
+            to[i] = end[i] > 0 ? *src[i] : make_uint4(0, 0, 0, 0);
             src[i] += 8;
             end[i] -= 128;
         }
@@ -564,7 +567,7 @@ __device__ __forceinline__ uint4 load16_any(const int8_t* p, int valid) {
     const uint32_t* q = reinterpret_cast<const uint32_t*>(at - sh);
     uint32_t w[5], v[4];
 #pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = (valid > 0 && i * 4 < valid + sh) ? __ldg(q + i) : 0u;
+    for (int i = 0; i < 5; ++i) w[i] = (valid > 0 && i * 4 < valid + sh) ? q[i] : 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[i] = __funnelshift_r(w[i], w[i + 1], sh * 8);
@@ -605,7 +608,7 @@ __global__ void __launch_bounds__(256, PER) scaled_few_kernel(const __grid_const
                 const int k = c * 128 + h * 64, valid = all ? 16 : a.k - k - q * 16;
                 auto get = [&](const int8_t* p, bool once) {
                     if constexpr (ANY) return load16_any(p + k, min(valid, 16));
-                    else return all || valid >= 16 ? (once ? ptx::ld_global_once(reinterpret_cast<const uint4*>(p + k)) : __ldg(reinterpret_cast<const uint4*>(p + k))) : load16_any(p + k, valid);
+                    else return all || valid >= 16 ? (once ? ptx::ld_global_once(reinterpret_cast<const uint4*>(p + k)) : *reinterpret_cast<const uint4*>(p + k)) : load16_any(p + k, valid);
                 };
 #pragma unroll
                 for (int m = 0; m < MT; ++m) { wv[h][m][0] = get(w[m][0], true); wv[h][m][1] = get(w[m][1], true); }

@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     ExpSums s{L::FLOOR * kLog2e, 0.0f, 0.0f};
     float m = L::FLOOR;
     float seen = -INFINITY;                           // the largest of the thread's vectors
-    // Past L1, unless many alternatives are looked for in what has been read (4096 x 65536: 112 -> 103 us with one, 134 -> 140 with 20).
+    // (Plain loads, here and below: the kernel before this one may have written the logits while this one started.)  Past L1, unless many alternatives are looked for in what has been read (4096 x 65536: 112 -> 103 us with one, 134 -> 140 with 20).
     const bool once = a.top <= 8;
     for (int i = tid; i < nv; i += THREADS * U) {
         uint4 v[U];
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
             for (int u = 0; u < U; ++u) v[u] = i + u * THREADS < nv ? ptx::ld_global_once(xv + i + u * THREADS) : make_uint4(L::NONE, L::NONE, L::NONE, L::NONE);
         } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = i + u * THREADS < nv ? __ldg(xv + i + u * THREADS) : make_uint4(L::NONE, L::NONE, L::NONE, L::NONE);
+            for (int u = 0; u < U; ++u) v[u] = i + u * THREADS < nv ? xv[i + u * THREADS] : make_uint4(L::NONE, L::NONE, L::NONE, L::NONE);
         }
         uint32_t best = L::max2(L::max2(v[0].x, v[0].y), L::max2(v[0].z, v[0].w));
 #pragma unroll
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
         const int n_seen = sh.n_seen;
         for (int c = warp; c < n_seen; c += Sh::WARPS)
             for (int i = sh.seen_by[c] + lane * THREADS; i < nv; i += 32 * THREADS) {
-                const uint4 v = __ldg(xv + i);
+                const uint4 v = xv[i];
                 float f[N];
                 L::values(v, f);
 #pragma unroll
