@@ -168,6 +168,9 @@ int32_t zant_b200_ctx_synchronize(zant_ctx* ctx);
  * weights a single-operator call brought along is part of staging them and is not counted. */
 uint64_t zant_b200_ctx_launch_count(zant_ctx* ctx);
 void zant_b200_ctx_reset_launch_count(zant_ctx* ctx);
+/* Name of the kernel that this context launched last (static text, "" before the first launch): with it a test can tell
+ * which of an operator's kernels its sizes and addresses chose.  No reference counterpart. */
+const char* zant_b200_ctx_last_kernel(const zant_ctx* ctx);
 
 /* Attainable int8 tensor-core rate of the context's device in TOP/s: a resident-tile
  * tcgen05.mma kind::i8 loop (128x256x32 per instruction, `iters` x 2 instructions per SM, no

@@ -110,6 +110,7 @@ def lib():
         _lib.zant_b200_last_error.restype = C.c_char_p
         _lib.zant_b200_ctx_stream.restype = C.c_void_p
         _lib.zant_b200_ctx_launch_count.restype = C.c_uint64
+        _lib.zant_b200_ctx_last_kernel.restype = C.c_char_p
         _lib.zant_b200_plan_arena_bytes.restype = C.c_size_t
         _lib.zant_b200_plan_tensor_ptr.restype = C.c_void_p
         _lib.zant_b200_plan_step_name.restype = C.c_char_p
@@ -431,6 +432,10 @@ class Context:
 
     def launch_count(self):
         return int(lib().zant_b200_ctx_launch_count(self._h))
+
+    def last_kernel(self):
+        """Name of the kernel that this context launched last."""
+        return lib().zant_b200_ctx_last_kernel(self._h).decode()
 
     def reset_launch_count(self):
         lib().zant_b200_ctx_reset_launch_count(self._h)

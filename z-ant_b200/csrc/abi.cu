@@ -136,6 +136,7 @@ int32_t zant_b200_ctx_synchronize(zant_ctx* ctx) {
 
 uint64_t zant_b200_ctx_launch_count(zant_ctx* ctx) { return ctx ? ctx->launches : 0; }
 void zant_b200_ctx_reset_launch_count(zant_ctx* ctx) { if (ctx) ctx->launches = 0; }
+const char* zant_b200_ctx_last_kernel(const zant_ctx* ctx) { return ctx ? ctx->last_kernel : ""; }
 
 int32_t zant_b200_measure_int8_peak(zant_ctx* ctx, int32_t iters, double* tera_ops_per_s) {
     ZB_NEED(tera_ops_per_s, "tera_ops_per_s");

@@ -22,6 +22,7 @@ struct zant_ctx {
     size_t arena_used = 0;
     size_t arena_limit = 0;       // 0 = the staging arena may grow on demand; else its hard cap in bytes
     uint64_t launches = 0;
+    const char* last_kernel = "";     // what check_launch saw last
     int sm_count = 148;
     int* status_word = nullptr;   // device int: kernels with bounded waits report here
     zb::HostStage* stage = nullptr;   // page-locked ring for pageable host buffers, created on first use
@@ -102,6 +103,7 @@ inline int32_t check_launch(zant_ctx* ctx, const char* what) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return fail(ZANT_E_CUDA, "launch of %s failed: %s", what, cudaGetErrorString(e));
     ctx->launches++;
+    ctx->last_kernel = what;
     return ZANT_OK;
 }
 

@@ -738,7 +738,7 @@ inline int32_t launch_scaled_tc(zant_ctx* ctx, const char* name, ScaledGemmArgs 
 }
 template <int NT>
 inline int32_t launch_scaled_gemm(zant_ctx* ctx, const ScaledGemmArgs& a) {
-    return launch_scaled_tc<scaled_gemm_kernel<NT>>(ctx, "scaled_gemm_kernel", a, ScaledCfg<NT>::STAGE, ScaledCfg<NT>::THREADS, NT, 128, 128, NT, 1);
+    return launch_scaled_tc<scaled_gemm_kernel<NT>>(ctx, NT == 64 ? "scaled_gemm_kernel<64>" : NT == 128 ? "scaled_gemm_kernel<128>" : "scaled_gemm_kernel<256>", a, ScaledCfg<NT>::STAGE, ScaledCfg<NT>::THREADS, NT, 128, 128, NT, 1);
 }
 inline int32_t launch_scaled_pair(zant_ctx* ctx, const ScaledGemmArgs& a) {
     return launch_scaled_tc<scaled_pair_kernel>(ctx, "scaled_pair_kernel", a, ScaledCfg<256>::STAGE_W + 128 * 128, ScaledCfg<256>::THREADS, 256, 256, 128, 128, 2);
