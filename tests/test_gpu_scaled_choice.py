@@ -58,6 +58,20 @@ def test_rows_read_where_they_are(tight, rows, k, n, off, kernel):
         sampled(torch, y, ops, "f16")
 
 
+@pytest.mark.parametrize("groups,rows,n", [(16, 528, 256), (30, 990, 128)])
+def test_groups_at_odd_addresses_are_laid_out(ctx, tight, groups, rows, n):
+    """Groups of 33 rows: few tiles if they lay side by side, too many for the few-token kernel as groups.  Where the arena has room they are laid out."""
+    import torch
+    k = 1001
+    offsets = np.arange(groups + 1) * 33
+    ops = operands(np.random.default_rng(rows), rows, k, n, groups)
+    y = grouped(ctx, torch, ops, offsets, "f32")
+    assert ctx.last_kernel() in GEMM.values()
+    check_groups(y, ops, offsets, "f32")
+    there = grouped(tight, torch, ops, offsets, "f32")
+    assert tight.last_kernel() == ANY and torch.equal(y, there)
+
+
 def test_in_a_graph(zb):
     """Each kernel captured, pairs of CTAs among them, and replayed on new values."""
     import torch

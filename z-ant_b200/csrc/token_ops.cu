@@ -66,6 +66,7 @@ inline int32_t scaled_gemm_entry(zant_ctx* ctx, const int8_t* a, size_t rows, si
     ScaledGemmArgs p{};
     p.a = a; p.a_stride = (long long)a_stride; p.w = w; p.w_stride = (long long)w_stride; p.y_stride = (long long)y_stride;
     p.rows = (int)rows; p.n = (int)n; p.k = (int)k; p.groups = (int)groups;
+    p.offsets = offsets;                              // (the choice of the kernel asks whether there are any)
     // Device rows that the TMA cannot read are laid out in the arena, if it holds them as it is and the call is not captured.
     size_t align_a = scaled_align_bytes(p, false, ctx->sm_count), align_w = scaled_align_bytes(p, true, ctx->sm_count);
     if ((align_a || align_w) && (align_a + align_w + 2 * kArenaAlign > ctx->arena_bytes || stream_capturing(ctx) || !is_device_ptr(a) || !is_device_ptr(w))) align_a = align_w = 0;
