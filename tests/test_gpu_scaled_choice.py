@@ -110,3 +110,24 @@ def test_in_a_graph(zb):
 def test_name_before_the_first_launch(zb):
     with zb.Context(0) as c:
         assert c.last_kernel() == ""
+
+
+def test_a_host_result_beside_rows_to_lay_out(zb):
+    """An arena that holds the host result but not the operands as well: they are read where they are, and a limit on the arena refuses nothing."""
+    import torch
+    rows, k, n = 200, 999, 300
+    ops = operands(np.random.default_rng(21), rows, k, n)
+    dev = [torch.from_numpy(v).cuda() for v in ops[:4]]
+    torch.cuda.synchronize()
+    laid_out = (rows + n) * 1008 + 512
+    size = max(laid_out, rows * n * 4 + 256) + 4096        # either has room, both have not
+    with zb.Context(0, arena_bytes=size) as c:
+        c.set_arena_limit(size)
+        y = torch.zeros(rows, n, device="cuda")
+        torch.cuda.synchronize()
+        c.qmatmul_scaled(*dev, out=y)
+        assert c.last_kernel() in GEMM.values()
+        c.synchronize()
+        host = c.qmatmul_scaled(*dev)
+        assert c.last_kernel() == ANY and np.array_equal(host, y.cpu().numpy())
+        sampled(torch, y, ops, "f32")

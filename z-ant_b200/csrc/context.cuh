@@ -326,6 +326,9 @@ class Stager {
         return (int)slots_.size() - 1;
     }
 
+    // The arena as it is has room for every staged slot and `more` bytes.
+    bool holds(size_t more) { return layout() + more <= ctx_->arena_bytes; }
+
     // Arena space for every staged slot.  False when the arena may not or cannot grow that far: a kernel that wants less workspace is
     // tried then.  (Anything else that is wrong with the buffers is left to commit.)
     bool room() {

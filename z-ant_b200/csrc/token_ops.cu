@@ -67,13 +67,15 @@ inline int32_t scaled_gemm_entry(zant_ctx* ctx, const int8_t* a, size_t rows, si
     p.a = a; p.a_stride = (long long)a_stride; p.w = w; p.w_stride = (long long)w_stride; p.y_stride = (long long)y_stride;
     p.rows = (int)rows; p.n = (int)n; p.k = (int)k; p.groups = (int)groups;
     p.offsets = offsets;                              // (the choice of the kernel asks whether there are any)
-    // Device rows that the TMA cannot read are laid out in the arena, if it holds them as it is and the call is not captured.
+    // Device rows that the TMA cannot read are laid out in the arena, if it holds them as it is (beside what host arrays of the call take) and the
+    // call is not captured.
     size_t align_a = scaled_align_bytes(p, false, ctx->sm_count), align_w = scaled_align_bytes(p, true, ctx->sm_count);
-    if ((align_a || align_w) && (align_a + align_w + 2 * kArenaAlign > ctx->arena_bytes || stream_capturing(ctx) || !is_device_ptr(a) || !is_device_ptr(w))) align_a = align_w = 0;
     Stager s(ctx);
     const int ia = s.in(a, a_bytes), ias = s.in(a_scale, rows * 4), iw = s.in(w, w_bytes), iws = s.in(w_scale, groups * n * 4), ib = s.in(bias, groups * n * 4);
     const int io = s.in(grouped ? offsets : nullptr, (groups + 1) * 4);
     const int iy = grouped || y_stride != n ? s.inout(y, y_bytes) : s.out(y, y_bytes);
+    if ((align_a || align_w) && (!s.holds(align_up(align_a, kArenaAlign) + align_up(align_w, kArenaAlign)) || stream_capturing(ctx) || !is_device_ptr(a) || !is_device_ptr(w)))
+        align_a = align_w = 0;
     const int ila = align_a ? s.scratch(align_a) : -1, ilw = align_w ? s.scratch(align_w) : -1;
     ZB_TRY(s.commit());
     p.a = s.ptr<int8_t>(ia); p.a_scale = s.ptr<float>(ias); p.w = s.ptr<int8_t>(iw); p.w_scale = s.ptr<float>(iws);
