@@ -4,9 +4,11 @@
 // One pass over the logits.  A thread keeps its own maximum, S and W, four 16-byte vectors at a time, and rescales when a batch raises its
 // maximum; the parts are joined at the end.  Everything is in units of log 2: d = x log2(e) - m log2(e) is one fused operation for two
 // logits, and the rounding of m log2(e), which all terms of a sum share, cancels in log p and the entropy because the token's own d is
-// taken the same way.  Logits of minus infinity are taken as a lowest value that no other term sees (a product of zero and infinity would
-// spoil W); rows for which that is not so (their maximum is about as low), rows about as large as their type can be, and rows with a NaN
-// or plus infinity go through a plain second form, one pass a result.
+// taken the same way, as long as it is a fraction of 1: from a maximum of 2^22 on it would be more than the differences themselves, and the
+// powers overflow or vanish (rows of -1e10 throughout, say, as a mask leaves them).  Logits of minus infinity are taken as a lowest value that no
+// other term sees (a product of zero and infinity would spoil W).  Rows whose maximum is beyond 2^22 to either side (in f16, so low that the
+// lowest value is seen) have their sums taken again in a plain second form, a pass each; rows with a NaN or plus infinity their alternatives
+// too, a pass each.
 //
 // The alternatives: tau, the n-th largest of the threads' maxima, is a lower bound of the n-th largest logit, and only threads whose maximum
 // reaches it have seen a logit that does.  About n threads do; their vectors (V / threads logits each) are read again, from L2, what
@@ -46,11 +48,11 @@ __device__ __forceinline__ unsigned long long key_of(uint32_t order, int id) { r
 
 // 16 bytes of logits.  LOW: bits of a float that its values leave 0; FLOOR: a thread's maximum before it has seen one; what stands for minus
 // infinity is FLOOR in f16, below it in the others, where the rounding of FLOOR log2(e) leaves a difference whose power would overflow;
-// LEAST: a maximum that both are far enough below to add nothing; MOST: one whose product with log2(e) is finite.
+// LEAST, MOST: between them a row's maximum leaves the rounding of m log2(e) a quarter at most, and the first two so far below that they add nothing.
 template <typename T> struct Logits;
 template <> struct Logits<float> {
     static constexpr int N = 4, LOW = 0;
-    static constexpr float FLOOR = -1e30f, LEAST = -0.9e30f, MOST = 1e38f;
+    static constexpr float FLOOR = -1e30f, LEAST = -4194304.0f, MOST = 4194304.0f;
     static constexpr uint32_t NONE = 0xff800000u;
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
     static __device__ __forceinline__ float max1(uint32_t a) { return __uint_as_float(a); }
@@ -59,7 +61,7 @@ template <> struct Logits<float> {
 };
 template <> struct Logits<__nv_bfloat16> {
     static constexpr int N = 8, LOW = 16;
-    static constexpr float FLOOR = -1e30f, LEAST = -0.9e30f, MOST = 1e38f;
+    static constexpr float FLOOR = -1e30f, LEAST = -4194304.0f, MOST = 4194304.0f;
     static constexpr uint32_t NONE = 0xff80ff80u, FLOOR2 = 0xf14af14au;       // -1.0002e30
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t r; asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
     static __device__ __forceinline__ uint32_t floored2(uint32_t a) { uint32_t r; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(FLOOR2)); return r; }
@@ -138,9 +140,9 @@ __device__ __forceinline__ V block_reduce(V v, V* part, F f) {
     return v;
 }
 
-// The plain form, one CTA, a pass for the maximum, one for the sums and one for each alternative.
+// The plain form, one CTA, a pass for the maximum, one for the sums and one for each alternative.  LISTED: the alternatives are known, sh.lists[0].
 template <typename T, typename Sh>
-__device__ __noinline__ void token_logprobs_plain(const TokenLogprobsArgs& a, long long r, Sh& sh) {
+__device__ __noinline__ void token_logprobs_plain(const TokenLogprobsArgs& a, long long r, bool listed, Sh& sh) {
     const T* x = static_cast<const T*>(a.x) + r * a.stride;
     const int step = blockDim.x;
     float m = -INFINITY;
@@ -163,6 +165,14 @@ __device__ __noinline__ void token_logprobs_plain(const TokenLogprobsArgs& a, lo
             a.logprob[r] = t < 0 ? 0.0f : (t >= a.vocab ? __uint_as_float(0x7fffffffu) : logp(as_float(x[t])));
         }
         if (a.entropy) a.entropy[r] = S == 0.0f ? 0.0f : ls - W / S;
+    }
+    if (listed) {
+        if (threadIdx.x < a.top) {
+            const int id = (int)~(uint32_t)sh.lists[0][threadIdx.x];
+            a.top_ids[r * a.top + threadIdx.x] = id;
+            a.top_logprobs[r * a.top + threadIdx.x] = logp(as_float(x[id]));
+        }
+        return;
     }
     unsigned long long last = ~0ull;
     for (int i = 0; i < a.top; ++i) {
@@ -395,7 +405,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
         h = fmaxf(h, sh.part_top[i]);
         odd |= sh.part_odd[i];
     }
-    if (odd || !(t.S < INFINITY) || !(h > L::LEAST) || !(h < L::MOST)) { token_logprobs_plain<T>(a, r, sh); return; }
+    // (Ranked as floats the alternatives are right whatever the sums are, but for a NaN, which makes S one: a thread's maximum does not see it.)
+    if (odd || !(t.S < INFINITY) || !(h > L::LEAST) || !(h < L::MOST)) { token_logprobs_plain<T>(a, r, !odd && t.S == t.S, sh); return; }
     const float ls = log2f(t.S);
     auto logp = [&](float v) {
         const float p = (fmaf(v, kLog2e, -t.m) - ls) * kLn2;
