@@ -264,12 +264,19 @@ def _matrices(a, what):
 
 
 def _values(a, n, code, what, result=False):
-    """(array to keep, address) of `n` dense values of type `code`; numpy arrays are cast, those for a result must be what they are said to be."""
+    """(array to keep, address) of `n` dense values of type `code`; numpy arrays are cast, those for a result must be what they are said to be.
+    Whole numbers beyond int32 become its ends, which mean the same: an index, a token or an offset outside."""
     try:
         ptr = a.data_ptr()
     except AttributeError:
         if result and (not isinstance(a, np.ndarray) or _ROW_DTYPE.get(a.dtype) != code or not a.flags.c_contiguous):
             raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array of its type") from None
+        if code == I32 and not result:
+            a = np.asarray(a)
+            if a.dtype.kind not in "iub" and a.size:
+                raise ZantError(-34, "InputArrayWrongType", f"{what} is {a.dtype}, not whole numbers") from None
+            if a.dtype.itemsize >= 4 and a.dtype != np.int32:
+                a = np.clip(a, -2 ** 31, 2 ** 31 - 1) if a.dtype.kind == "i" else np.minimum(a, 2 ** 31 - 1)
         a = np.ascontiguousarray(a, dtype=NP_DTYPE[code])
         if a.size != n:
             raise ZantError(-35, "InputArrayWrongSize", f"{what} holds {a.size} values, not {n}") from None
