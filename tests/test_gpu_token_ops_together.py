@@ -167,3 +167,38 @@ def test_launches_are_counted(ctx):
     b.run()
     ctx.synchronize()
     assert ctx.launch_count() - before == 11
+
+
+def test_each_call_with_host_operands_is_refused_in_a_capture(zb):
+    """With results of the right size on the device, so that nothing but the host operand is refused, by the library and with its reason."""
+    import torch
+    c = zb.Context(0)
+    stream = torch.cuda.Stream()
+    c.set_stream(stream.cuda_stream)
+    x = torch.ones(4, 64, device="cuda")
+    q, s = torch.zeros(4, 64, dtype=torch.int8, device="cuda"), torch.zeros(4, device="cuda")
+    w, ws, off = torch.ones(5, 64, dtype=torch.int8, device="cuda"), torch.ones(5, device="cuda"), torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    y, lp, h, none = torch.full((4, 5), 7.0, device="cuda"), torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda"), (torch.zeros(4, 0, dtype=torch.int32, device="cuda"), torch.zeros(4, 0, device="cuda"))
+    ones = np.ones
+    refused = [lambda: c.quantize_rows(ones((4, 64), np.float32), out=q, out_scale=s), lambda: c.quantize_rows(x, index=[0, 1, 2, 3], out=q, out_scale=s),
+               lambda: c.qmatmul_scaled(q, s, ones((5, 64), np.int8), ws, out=y), lambda: c.qmatmul_scaled(ones((4, 64), np.int8), s, w, ws, out=y),
+               lambda: c.qmatmul_scaled(q, s, w, ones(5, np.float32), out=y), lambda: c.qmatmul_scaled(q, s, w, ws, out=torch.zeros(4, 5)),
+               lambda: c.qmatmul_grouped(q, s, w[None], ws[None], [0, 4], out=y), lambda: c.token_logprobs(x, [1, 2, 3, 4], out=(lp, h) + none)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+        c.quantize_rows(x, out=q, out_scale=s)
+        for call in refused:
+            with pytest.raises(zb.ZantError) as e:
+                call()
+            assert "cannot be captured" in str(e.value)
+        c.qmatmul_grouped(q, s, w[None], ws[None], off, out=y)
+    torch.cuda.synchronize()
+    assert (y == 7).all()
+    graph.replay()
+    torch.cuda.synchronize()
+    # sums of 64 * 127, times a scale of 1 / 127 that was rounded once, and two products that round once each
+    assert ((y.double() - 64.0).abs() <= 64 * 3.1 * ref.U).all()
+    del graph
+    c.set_stream(torch.cuda.default_stream().cuda_stream)
+    c.close()
