@@ -108,3 +108,13 @@ def test_status_mapping_is_total():
     for code, zig_name in re.findall(r"^\s*(-\d+) => \w+\.(\w+),", check, flags=re.M):
         c_name = re.search(r"ZANT_E_(\w+) = " + code + r"\b", enum).group(1)
         assert c_name.replace("_", "").lower() == zig_name.lower(), (code, c_name, zig_name)
+
+
+def test_log_probabilities_of_no_rows_are_nothing_to_do():
+    """Alternatives asked for or not: no rows are no error, and nothing is divided by their number."""
+    src, _fns, _types, _externs = shim_symbols()
+    body = src[src.index("pub fn token_logprobs_lean("):]
+    body = body[:body.index("\n}\n")]
+    assert "rows == 0 or" not in body
+    guard = body.index("if (rows > 0) {")
+    assert all(m.start() > guard for m in re.finditer(r"[%/] rows", body))

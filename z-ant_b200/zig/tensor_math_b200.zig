@@ -521,8 +521,11 @@ pub fn token_logprobs_lean(comptime T: type, logits: *const Tensor(T), tokens: *
     var top: usize = 0;
     if (top_ids) |ids| {
         if (top_logprobs == null) return B200Error.NullPointer;
-        if (rows == 0 or ids.size % rows != 0 or ids.size / rows > 32 or top_logprobs.?.size != ids.size) return TensorMathError.OutputTensorDifferentSize;
-        top = ids.size / rows;
+        if (top_logprobs.?.size != ids.size or (rows == 0 and ids.size != 0)) return TensorMathError.OutputTensorDifferentSize;
+        if (rows > 0) { // no rows: nothing to do, as in the other calls
+            if (ids.size % rows != 0 or ids.size / rows > 32) return TensorMathError.OutputTensorDifferentSize;
+            top = ids.size / rows;
+        }
     }
     try check(zant_b200_token_logprobs(context(), rowTypeOf(T), logits.data.ptr, rows, logits.shape[1], 0, tokens.data.ptr, logprob.data.ptr, entropy.data.ptr, @intCast(top), if (top_ids) |t| t.data.ptr else null, if (top_logprobs) |t| t.data.ptr else null));
 }
