@@ -196,7 +196,7 @@ int32_t zant_b200_selftest_bounded_wait(zant_ctx* ctx, uint32_t budget_us);
  * `cta`, modulo the launch's CTAs, acts as if its first bounded wait had run out: it fetches no further weights and gives
  * up later waits soon.  That run reports
  * ZANT_E_DEVICE_TIMEOUT as zant_b200_selftest_bounded_wait describes, and the runs after it are right again.
- * A negative `cta` disarms it. */
+ * A negative `cta` disarms it.  A launch that is being captured counts: each replay of it gives up. */
 int32_t zant_b200_selftest_give_up(zant_ctx* ctx, int32_t cta);
 
 /* Test hook (no reference counterpart): makes the `nth` next device allocation of this library

@@ -339,9 +339,9 @@ __global__ void __launch_bounds__(ScaledCfg<NT>::THREADS, 1) scaled_gemm_kernel(
 // ------------------------------------------------------------------------------------------------------------------------------
 // Rows that start anywhere.  Sixteen warps read the aligned 16-byte blocks that a row's 16-byte chunks begin in (only blocks that hold a byte of the
 // row), two or three stages ahead in registers, get the following block from the lane that has it, shift the two and write the chunk where the TMA
-// would have.  An operand that the TMA can read comes by TMA all the same.  (257 x 4095 x 5001: 30 us, as long as with asynchronous copies to a
-// ring of raw rows and other warps that shift from there; the loads bound both.  Calls that may use the context's arena lay such rows
-// out first, scaled_align_kernel, and take the TMA's kernels: 20 us.)
+// would have.  An operand that the TMA can read comes by TMA all the same.  (257 x 4095 x 5001: 30 us with odd weights, 43 with odd tokens too;
+// 30 also with asynchronous copies to a ring of raw rows and other warps that shift from there; the loads bound both.  Calls that may use the
+// context's arena lay such rows out first, scaled_align_kernel, and take the TMA's kernels: 20 us.)
 //
 //   warp 0  TMA        warp 1  TMEM owner, MMA issuer        warps 2 .. 9  epilogue        10 .. 25  loaders
 struct ScaledAny {

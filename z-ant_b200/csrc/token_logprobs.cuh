@@ -13,7 +13,8 @@
 // The alternatives: tau, the n-th largest of the threads' maxima, is a lower bound of the n-th largest logit, and only threads whose maximum
 // reaches it have seen a logit that does.  About n threads do; their vectors (V / threads logits each) are read again, from L2, what
 // reaches tau is collected, and each candidate's rank among them is its place in the result.  Equal logits rank by id; where hundreds of
-// them equal tau (a mask that leaves fewer than n tokens), the row is read from its start for the lowest ids.
+// them equal tau (a mask that leaves fewer than n tokens), the row is read from its start for the lowest ids.  That is slow: where a CTA has fewer
+// than n threads with an unmasked logit, tau is the mask's value (64 x 128000 bf16, n = 20: 12 us with 99 % masked, 69 with 99.99 %).
 //
 // Few rows: a cluster of 2, 4 or 8 CTAs shares a row; the first joins the sums and the lists, which come by distributed shared memory.
 #pragma once
