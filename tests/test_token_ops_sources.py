@@ -32,3 +32,14 @@ def test_what_the_kernel_before_may_write_is_read_by_coherent_loads():
     once = source("ptx_sm100.cuh")
     once = once[once.index("uint4 ld_global_once("):]
     assert "asm volatile" in once[:once.index("}")] and ".nc" not in once[:once.index("}")]
+
+
+def test_lanes_come_together_in_front_of_instructions_of_the_whole_warp():
+    """tcgen05.ld, mma.sync and barrier.cluster are executed by all lanes of a warp at once: behind stores, loads or branches of single lanes stands a warp barrier."""
+    gemm, logp = source("scaled_gemm_q8.cuh"), source("token_logprobs.cuh")
+    epilogue = gemm[gemm.index("tmem_ld32("):gemm.index("tc_fence_before", gemm.index("tmem_ld32("))]
+    assert re.search(r"store_columns_any\([^;]*;\s*if \(!all_live\) __syncwarp\(\);\s*\}", epilogue)
+    step = gemm[gemm.index("auto step = [&](int c, bool all)"):gemm.index("mma_m16n8k32_s8(")]
+    assert re.search(r"if \(ANY \|\| !all\) __syncwarp\(\);", step)
+    for m in re.finditer(r"cluster_arrive\(\)", logp):
+        assert re.search(r"__syncwarp\(\);\s*(if \(P > 1\) )?ptx::$", logp[:m.start()])

@@ -224,7 +224,7 @@ __device__ __forceinline__ void scaled_epilogue_role(const ScaledGemmArgs& a, co
         const TileAt at = tile_at(t, row_tiles, a.n_tiles);
         const RowTile rt = row_tile_of(a, grow, gfirst, at.m, NT);
         const int n = (PAIR ? at.n * 256 + rank * 128 : at.n * 128) + quarter * 32 + lane, b = ti & 1;
-        const bool live = n < a.n;
+        const bool live = n < a.n, all_live = n - lane + 32 <= a.n;
         const long long wat = (long long)rt.group * a.n + n;
         const float ws = live ? a.w_scale[wat] : 0.0f, bias = live && a.bias ? a.bias[wat] : 0.0f;
         const int col0 = part * Cfg::COLS, cols = min(Cfg::COLS, rt.rows - col0), own = quarter * (Cfg::COLS / 4) + lane;
@@ -243,6 +243,7 @@ __device__ __forceinline__ void scaled_epilogue_role(const ScaledGemmArgs& a, co
             ptx::tmem_ld32(taddr + (uint32_t)c, v);
             ptx::tmem_wait_ld32(v);
             store_columns_any(a, v, (long long)rt.row + col0 + c, n, cols - c, scales + c, ws, bias);
+            if (!all_live) __syncwarp();              // (lanes without a channel store nothing; the next load wants them all)
         }
         ptx::tc_fence_before();
         __syncwarp();
@@ -615,6 +616,7 @@ __global__ void __launch_bounds__(256, PER) scaled_few_kernel(const __grid_const
 #pragma unroll
                 for (int i = 0; i < NTL; ++i) xv[h][i] = get(x[i], false);
             }
+            if (ANY || !all) __syncwarp();            // (which words a lane reads is its own; the MMAs want all lanes)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll

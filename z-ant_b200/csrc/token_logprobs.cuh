@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     const int part = P > 1 ? (int)ptx::cluster_rank() : 0;
     const long long r = (long long)blockIdx.x / P;
     if (tid == 0) sh.n_seen = sh.n_over = sh.n_equal = 0;
+    __syncwarp();
     if (P > 1) ptx::cluster_arrive();                 // its shared memory may be written to
     ptx::grid_start();
     const T* row = static_cast<const T*>(a.x) + r * a.stride;
