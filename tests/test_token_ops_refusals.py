@@ -164,3 +164,22 @@ def test_other_operators_refuse_the_new_types(zb):
     for dtype in (4, 5):
         assert L.zant_b200_status_name(C.c_int32(L.zant_b200_transpose_onnx(None, C.c_int32(dtype), C.c_void_p(p), sh, C.c_size_t(2), None, C.c_size_t(0), C.c_void_p(p), sh, C.c_size_t(2)))) == b"InputArrayWrongType"
         assert L.zant_b200_status_name(C.c_int32(L.zant_b200_dequantize_linear(None, dtype, p, 8, 1.0, 0, p))) == b"InputArrayWrongType"
+
+
+def test_results_that_may_not_be_written(zb, nogpu):
+    """Read-only arrays (of bytes, of a file mapped for reading) are refused where a result would go."""
+    def ro(v):
+        v.flags.writeable = False
+        return v
+    x, a, s, w, ws = np.ones((3, 8), F), np.ones((3, 8), np.int8), np.ones(3, F), np.ones((5, 8), np.int8), np.ones(5, F)
+    fixed = np.frombuffer(bytes(24), np.int8).reshape(3, 8)
+    refused(zb, "InputArrayWrongType", lambda: nogpu.quantize_rows(x, out=fixed))
+    refused(zb, "InputArrayWrongType", lambda: nogpu.quantize_rows(x, out_scale=ro(np.zeros(3, F))))
+    refused(zb, "InputArrayWrongType", lambda: nogpu.qmatmul_scaled(a, s, w, ws, out=ro(np.zeros((3, 5), F))))
+    refused(zb, "InputArrayWrongType", lambda: nogpu.qmatmul_grouped(a, s, w[None], ws[None], [0, 3], out=ro(np.zeros((3, 5), F))))
+    good = [np.zeros(3, F), np.zeros(3, F), np.zeros((3, 2), np.int32), np.zeros((3, 2), F)]
+    for i in range(4):
+        out = [v.copy() for v in good]
+        ro(out[i])
+        refused(zb, "InputArrayWrongType", lambda: nogpu.token_logprobs(x, [0, 1, 2], top=2, out=tuple(out)))
+    refused(zb, "CudaUnavailable", lambda: nogpu.token_logprobs(ro(x), ro(np.zeros(3, np.int32)), top=2, out=tuple(good)))

@@ -220,8 +220,8 @@ def _rows(a, what, result=False):
     try:
         ptr = a.data_ptr()
     except AttributeError:
-        if result and (not isinstance(a, np.ndarray) or not a.flags.c_contiguous):
-            raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array") from None
+        if result and (not isinstance(a, np.ndarray) or not a.flags.c_contiguous or not a.flags.writeable):
+            raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array that may be written") from None
         a = np.asarray(a)
         if a.ndim != 2:
             raise ZantError(-59, "InvalidRank", f"{what} has {a.ndim} dimensions, not 2") from None
@@ -269,8 +269,8 @@ def _values(a, n, code, what, result=False):
     try:
         ptr = a.data_ptr()
     except AttributeError:
-        if result and (not isinstance(a, np.ndarray) or _ROW_DTYPE.get(a.dtype) != code or not a.flags.c_contiguous):
-            raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array of its type") from None
+        if result and (not isinstance(a, np.ndarray) or _ROW_DTYPE.get(a.dtype) != code or not a.flags.c_contiguous or not a.flags.writeable):
+            raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array of its type that may be written") from None
         if code == I32 and not result:
             a = np.asarray(a)
             if a.dtype.kind not in "iub" and a.size:
