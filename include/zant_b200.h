@@ -88,8 +88,8 @@ typedef enum zant_dtype {
     ZANT_I8 = 1,
     ZANT_U8 = 2,
     ZANT_I32 = 3,
-    /* Taken by the operators that name them (quantize_rows, qmatmul_scaled, qmatmul_grouped, token_logprobs); all others
-     * return ZANT_E_INPUT_ARRAY_WRONG_TYPE. */
+    /* Taken by the operators that name them (quantize_rows, qmatmul_scaled, qmatmul_grouped, token_logprobs, kv_cache_write,
+     * kv_cache_read, kv_cache_attention, verify_drafts); all others return ZANT_E_INPUT_ARRAY_WRONG_TYPE. */
     ZANT_F16 = 4,
     ZANT_BF16 = 5
 } zant_dtype;
@@ -621,6 +621,70 @@ int32_t zant_b200_qmatmul_grouped(zant_ctx* ctx, const int8_t* a, size_t rows, s
 int32_t zant_b200_token_logprobs(zant_ctx* ctx, int32_t dtype, const void* logits, size_t rows, size_t vocab, size_t stride,
                                  const int32_t* tokens, float* logprob, float* entropy,
                                  int32_t top, int32_t* top_ids, float* top_logprobs);
+
+/* ------------------------------------------------------------------------------------------
+ * A decoder's key-value cache in 8 bits, attention over it, and the check of drafted tokens: for the layers and the logits that the operators above
+ * compute.  The same rules hold (strides, alignment, capture, calls with no rows).
+ *
+ * The cache is pages of tokens.  Codes are [pages, heads, page, dim], one scale for each page and head is [pages, heads], keys and values alike; a cached value is
+ * code * scale.  `page` is 16, 32, 64, 128 or 256 tokens (else InvalidInput), `dim` a multiple of 16 up to 256 (else UnsupportedDimension).  Codes in device memory
+ * start at a multiple of 16 bytes (InvalidInput).
+ *
+ * The sequences of a call: page i of sequence s is table[s, i] (table [seqs, width], int32); lengths[s] tokens of it are in the cache, the call's new ones
+ * included.  The new tokens of all sequences are the rows of one matrix, those of sequence s the rows offsets[s] to offsets[s + 1] - 1 (seqs + 1 values; NULL:
+ * rows / seqs each, InputTensorDifferentSize where that leaves some), and they are the last ones of the sequence: row i of n stands at position
+ * lengths[s] - n + i.  A row has the heads behind one another, [heads * dim].
+ * Table, lengths and offsets are read on the device, and any values are safe: lengths are taken as clamped to [0, width * page], offsets to [0, rows];
+ * a sequence whose offsets decrease has no rows; of offsets that are out of order it is not defined which rows a sequence has.  A page outside the cache (-1 by custom, for pages
+ * that a window has left behind) is not written, reads as zeros and is seen by no query.  Rows that belong to no sequence are left as they were in the results.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct zant_kv_cache {
+    int8_t* k; float* k_scale;
+    int8_t* v; float* v_scale;
+    size_t pages, heads, page, dim;
+} zant_kv_cache;
+
+/* Quantizes the keys and values of new tokens (F32, F16 or BF16) into their places.  For each page and head, keys and values apart, with
+ * m = the largest magnitude of the new values there:
+ *   scale' = max(scale, m / 127)                        (fp32 division; scale is taken as 0 where the page's first token is among the new ones)
+ *   codes of new tokens:  the integer nearest to x / scale', ties to even
+ *   codes of the tokens before them in the page, where the scale grows:  the integer nearest to code * scale / scale', ties to even
+ * Quotients are the exact ones.  Where scale' is 0 codes are 0.  A NaN or an infinity makes the scale of its page and head NaN and its codes 0, until the page begins anew.
+ * Codes behind the sequence's last token are left as they were.  A token at a negative position is not written.  A page that two sequences write in one
+ * call holds the tokens of either or of both. */
+int32_t zant_b200_kv_cache_write(zant_ctx* ctx, const zant_kv_cache* cache, int32_t dtype,
+                                 const void* k, size_t k_stride, const void* v, size_t v_stride, size_t rows,
+                                 const int32_t* table, size_t seqs, size_t width, const int32_t* lengths, const int32_t* offsets);
+
+/* Brings cached tokens back as rows: the last offsets[s + 1] - offsets[s] tokens of sequence s, code * scale in fp32, rounded to `dtype`.  k or v may be NULL.
+ * Positions below zero read as zeros. */
+int32_t zant_b200_kv_cache_read(zant_ctx* ctx, const zant_kv_cache* cache, int32_t dtype,
+                                void* k, size_t k_stride, void* v, size_t v_stride, size_t rows,
+                                const int32_t* table, size_t seqs, size_t width, const int32_t* lengths, const int32_t* offsets);
+
+/* Attention of new tokens, whose keys and values are in the cache already, over their sequences:
+ *   out[r, h] = sum over j of w_j v_j,   w = softmax over the seen j of  scale * q[r, h] . k_j
+ * q and out are [rows, heads * dim] of one type; `heads` is a multiple of the cache's, head h reads the cache's head h / (heads / cache heads) (InputTensorsWrongShape).
+ * The token at position i sees position j where j <= i and, with window > 0, j > i - window or j < sinks; window 0 is none.  A query that sees nothing has the result 0.
+ * lse [rows, heads] fp32, may be NULL: the logarithm of the sum of exp(scale * q . k_j), minus infinity where nothing is seen.
+ * Weights and sums are fp32; weights are rounded to f16 in front of the product with v where the result has 16 bits, and to 22 bits where it is F32.  A query with
+ * a NaN or an infinity, and one that sees a page with a scale of NaN, has NaN. */
+int32_t zant_b200_kv_cache_attention(zant_ctx* ctx, const zant_kv_cache* cache, int32_t dtype, const void* q, size_t q_stride, size_t rows, size_t heads,
+                                     const int32_t* table, size_t seqs, size_t width, const int32_t* lengths, const int32_t* offsets,
+                                     float scale, int32_t window, int32_t sinks, void* out, size_t out_stride, float* lse);
+
+/* Which drafted tokens stand against the target model's probabilities, and the token that follows them (speculative decoding).  Sequence s has the drafts offsets[s] to
+ * offsets[s + 1] - 1 (NULL: drafts / seqs each) and one row of `target` more than it has drafts: rows offsets[s] + s to offsets[s + 1] + s of [drafts + seqs, vocab].  `drafted`
+ * [drafts, vocab] are the probabilities that the tokens were drawn from, NULL where the draft model was certain of each.  Both F32, F16 or BF16.
+ *   draft i stands while  accept[i] * drafted[i, t] < target[i + s, t],  t = tokens[i]     (with NULL: accept[i] < target[i + s, t])
+ *   accepted[s] = the drafts before the first that does not stand
+ *   next[s]     = the least v with  sum over w <= v of r_w  >  sample[s] * sum of r,   r = max(target - drafted, 0) of the row of the draft that did not stand (with
+ *                 NULL: target without that draft), the row of the target itself where all stand or that leaves nothing
+ * accept holds `drafts` numbers in [0, 1), sample `seqs`.  Products and differences are exact, sums fp64.  A negative token ends a sequence's drafts (padding), one >= vocab does not stand.
+ * Probabilities that are NaN, negative or infinite count as 0 in r; where nothing is left next is -1. */
+int32_t zant_b200_verify_drafts(zant_ctx* ctx, int32_t dtype, const void* target, size_t target_stride, const void* drafted, size_t drafted_stride, size_t vocab,
+                                const int32_t* tokens, size_t drafts, const int32_t* offsets, size_t seqs, const float* accept, const float* sample,
+                                int32_t* accepted, int32_t* next);
 
 /* ------------------------------------------------------------------------------------------
  * Plan: the run-time form of a generated predict() (src/codeGen/predict.zig:23-70).  One

@@ -22,7 +22,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libzant_b200.so")
 
 F32, I8, U8, I32 = 0, 1, 2, 3
-F16, BF16 = 4, 5        # quantize_rows, qmatmul_scaled, qmatmul_grouped and token_logprobs only
+F16, BF16 = 4, 5        # quantize_rows, qmatmul_scaled, qmatmul_grouped, token_logprobs, the kv_cache operators and verify_drafts only
 NP_DTYPE = {F32: np.float32, I8: np.int8, U8: np.uint8, I32: np.int32}
 DTYPE_OF = {np.dtype(np.float32): F32, np.dtype(np.int8): I8, np.dtype(np.uint8): U8, np.dtype(np.int32): I32}
 AUTO_PAD = {"NOTSET": 0, "SAME_UPPER": 1, "SAME_LOWER": 2, "VALID": 3}
@@ -79,6 +79,29 @@ class NodeAttrs(C.Structure):
     ]
 
 
+class _CacheStruct(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("k_scale", C.c_void_p), ("v", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_size_t), ("heads", C.c_size_t), ("page", C.c_size_t), ("dim", C.c_size_t)]
+
+
+class KvCache:
+    """A decoder's key-value cache in 8 bits: codes `k` and `v` int8 [pages, heads, page, dim], dense, and `k_scale` and `v_scale` float32
+    [pages, heads]; a cached value is code * scale.  Holds on to the four arrays (numpy or torch), which the program makes once, and which
+    kv_cache_write changes in place.  Pages need not be cleared: a page begins anew when its first token is written."""
+
+    def __init__(self, k, k_scale, v, v_scale):
+        if len(k.shape) != 4 or tuple(v.shape) != tuple(k.shape):
+            raise ZantError(-59 if len(k.shape) != 4 else -5, "InvalidRank" if len(k.shape) != 4 else "InputTensorsWrongShape",
+                            f"codes are [pages, heads, page, dim], not {tuple(k.shape)} and {tuple(v.shape)}")
+        pages, heads, page, dim = (int(n) for n in k.shape)
+        arrays = [_values(k, pages * heads * page * dim, I8, "k", True), _values(k_scale, pages * heads, F32, "k_scale", True),
+                  _values(v, pages * heads * page * dim, I8, "v", True), _values(v_scale, pages * heads, F32, "v_scale", True)]
+        self.k, self.k_scale, self.v, self.v_scale = (a for a, _ in arrays)
+        self.pages, self.heads, self.page, self.dim = pages, heads, page, dim
+        self._struct = _CacheStruct(*(p for _, p in arrays), pages, heads, page, dim)
+        self._at = C.addressof(self._struct)
+
+
 # Argument types of the entry points that are called per operator or per pass: with them ctypes converts Python integers and
 # addresses itself (a conv call spent half of its 9 us on the host wrapping 22 arguments one by one).
 # p pointer, z size_t, i int32, f float; n: a size_t that is not negative, converted as a pointer (a third of the time).
@@ -91,6 +114,8 @@ _SIGNATURES = {
     "qlinearmatmul": "p i ppz f i ppz pp z f i p z i ppz i", "qlinearadd": "p i p f i p f i f i p z i", "plan_run": "p pp",
     "quantize_rows": "p i pnnn pn pnp", "qmatmul_scaled": "p pnnnp pnnpp ipn", "qmatmul_grouped": "p pnnnp pnnnpp p ipn",
     "token_logprobs": "p i pnnn ppp ipp",
+    "kv_cache_write": "p p i pn pn n pnn pp", "kv_cache_read": "p p i pn pn n pnn pp", "kv_cache_attention": "p p i pn nn pnn pp fii pn p",
+    "verify_drafts": "p i pn pn n pn pn pp pp",
 }
 _CTYPE = {"p": C.c_void_p, "z": C.c_size_t, "i": C.c_int32, "f": C.c_float, "n": C.c_void_p}
 
@@ -238,9 +263,27 @@ def _rows(a, what, result=False):
         code = _row_code(a.dtype, what)
     if rows <= 1:
         row = cols
-    if row < cols or (col != 1 and cols > 1):
+    if row < cols or (col != 1 and cols > 1 and rows):
         raise _strides_refused(what, strides)
     return a, ptr, rows, cols, row, code
+
+
+def _head_rows(a, dim, what, result=False):
+    """The same of rows that hold heads behind one another: [rows, heads * dim] or [rows, heads, dim] with dense rows."""
+    if len(a.shape) != 3:
+        return _rows(a, what, result)
+    if not hasattr(a, "data_ptr"):
+        if result and (not isinstance(a, np.ndarray) or not a.flags.c_contiguous or not a.flags.writeable):
+            raise ZantError(-34, "InputArrayWrongType", f"{what} is not a dense array that may be written")
+        a = np.ascontiguousarray(a)
+        return _rows(a.reshape(a.shape[0], a.shape[1] * a.shape[2]), what, result)
+    row, head, one = a.stride()
+    rows, heads, d = a.shape
+    if rows <= 1:
+        row = heads * d
+    if rows and ((one != 1 and d > 1) or (head != d and heads > 1) or row < heads * d):
+        raise _strides_refused(what, a.stride())
+    return a, a.data_ptr(), rows, heads * d, row, _row_code(a.dtype, what)
 
 
 def _matrices(a, what):
@@ -912,6 +955,108 @@ class Context:
         if top:
             idp, lkp = _values(ids, rows * top, I32, "top_ids", True)[1], _values(likely, rows * top, F32, "top_logprobs", True)[1]
         check(lib().zant_b200_token_logprobs(self._h, code, xp, rows, vocab, stride, tp, lp, ep, top, idp, lkp))
+        return out
+
+    def _sequences(self, table, lengths, offsets):
+        """(arrays to keep, address of the table, sequences, its width, addresses of lengths and offsets)."""
+        if not hasattr(table, "shape"):
+            table = np.asarray(table)
+        if len(table.shape) != 2:
+            raise ZantError(-59, "InvalidRank", f"table has {len(table.shape)} dimensions, not 2")
+        seqs, width = table.shape
+        table, tp = _values(table, seqs * width, I32, "table")
+        lengths, lp = _values(lengths, seqs, I32, "lengths")
+        op = None
+        if offsets is not None:
+            offsets, op = _values(offsets, seqs + 1, I32, "offsets")
+        return (table, lengths, offsets), tp, seqs, width, lp, op
+
+    def kv_cache_write(self, cache, k, v, table, lengths, offsets=None):
+        """Quantizes the keys and values of new tokens, k and v [rows, heads * dim] (or [rows, heads, dim]), into a KvCache.  Sequence s has its pages in
+        table[s] (int32 [seqs, width]) and lengths[s] tokens, of which the last are the new ones: rows offsets[s] to offsets[s + 1] - 1, or
+        rows / seqs each.  The scale of a page and head is the largest that its tokens asked for; codes of tokens that were there follow it."""
+        k, kp, rows, cols, k_stride, code = _head_rows(k, cache.dim, "k")
+        v, vp, v_rows, v_cols, v_stride, v_code = _head_rows(v, cache.dim, "v")
+        if v_code != code:
+            raise ZantError(-34, "InputArrayWrongType", "k and v are of one type")
+        if cols != cache.heads * cache.dim or v_cols != cols or v_rows != rows:
+            raise ZantError(-5, "InputTensorsWrongShape", f"k is {rows} x {cols}, v {v_rows} x {v_cols}, the cache has rows of {cache.heads} x {cache.dim}")
+        keep, tp, seqs, width, lp, op = self._sequences(table, lengths, offsets)
+        check(lib().zant_b200_kv_cache_write(self._h, cache._at, code, kp, k_stride, vp, v_stride, rows, tp, seqs, width, lp, op))
+
+    def kv_cache_read(self, cache, table, lengths, offsets=None, out=None, rows=None):
+        """(k, v): the last offsets[s + 1] - offsets[s] cached tokens of each sequence as rows [rows, heads * dim] in the type of `out` (a pair, either may be
+        None); without `out` float32 arrays of `rows` rows."""
+        wide = cache.heads * cache.dim
+        if out is None:
+            if rows is None:
+                raise ZantError(-102, "NullPointer", "give `out` or the number of rows")
+            out = (np.zeros((rows, wide), np.float32), np.zeros((rows, wide), np.float32))
+        keep, tp, seqs, width, lp, op = self._sequences(table, lengths, offsets)
+        found = [(None, None, None, wide, 0, None) if o is None else _head_rows(o, cache.dim, what, True) for o, what in zip(out, ("k", "v"))]
+        (_, kp, k_rows, k_cols, k_stride, k_code), (_, vp, v_rows, v_cols, v_stride, v_code) = found
+        if kp is None:
+            k_rows, k_code = v_rows, v_code
+        elif vp is None:
+            v_rows, v_code = k_rows, k_code
+        if k_code is None:
+            return out
+        if k_code != v_code:
+            raise ZantError(-34, "InputArrayWrongType", "k and v are of one type")
+        if k_cols != wide or v_cols != wide or k_rows != v_rows:
+            raise ZantError(-6, "OutputTensorDifferentSize", f"k is {k_rows} x {k_cols}, v {v_rows} x {v_cols}, the cache has rows of {cache.heads} x {cache.dim}")
+        check(lib().zant_b200_kv_cache_read(self._h, cache._at, k_code, kp, k_stride, vp, v_stride, k_rows, tp, seqs, width, lp, op))
+        return out
+
+    def kv_cache_attention(self, cache, q, table, lengths, offsets=None, scale=None, window=0, sinks=0, out=None, lse=None):
+        """Attention of new tokens, q [rows, heads * dim] (or [rows, heads, dim]), over their sequences in a KvCache, to which their own keys and values have been written; sequences as
+        in kv_cache_write.  `scale` is 1 / sqrt(dim) where it is not given.  A token sees itself and those before it; with `window` the last `window` of these and the
+        sequence's first `sinks`.  A query that sees nothing has 0.  `lse` (float32 [rows, heads]) takes the logarithms of the sums."""
+        q, qp, rows, cols, q_stride, code = _head_rows(q, cache.dim, "q")
+        heads = cols // cache.dim
+        if heads * cache.dim != cols:
+            raise ZantError(-5, "InputTensorsWrongShape", f"q has rows of {cols}, the cache's heads {cache.dim} dimensions")
+        if out is None:
+            if code not in (F32, F16):
+                raise ZantError(-34, "InputArrayWrongType", "numpy results are F32 or F16: give `out`")
+            out = np.zeros((rows, cols), np.float32 if code == F32 else np.float16)
+        _, yp, y_rows, y_cols, y_stride, y_code = _head_rows(out, cache.dim, "out", True)
+        if y_code != code:
+            raise ZantError(-34, "InputArrayWrongType", "q and out are of one type")
+        if y_rows != rows or y_cols != cols:
+            raise ZantError(-6, "OutputTensorDifferentSize", f"out is {y_rows} x {y_cols}, not {rows} x {cols}")
+        keep, tp, seqs, width, lp, op = self._sequences(table, lengths, offsets)
+        sp = None if lse is None else _values(lse, rows * heads, F32, "lse", True)[1]
+        check(lib().zant_b200_kv_cache_attention(self._h, cache._at, code, qp, q_stride, rows, heads, tp, seqs, width, lp, op,
+                                                 cache.dim ** -0.5 if scale is None else scale, window, sinks, yp, y_stride, sp))
+        return out
+
+    def verify_drafts(self, target, drafted, tokens, accept, sample, offsets=None, out=None):
+        """(accepted, next): how many drafted `tokens` (int32) of each sequence stand against the probabilities of the target model, and the token that follows them.
+        `target` [drafts + seqs, vocab] has a row for each draft of a sequence and one behind them, `drafted` [drafts, vocab] the probabilities that the
+        drafts were drawn from (None: certainties).  `accept` [drafts] and `sample` [seqs] are random numbers in [0, 1); sequence s has the
+        drafts offsets[s] to offsets[s + 1] - 1, or drafts / seqs each."""
+        p, pp, p_rows, vocab, p_stride, code = _rows(target, "target")
+        drafts, seqs = _numel(tokens.shape) if hasattr(tokens, "shape") else len(tokens), _numel(sample.shape) if hasattr(sample, "shape") else len(sample)
+        if p_rows != drafts + seqs:
+            raise ZantError(-5, "InputTensorsWrongShape", f"target has {p_rows} rows, not {drafts} + {seqs}")
+        qp, q_stride = None, 0
+        if drafted is not None:
+            drafted, qp, q_rows, q_vocab, q_stride, q_code = _rows(drafted, "drafted")
+            if q_code != code:
+                raise ZantError(-34, "InputArrayWrongType", "target and drafted are of one type")
+            if q_rows != drafts or q_vocab != vocab:
+                raise ZantError(-5, "InputTensorsWrongShape", f"drafted is {q_rows} x {q_vocab}, not {drafts} x {vocab}")
+        tokens, kp = _values(tokens, drafts, I32, "tokens")
+        accept, ap = _values(accept, drafts, F32, "accept")
+        sample, sp = _values(sample, seqs, F32, "sample")
+        op = None
+        if offsets is not None:
+            offsets, op = _values(offsets, seqs + 1, I32, "offsets")
+        if out is None:
+            out = (np.zeros(seqs, np.int32), np.zeros(seqs, np.int32))
+        cp, np_ = _values(out[0], seqs, I32, "accepted", True)[1], _values(out[1], seqs, I32, "next", True)[1]
+        check(lib().zant_b200_verify_drafts(self._h, code, pp, p_stride, qp, q_stride, vocab, kp, drafts, op, seqs, ap, sp, cp, np_))
         return out
 
     def lut_q8(self, x, lut, out=None):

@@ -31,16 +31,6 @@
 
 using namespace zb;
 
-#define ZB_NEED(ptr, what) \
-    do { if ((ptr) == nullptr) return fail(ZANT_E_NULL_POINTER, "%s is NULL", what); } while (0)
-
-#define ZB_NEED_CTX(ctx)                                                                                     \
-    do {                                                                                                     \
-        if ((ctx) == nullptr) return fail(ZANT_E_CUDA_UNAVAILABLE, "no context (zant_b200_ctx_create failed or was not called); there is no CPU fallback"); \
-        ZB_CUDA(cudaSetDevice((ctx)->device));                                                               \
-    } while (0)
-
-
 extern "C" {
 
 // ------------------------------------------------------------------------------------ library / context

@@ -34,6 +34,11 @@ struct zant_ctx {
 
 namespace zb {
 
+enum DeviceError : int {
+    DEV_OK = 0,
+    DEV_ERR_WAIT_TIMEOUT = 1,   // a bounded mbarrier wait gave up
+};
+
 #define ZB_CUDA(expr)                                                                         \
     do {                                                                                      \
         cudaError_t _e = (expr);                                                              \
@@ -59,6 +64,15 @@ namespace zb {
         cudaError_t _e = zb::dev_malloc((void**)&(ptr), (bytes));                             \
         if (_e == cudaErrorMemoryAllocation) { cudaGetLastError(); return zb::fail(ZANT_E_MEM_ERROR, "device allocation of %zu bytes failed", (size_t)(bytes)); } \
         if (_e != cudaSuccess) return zb::fail(ZANT_E_CUDA, "cudaMalloc(%zu) -> %s", (size_t)(bytes), cudaGetErrorString(_e)); \
+    } while (0)
+
+#define ZB_NEED(ptr, what) \
+    do { if ((ptr) == nullptr) return zb::fail(ZANT_E_NULL_POINTER, "%s is NULL", what); } while (0)
+
+#define ZB_NEED_CTX(ctx)                                                                                     \
+    do {                                                                                                     \
+        if ((ctx) == nullptr) return zb::fail(ZANT_E_CUDA_UNAVAILABLE, "no context (zant_b200_ctx_create failed or was not called); there is no CPU fallback"); \
+        ZB_CUDA(cudaSetDevice((ctx)->device));                                                               \
     } while (0)
 
 #ifndef ZB_TRY

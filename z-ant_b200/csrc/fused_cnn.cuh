@@ -16,15 +16,11 @@
 #include <cstdint>
 #include <cstring>
 
+#include "context.cuh"
 #include "kernels_q8.cuh"
 #include "ptx_sm100.cuh"
 
 namespace zb {
-
-enum DeviceError : int {
-    DEV_OK = 0,
-    DEV_ERR_WAIT_TIMEOUT = 1,   // a bounded mbarrier wait gave up
-};
 
 // =============================================================================================
 // Stage 1: QuantizeLinear(uint8) + QLinearConv(1 -> 32, 3x3, stride 1, no pad) + ReLU + MaxPool 2x2/2

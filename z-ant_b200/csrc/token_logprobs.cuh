@@ -24,7 +24,7 @@
 
 #include "context.cuh"
 #include "ptx_sm100.cuh"
-#include "quantize_rows.cuh"
+#include "row_codes.cuh"
 
 namespace zb {
 
@@ -88,9 +88,6 @@ template <> struct Logits<__half> {
         for (int i = 0; i < 4; ++i) { const float2 p = pair(w[i]); f[2 * i] = p.x; f[2 * i + 1] = p.y; }
     }
 };
-
-__device__ __forceinline__ float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // m log2(e), S and W (in log 2) of what a thread has seen.
 struct ExpSums {

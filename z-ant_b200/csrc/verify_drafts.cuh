@@ -1,0 +1,167 @@
+// Drafted tokens against the target's probabilities, with given random numbers.
+//
+//   draft i of a sequence stands while u_i q_i(d_i) < p_i(d_i); behind the first n that stand comes the token
+//   min { v : sum of r_w over w <= v  >  u sum of r },   r = max(p_n - q_n, 0), or p_n where all drafts stand
+//
+// Probabilities are what the program has made of its logits, so that everything here is exact but sums, which are fp64: products of
+// two fp32 numbers and differences fit 53 bits, and the border of a token in the running sum is off by 2^-53 of the whole, 2^29 times less than an fp32 sum's.
+//
+// Bound by memory: a sequence's own two rows are read once, in segments (16 a CTA, up to 8 CTAs a sequence) whose sums every CTA of the cluster gets; the CTA that
+// has the segment in which the border lies reads that one again.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "context.cuh"
+#include "ptx_sm100.cuh"
+#include "row_codes.cuh"
+
+namespace zb {
+
+struct VerifyArgs {
+    const void* target; long long target_stride; const void* drafted; long long drafted_stride; int vocab;
+    const int32_t* tokens; const int32_t* offsets; int drafts, seqs, per;
+    const float* accept; const float* sample;
+    int32_t* accepted; int32_t* next;
+    int parts;
+};
+
+struct VerifyShared {
+    static constexpr int THREADS = 512, SEGS = 16;
+    double seg[SEGS];                                 // a warp's sums, of this CTA's part of the row
+    double warp_sum[SEGS];
+    int n, begin, end, found, last;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(VerifyShared::THREADS) verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
+    using Sh = VerifyShared;
+    __shared__ Sh sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, P = a.parts;
+    const int part = P > 1 ? (int)ptx::cluster_rank() : 0, s = (int)(blockIdx.x / (unsigned)P);
+    ptx::grid_start();
+    const T* target = static_cast<const T*>(a.target);
+    const T* drafted = static_cast<const T*>(a.drafted);
+    if (warp == 0) {
+        const int b = a.offsets ? min(max(a.offsets[s], 0), a.drafts) : s * a.per;
+        int e = a.offsets ? min(max(a.offsets[s + 1], b), a.drafts) : b + a.per;
+        int n = 0;
+        for (bool more = true; more && b + n < e;) {
+            const int i = b + n + lane;
+            int state = 0;                            // 0 stands, 1 does not, 2 no draft
+            if (i < e) {
+                const int t = a.tokens[i];
+                if (t < 0) state = 2;
+                else if (t >= a.vocab) state = 1;
+                else {
+                    const double p = as_float(target[(long long)(i + s) * a.target_stride + t]);
+                    const double q = drafted ? (double)as_float(drafted[(long long)i * a.drafted_stride + t]) : 1.0;
+                    state = (double)a.accept[i] * q < p ? 0 : 1;
+                }
+            } else state = 2;
+            const unsigned stop = __ballot_sync(0xffffffffu, state != 0);
+            if (stop) {
+                const int first = __ffs(stop) - 1;
+                n += first;
+                if (__shfl_sync(0xffffffffu, state, first) == 2) e = b + n;
+                more = false;
+            } else n += 32;
+        }
+        if (lane == 0) { sh.n = n; sh.begin = b; sh.end = e; }
+    }
+    __syncthreads();
+    const int n = sh.n, at = sh.begin + n;
+    const T* p = target + (long long)(at + s) * a.target_stride;
+    bool less = at < sh.end;                          // a draft that did not stand
+    const T* q = less && drafted ? drafted + (long long)at * a.drafted_stride : nullptr;
+    const int given = less && !drafted ? a.tokens[at] : -1;
+    auto mass = [&](int v) -> double {
+        double r = as_float(p[v]);
+        if (less) r -= q ? (double)as_float(q[v]) : (v == given ? 1.0 : 0.0);
+        return r > 0.0 && r < INFINITY ? r : 0.0;
+    };
+    // segments in order: warp w of part i has the (16 i + w)-th
+    const int segs = P * Sh::SEGS;
+    auto seg_begin = [&](int i) { return (int)((long long)a.vocab * i / segs); };
+    const double u = a.sample[s];
+    for (int round = 0; round < 2; ++round) {
+        const int v0 = seg_begin(part * Sh::SEGS + warp), v1 = seg_begin(part * Sh::SEGS + warp + 1);
+        double sum = 0.0;
+        for (int v = v0 + lane; v < v1; v += 32) sum += mass(v);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) sh.seg[warp] = sum;
+        if (tid == 0) { sh.found = 0x7fffffff; sh.last = -1; }
+        __syncthreads();
+        if (P > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); }
+        auto seg_sum = [&](int i) {
+            if (P == 1) return sh.seg[i];
+            double v;
+            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(ptx::cluster_addr(ptx::smem_u32(&sh.seg[i % Sh::SEGS]), (uint32_t)(i / Sh::SEGS))) : "memory");
+            return v;
+        };
+        double total = 0.0;
+        for (int i = 0; i < segs; ++i) total += seg_sum(i);
+        if (total == 0.0 && less && round == 0) {     // nothing is left of the target's row: the row itself
+            less = false;
+            __syncwarp();
+            if (P > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); }
+            __syncthreads();
+            continue;
+        }
+        const double border = u * total;
+        double before = 0.0, sofar = 0.0;
+        int mine = -1, filled = -1;                   // the segment in which the sum passes the border, the last one that holds anything
+        double filled_before = 0.0;
+        for (int i = 0; i < segs; ++i) {
+            const double v = seg_sum(i);
+            if (v > 0.0) { filled = i; filled_before = sofar; }
+            if (mine < 0 && sofar + v > border && v > 0.0) { mine = i; before = sofar; }
+            sofar += v;
+        }
+        if (mine < 0) { mine = filled; before = filled_before; }
+        if (P > 1) { __syncwarp(); ptx::cluster_arrive(); ptx::cluster_wait(); }     // nobody leaves while its sums are read
+        if (total == 0.0) {
+            if (part == 0 && tid == 0) { a.accepted[s] = n; a.next[s] = -1; }
+            return;
+        }
+        if (mine / Sh::SEGS != part) return;
+        const int w0 = seg_begin(mine), w1 = seg_begin(mine + 1);
+        for (int v0b = w0; v0b < w1; v0b += Sh::THREADS) {
+            const int v = v0b + tid;
+            const double r = v < w1 ? mass(v) : 0.0;
+            double run = r;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) { const double o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
+            if (lane == 31) sh.warp_sum[warp] = run;
+            __syncthreads();
+            double base = before, all = 0.0;
+            for (int i = 0; i < Sh::SEGS; ++i) { if (i < warp) base += sh.warp_sum[i]; all += sh.warp_sum[i]; }
+            if (r > 0.0) {
+                if (base + run > border) atomicMin(&sh.found, v);
+                atomicMax(&sh.last, v);
+            }
+            before += all;
+            __syncthreads();
+            if (sh.found != 0x7fffffff) break;
+        }
+        if (tid == 0) { a.accepted[s] = n; a.next[s] = sh.found != 0x7fffffff ? sh.found : sh.last; }
+        return;
+    }
+}
+
+inline int32_t run_verify_drafts(zant_ctx* ctx, int32_t dtype, VerifyArgs a) {
+    int parts = 1;
+    while (parts < 8 && (long long)a.seqs * parts * 2 <= 2LL * ctx->sm_count && a.vocab / (parts * 2) >= 4096) parts *= 2;
+    a.parts = parts;
+    auto go = [&](auto kernel) {
+        launch_cluster(ctx, kernel, dim3((unsigned)((long long)a.seqs * parts)), VerifyShared::THREADS, 0, (unsigned)parts, a);
+        return check_launch(ctx, "verify_drafts_kernel");
+    };
+    if (dtype == ZANT_F32) return go(verify_drafts_kernel<float>);
+    if (dtype == ZANT_F16) return go(verify_drafts_kernel<__half>);
+    return go(verify_drafts_kernel<__nv_bfloat16>);
+}
+
+}  // namespace zb
