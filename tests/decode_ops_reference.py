@@ -85,8 +85,9 @@ def read(cache, kv, rows, table, lengths, offsets):
 def attention(cache, q, table, lengths, offsets, kind, scale=None, window=0, sinks=0):
     """(out, how far off it may be, lse, how far off it may be, rows of sequences) of q float64 [rows, heads, dim].
 
-    A score x is a sum of dim exact products, added in fp32 with at most one step (2 U) of the sum of magnitudes for each, times three factors: off by
-    dx = 2 U (dim + 2) scale sum |q k| and, with the difference to the maximum and the power of two, by 6 U |x - max| + 8 U relative to the weight.  A weight in f16 is
+    A score x is a sum of dim products of exact codes with q, which is exact or (few rows) rounded to whole numbers of which the row's largest is 2^19 (2^26 for f32) at least,
+    half a step of which is 2^-20 (2^-27) of that value; added exactly or in fp32 with at most one step (2 U) of the sum of magnitudes for each, times three factors: off by
+    dx = 2 U (dim + 2) scale sum |q k| + 2^-20 scale max |q| sum |k| and, with the difference to the maximum and the power of two, by 6 U |x - max| + 8 U relative to the weight.  A weight in f16 is
     off by 2**-11, in two f16 numbers by 2**-22, and by 2**-39 of the largest weight times the largest scale where it is tiny.  Sums over n tokens are
     added in fp32, 16 at a time, and rescaled at most every 32: n / 4 + 64 steps in all."""
     rows, heads, dim = q.shape
@@ -122,7 +123,7 @@ def attention(cache, q, table, lengths, offsets, kind, scale=None, window=0, sin
                         e = np.exp(x - top)
                         w = e / e.sum()
                         out[row + i, g] = w @ v[j]
-                        dx = 2 * U * (dim + 2) * size.max()
+                        dx = (2 * U * (dim + 2) * size + (2.0 ** -27 if kind == "f32" else 2.0 ** -20) * abs(scale) * np.abs(q[row + i, g]).max() * np.abs(k[j]).sum(1)).max()
                         dw = 2 * (dx + 8 * U + 6 * U * np.abs(x - top))
                         mean = w @ np.abs(v[j])
                         wide = 2 * U * (len(j) / 4 + 64)

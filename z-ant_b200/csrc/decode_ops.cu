@@ -139,6 +139,7 @@ int32_t zant_b200_kv_cache_attention(zant_ctx* ctx, const zant_kv_cache* cache, 
         ZB_TRY(kv_check(cache, rows, offsets, seqs, width, codes, scales));
         if (heads == 0 || heads % cache->heads) return fail(ZANT_E_INPUT_TENSORS_WRONG_SHAPE, "%zu heads of queries over %zu heads of keys", heads, cache->heads);
         if (heads > 65535) return fail(ZANT_E_TOO_LARGE, "%zu heads", heads);
+        ZB_TRY(check_int("pages of all heads", cache->pages * cache->heads));
         if (window < 0 || sinks < 0) return fail(ZANT_E_INVALID_INPUT, "window %d, sinks %d", window, sinks);
         const size_t group = heads / cache->heads, len = heads * cache->dim;
         ZB_TRY(check_int("rows of a key head", rows * group));

@@ -3,21 +3,21 @@
 //
 //   x_ij = scale q_i . k_j,   out_i = sum over j of exp(x_ij - m) v_j / sum over j of exp(x_ij - m)
 //
-// One pass over the codes with a running maximum.  The rows of a tile are (new token, head) pairs that share a key head: 8 NT of them.  Codes become
-// f16 on the way (exactly) and both products run on the tensor core with the cache as the A operand, transposed: X^T = K Q^T and O^T = V^T P^T, so that
-// 8 rows fill an MMA (16 would be needed the other way round).  How codes lie in a thread is free as long as both operands of a product
-// agree: a lane takes 16 bytes of a token as they lie and multiplies them with the same dimensions of q, and V's dimensions are put right when results are stored.  So
-// nothing is transposed or moved between lanes but P (movmatrix).
+// One pass over the codes with a running maximum.  The rows of a tile are (new token, head) pairs that share a key head: 8 NT of them.  Both products run on
+// the tensor core with the cache as the A operand, transposed: X^T = K Q^T and O^T = V^T P^T, so that 8 rows fill an MMA (16 would be needed the other way round).  How codes lie in
+// a thread is free as long as both operands of a product agree: a lane takes 16 bytes of a token as they lie and multiplies them with the same dimensions of q, and
+// V's dimensions are put right when results are stored.  So nothing is transposed or moved between lanes but P (movmatrix).
 //
-// q goes in as f16 times a power of two for each row, so that its largest value lies in [2^14, 2^15): f16 and bf16 values lose nothing down to 2^-28 of that one;
-// f32 is the sum of two f16 numbers (SPLIT; 2^-39 of the largest value is lost), and so is P.  P is rounded to f16 (2^-12 relative for results in 16 bits), each weight times
-// its page's scale over the largest scale so far, times 2^14, so that what is rounded is at most 2^14 and weights down to 2^-28 keep their 11 bits.  Statistics
-// and sums are fp32.
+// K stays int8: q goes in as whole numbers whose largest in a row is about 2^20 (of F32 2^27), in 3 (4) digits of 7 bits, whose products are int8 products with exact
+// sums; a value of q loses 2^-20 of the largest of its row at most (2^-27).  K in f16 took 96 more ALU instructions of 510 for a step, and ALU is the busiest pipe.
+// V becomes f16 on the way (exactly) and P is rounded to f16 (2^-11 relative, for results in 16 bits; of F32 the sum of two f16 numbers), each weight times its page's scale
+// over the largest scale so far, times 2^14, so that what is rounded is at most 2^14 and weights down to 2^-28 keep their 11 bits.  Statistics and sums are fp32.
 //
-// Memory is the bound (a cached token of 128 dimensions is 256 bytes for 4 x 8 x 128 operations of 8 rows).  Each warp takes every so many'th 32 tokens and
-// brings them by asynchronous copies of 16 bytes into slots of its own lanes, DEPTH steps ahead: a lane reads what it copied itself, in its own order, so that there is no
-// bank conflict and no barrier.  The warps of a CTA, and the CTAs of a cluster that share a tile, join their sums at the end.
+// Memory is the bound (a cached token of 128 dimensions is 256 bytes for 4 x 8 x 128 operations of 8 rows).  Each warp takes every so many'th step of 32 tokens (16 of
+// 256 dimensions), which its first lane brings by TMA into a ring of the warp's own, swizzled so that the lanes' 16-byte reads meet no bank twice.  No warp waits for
+// another until the end, when the warps of a CTA, and the CTAs of a cluster that share a tile, join their sums.
 #pragma once
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -29,6 +29,7 @@
 #include "kv_cache.cuh"
 #include "ptx_sm100.cuh"
 #include "row_codes.cuh"
+#include "tensor_map.cuh"
 
 namespace zb {
 
@@ -39,24 +40,19 @@ struct KvAttendArgs {
     float scale_log2;                                 // scale log2(e)
     int window, sinks;
     bool wide_q;                                      // q in whole 16-byte blocks
-    int parts, tiles;                                 // CTAs of a tile; row tiles of the grid
+    int parts;                                        // CTAs of a tile
+    int* status;
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
-}
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(there ? 8u : 0u) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4u : 0u) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// int8 products, 16 x 8 x 32.
+__device__ __forceinline__ void mma_i8_16x8(int (&d)[4], const uint32_t (&a)[4], uint2 b, bool first) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(first ? 0 : d[0]), "r"(first ? 0 : d[1]), "r"(first ? 0 : d[2]), "r"(first ? 0 : d[3]));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -125,101 +121,133 @@ struct KvSteps {
 
 template <int DP_, int NT_, bool SPLIT_>
 struct KvAttendCfg {
-    static constexpr int DP = DP_, NT = NT_, ROWS = 8 * NT, WARPS = 4, THREADS = 32 * WARPS, STEP = 32;
+    static constexpr int DP = DP_, NT = NT_, ROWS = 8 * NT, STEP = DP == 256 ? 16 : 32, HALVES = STEP / 16;
     static constexpr bool SPLIT = SPLIT_;
-    static constexpr int KS = DP / 16;                // MMA steps of the dimensions
-    static constexpr int CH = DP < 128 ? 1 : DP / 128;       // a lane's chunks of a token of V
-    static constexpr int VB = DP < 128 ? 8 : 16;      // bytes of each
-    static constexpr int MT = DP / 16;                // MMA tiles of the dimensions in O^T
-    static constexpr int HALF = STEP * DP, STAGE = 2 * HALF + 32;       // K, V, what the pages say
-    static constexpr int DEPTH = DP == 256 ? 3 : (DP == 128 ? 3 : 5);
-    static constexpr int QF = KS * NT * (SPLIT ? 2 : 1);     // fragments of q, 8 bytes a lane
+    static constexpr int MT = DP / 16, KS = DP / 32;  // MMA tiles of the dimensions in O^T, MMA steps of them in X^T
+    static constexpr int DIGITS = SPLIT ? 4 : 3;      // of q
+    static constexpr int BOX = DP < 128 ? DP : 128, BOXES = DP / BOX;       // bytes of a token in a box
+    static constexpr int VB = DP < 128 ? 8 : 16;      // bytes of V that a lane takes of each
+    static constexpr int HALF = STEP * DP, STAGE = 2 * HALF;       // K, V
+    static constexpr int DEPTH = DP == 64 ? 4 : 2;
+    // Warps of an SM: what the ring leaves and registers allow, as CTAs of 4 or as one.
+    static constexpr int MOST_WARPS = NT == 1 && DP < 256 ? 12 : 8;
+    static constexpr int QF = KS * NT * DIGITS;       // fragments of q, 8 bytes a lane
     static constexpr bool Q_SHARED = QF > 16;
     static constexpr int PITCH = DP + 4;
-    static constexpr int RING = WARPS * DEPTH * STAGE;
-    static constexpr int JOIN = WARPS * ROWS * PITCH * 4;
-    static constexpr int BIG = RING > JOIN ? RING : JOIN;
-    static constexpr int OFF_Q = BIG, OFF_STAT = OFF_Q + (Q_SHARED ? QF * 256 : 0);
-    static constexpr int SMEM = OFF_STAT + (WARPS * ROWS * 3 + ROWS * 2) * 4;
+    static constexpr int Q_BYTES = QF * 256;
+    static __host__ __device__ constexpr int big(int warps) {
+        const int ring = warps * DEPTH * STAGE, join = warps * ROWS * PITCH * 4;
+        return ring > join ? ring : join;
+    }
+    // ring or sums, q, statistics of warps and of the CTA, factors of rows, barriers, flag
+    static __host__ __device__ constexpr int smem(int warps) { return big(warps) + Q_BYTES + (warps * ROWS * 3 + ROWS * 3) * 4 + warps * DEPTH * 8 + 16; }
 };
 
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+// A part's sum and the factor that brings it to the common maximum: parts that saw nothing add nothing, NaN stays NaN.
+__device__ __forceinline__ float join_factor(float m, float l, float top) { return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2(m - top); }
+__device__ __forceinline__ float times(float v, float f) { return v == 0.0f ? 0.0f : v * f; }
+
 template <int DP, int NT, bool SPLIT>
-__global__ void __launch_bounds__(128) kv_attention_kernel(const __grid_constant__ KvAttendArgs a) {
+__global__ void __launch_bounds__(32 * KvAttendCfg<DP, NT, SPLIT>::MOST_WARPS, 1)
+kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using F = KvAttendCfg<DP, NT, SPLIT>;
-    constexpr int STEP = F::STEP, D = F::DEPTH, KS = F::KS;
-    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int STEP = F::STEP, H = F::HALVES, D = F::DEPTH, MT = F::MT, DIG = F::DIGITS;
+    extern __shared__ __align__(1024) uint8_t smem[];
     const KvArgs& c = a.c;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l4 = lane >> 2, c4 = lane & 3, P = a.parts;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l4 = lane >> 2, c4 = lane & 3, P = a.parts, W = blockDim.x >> 5;
     const int rank = P > 1 ? (int)ptx::cluster_rank() : 0;
+    uint2* qs = reinterpret_cast<uint2*>(smem + F::big(W));
+    float* stat = reinterpret_cast<float*>(smem + F::big(W) + F::Q_BYTES);       // [warp][row]: m, l, scale
+    float* joined = stat + 3 * W * F::ROWS;           // [row]: m, l of the CTA
+    float* row_factor = joined + 2 * F::ROWS;
+    uint8_t* tail = reinterpret_cast<uint8_t*>(row_factor + F::ROWS);
+    const uint32_t full = ptx::smem_u32(tail) + warp * D * 8;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + W * D * 8);
+    if (lane == 0) {
+        for (int i = 0; i < D; ++i) ptx::mbar_init(full + 8 * i, 1);
+        ptx::mbar_fence_init();
+    }
+    if (threadIdx.x == 0) *abort_flag = 0;
+    __syncthreads();
     ptx::grid_start();
     const int work = (int)(blockIdx.x / (unsigned)P), h = work % c.heads;
     KvSeq q; int unit;
-    bool any = kv_locate(c, work / c.heads, a.group, F::ROWS, 1, q, unit);
+    const bool any = kv_locate(c, work / c.heads, a.group, F::ROWS, 1, q, unit);
     const int row0 = unit * F::ROWS, rows = any ? min(F::ROWS, q.n * a.group - row0) : 0;
     if (rows <= 0) return;                            // (all CTAs of a cluster)
     const int low = max(q.first + row0 / a.group, -1), high = max(q.first + (row0 + rows - 1) / a.group, -1);      // (below zero: nothing is seen)
     const KvSteps steps(low, high, a.window, a.sinks, STEP);
-    const int stride_k = P * F::WARPS, k0 = rank * F::WARPS + warp;
+    const int stride_k = P * W, k0 = rank * W + warp;
 
-    const uint32_t ring = ptx::smem_u32(smem) + warp * D * F::STAGE;
-    uint8_t* ring_p = smem + warp * D * F::STAGE;
+    const uint8_t* ring = smem + warp * D * F::STAGE;
     const int pl = c.page_log2, inpage = c.page - 1;
-    // pages of both halves of step k (-1: none)
-    auto pages_of = [&](int k, long long (&id)[2]) {
-        id[0] = id[1] = -1;
-        if (k >= steps.total) return;
-        const int t = steps.at(k, STEP);
-        id[0] = kv_page(c, q.s, t >> pl);
-        id[1] = pl == 4 ? kv_page(c, q.s, (t >> pl) + 1) : id[0];
+    const bool two = H == 2 && pl == 4;               // a step is on two pages
+    // What the table and the scales say of 32 of the warp's steps, one a lane: pages of the step's 16 tokens each (-1: none) and their scales.
+    struct Batch {
+        int page[H]; float k[H], v[H];
+        unsigned there[H];                            // lanes with a page
     };
-    auto issue = [&](int k, int stage, const long long (&id)[2]) {
-        if (k < steps.total) {
-            const int t = steps.at(k, STEP);
-            const uint32_t dst = ring + stage * F::STAGE + lane * 16;
+    auto batch_of = [&](int i) {
+        Batch b;
+        const int k = k0 + (i + lane) * stride_k, t = k < steps.total ? steps.at(k, STEP) >> pl : -1;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const bool ok = id[half] >= 0;
-                const long long block = (ok ? id[half] : 0) * c.heads + h, off = (block * c.page + ((t + 16 * half) & inpage)) * c.dim;
-                const int8_t* pk = c.k + off;
-                const int8_t* pv = c.v + off;
+        for (int z = 0; z < H; ++z) {
+            b.page[z] = z == 0 || two ? (int)kv_page(c, q.s, t < 0 ? -1 : t + z) : b.page[0];
+            b.there[z] = __ballot_sync(0xffffffffu, b.page[z] >= 0);
+            const long long at = (long long)max(b.page[z], 0) * c.heads + h;
+            b.k[z] = z == 0 || two ? (b.page[z] >= 0 ? c.k_scale[at] : 0.0f) : b.k[0];
+            b.v[z] = z == 0 || two ? (b.page[z] >= 0 ? c.v_scale[at] : 0.0f) : b.v[0];
+        }
+        return b;
+    };
+    Batch cur = batch_of(0), nxt;
+    // Step i of the warp goes into the ring, by its first lane.
+    auto issue = [&](int i, int stage, const Batch& b) {
+        int page[H];
+        page[0] = __shfl_sync(0xffffffffu, b.page[0], i & 31);
+        if (H > 1) page[H - 1] = two ? __shfl_sync(0xffffffffu, b.page[H - 1], i & 31) : page[0];
+        const int k = k0 + i * stride_k;
+        if (lane != 0 || k >= steps.total) return;
+        const uint32_t dst = ptx::smem_u32(ring) + stage * F::STAGE, bar = full + 8 * stage;
+        if (!two) {                                   // one page: boxes of STEP tokens
+            ptx::mbar_arrive_expect_tx(bar, page[0] >= 0 ? F::STAGE : 0);
+            if (page[0] >= 0) {
+                const int t = steps.at(k, STEP) & inpage, block = page[0] * c.heads + h;
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int j = 0; j < DP / 64; ++j) {
-                        const int d = (c4 + 4 * j) * 16;
-                        const bool in = ok && d < c.dim;
-                        cp_async16(dst + ((half * 2 + b) * (DP / 64) + j) * 512, pk + (in ? (8 * b + l4) * c.dim + d : 0), in);
-                    }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < F::CH; ++j) {
-                        const int tok = (i & 2) * 4 + 2 * c4 + (i & 1), d = l4 * F::VB + 128 * j;
-                        const bool in = ok && d < c.dim;
-                        if (F::VB == 16) cp_async16(dst + F::HALF + ((half * 4 + i) * F::CH + j) * 512, pv + (in ? tok * c.dim + d : 0), in);
-                        else cp_async8(dst - lane * 8 + F::HALF + (half * 4 + i) * 256, pv + (in ? tok * c.dim + d : 0), in);
-                    }
-                if (lane == half) {
-                    cp_async4(ring + stage * F::STAGE + 2 * F::HALF + 8 * half, c.k_scale + block, ok);
-                    cp_async4(ring + stage * F::STAGE + 2 * F::HALF + 8 * half + 4, c.v_scale + block, ok);
-                    *reinterpret_cast<int*>(ring_p + stage * F::STAGE + 2 * F::HALF + 16 + 4 * half) = ok;
+                for (int z = 0; z < F::BOXES; ++z) {
+                    ptx::tma_load_3d(dst + z * STEP * F::BOX, &k_map, z * F::BOX, t, block, bar);
+                    ptx::tma_load_3d(dst + F::HALF + z * STEP * F::BOX, &v_map, z * F::BOX, t, block, bar);
                 }
             }
+        } else {
+            ptx::mbar_arrive_expect_tx(bar, (page[0] >= 0 ? F::STAGE / 2 : 0) + (page[H - 1] >= 0 ? F::STAGE / 2 : 0));
+#pragma unroll
+            for (int z = 0; z < H; ++z)
+                if (page[z] >= 0) {
+                    ptx::tma_load_3d(dst + z * 16 * F::BOX, &k_map, 0, 0, page[z] * c.heads + h, bar);
+                    ptx::tma_load_3d(dst + F::HALF + z * 16 * F::BOX, &v_map, 0, 0, page[z] * c.heads + h, bar);
+                }
         }
-        cp_async_commit();
     };
-    long long id[2];
-    for (int s = 0; s < D - 1; ++s) { pages_of(k0 + s * stride_k, id); issue(k0 + s * stride_k, s, id); }
-    pages_of(k0 + (D - 1) * stride_k, id);
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i) issue(i, i, cur);
 
     // q: lane's columns of B are row l4 of each 8, dimensions as its chunks of K have them; its columns of X^T are rows 2 c4 and 2 c4 + 1
-    uint2 qf[F::Q_SHARED ? 1 : F::QF];
-    uint2* qs = reinterpret_cast<uint2*>(smem + F::OFF_Q);
-    float factor[NT][2];
-    int seen_to[NT][2];                               // positions of the lane's two rows
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int r = row0 + 8 * n + l4;
+    // (Warp n turns 8 rows into digits, for all: each warp for itself took as many instructions as two steps.)
+    constexpr int BITS = 7 * DIG - 1;                 // the largest value of a row in [2^(BITS - 1), 2^BITS)
+    auto dim_of = [&](int j) { return DP == 64 ? c4 * 16 : (j >> 1) * 128 + (2 * c4 + (j & 1)) * 16; };
+    if (warp < NT) {
+        const int n = warp, r = row0 + 8 * n + l4;
         const bool there = 8 * n + l4 < rows;
         const long long at = (long long)(q.row + (there ? r / a.group : 0)) * a.q_stride + (long long)(h * a.group + (there ? r % a.group : 0)) * c.dim;
         float v[DP / 64][16];
@@ -227,103 +255,142 @@ __global__ void __launch_bounds__(128) kv_attention_kernel(const __grid_constant
         bool odd = false;
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) {
-            const int d = (c4 + 4 * j) * 16;
+            const int d = dim_of(j);
             if (there && d < c.dim) kv_values16(a.q, a.q_type, a.wide_q, at + d, v[j]);
             else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) v[j][i] = 0.0f;
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) { top = fmaxf(top, fabsf(v[j][i])); odd |= !(fabsf(v[j][i]) < INFINITY); }
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        odd = (__ballot_sync(0xffffffffu, odd) >> (lane & 28)) & 15;
-        // 2^-e with top 2^-e in [2^14, 2^15); of numbers below 2^-100 what fits
-        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -114), 127);
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(127 + e, 1) << 23);
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x[4], y[4];
+            for (int i = 0; i < 16; ++i) { top = fmaxf(top, fabsf(v[j][i])); odd |= !(fabsf(v[j][i]) < INFINITY); }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        odd = (__ballot_sync(0xffffffffu, odd) >> (lane & 28)) & 15;
+        // 2^-e, clamped where it would leave the normal numbers (values below 2^-98 keep fewer bits)
+        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - (BITS - 1), -125), 126);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)(127 + e) << 23);
+        if (c4 == 0) row_factor[8 * n + l4] = up * a.scale_log2;
 #pragma unroll
-                for (int z = 0; z < 4; ++z) { x[z] = odd ? 0.0f : v[j][4 * i + z] * down; y[z] = x[z] - __half2float(__float2half_rn(x[z])); }
-                const uint2 hi = make_uint2(pack_f16(x[0], x[2]), pack_f16(x[1], x[3])), lo = make_uint2(pack_f16(y[0], y[2]), pack_f16(y[1], y[3]));
-                const int f = (j * 4 + i) * NT + n;
-                if (F::Q_SHARED) {
-                    if (warp == 0) { qs[f * 32 + lane] = hi; if (SPLIT) qs[(KS * NT + f) * 32 + lane] = lo; }
-                } else {
-                    qf[f] = hi;
-                    if (SPLIT) qf[KS * NT + f] = lo;
+        for (int j = 0; j < DP / 64; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {             // 8 values: a fragment of 4 and 4
+                uint32_t digit[DIG][2] = {};
+#pragma unroll
+                for (int z = 0; z < 8; ++z) {
+                    int x = odd ? 0 : __float2int_rn(v[j][8 * i + z] * down);
+#pragma unroll
+                    for (int g = 0; g < DIG; ++g) {   // digits from -64 to 63, the last one what is left (64 at most)
+                        const int lowest = g == DIG - 1 ? x : ((x + 64) & 127) - 64;
+                        digit[g][z >> 2] |= (uint32_t)(lowest & 255) << (8 * (z & 3));
+                        x = (x - lowest) >> 7;
+                    }
                 }
+#pragma unroll
+                for (int g = 0; g < DIG; ++g) qs[(((j * 2 + i) * NT + n) * DIG + g) * 32 + lane] = make_uint2(digit[g][0], digit[g][1]);
             }
-        const float fac = up * a.scale_log2;
+    }
+    __syncthreads();
+    uint2 qf[F::Q_SHARED ? 1 : F::QF];
+    if (!F::Q_SHARED) {
+#pragma unroll
+        for (int f = 0; f < F::QF; ++f) qf[F::Q_SHARED ? 0 : f] = qs[f * 32 + lane];
+    }
+    auto q_at = [&](int f) -> uint2 { return F::Q_SHARED ? qs[f * 32 + lane] : qf[F::Q_SHARED ? 0 : f]; };
+    float factor[NT][2];
+    int seen_to[NT][2];                               // positions of the lane's two rows
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            factor[n][i] = __shfl_sync(0xffffffffu, fac, (2 * c4 + i) * 4);
-            const int row = row0 + min(8 * n + 2 * c4 + i, rows - 1);
-            seen_to[n][i] = max(q.first + row / a.group, -1);
+            factor[n][i] = row_factor[8 * n + 2 * c4 + i];
+            seen_to[n][i] = max(q.first + (row0 + min(8 * n + 2 * c4 + i, rows - 1)) / a.group, -1);
         }
-    }
-    if (F::Q_SHARED) __syncthreads();
-    auto q_at = [&](int f) -> uint2 { return F::Q_SHARED ? qs[f * 32 + lane] : qf[F::Q_SHARED ? 0 : f]; };
 
-    float o[F::MT][NT][4];
-    float m[NT][2], l[NT][2], vs = 0.0f;
+    float o[MT][NT][4];
+    float m[NT][2], l[NT][2], vs = 0.0f, over = 0.0f;     // over: 2^14 / vs
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         m[n][0] = m[n][1] = -INFINITY;
         l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < F::MT; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
+        for (int j = 0; j < MT; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
     }
 
+    // the lane's 16 bytes of token l4 (of 8), dimensions dim_of(j); and of V's token 2 c4 (+ 1)
+    auto k_at = [&](const uint8_t* st, int group8, int j) {
+        if (DP == 64) return st + (group8 * 8 + l4) * 64 + ((c4 ^ (l4 >> 1)) << 4);
+        return st + (j >> 1) * STEP * 128 + (group8 * 8 + l4) * 128 + (((2 * c4 + (j & 1)) ^ l4) << 4);
+    };
+    auto v_at = [&](const uint8_t* st, int group8, int odd_token, int box) {
+        const int r = 2 * c4 + odd_token;
+        if (DP == 64) return st + (group8 * 8 + r) * 64 + (((l4 >> 1) ^ (r >> 1)) << 4) + (l4 & 1) * 8;
+        return st + box * STEP * 128 + (group8 * 8 + r) * 128 + ((l4 ^ r) << 4);
+    };
     int stage = 0, ahead = D - 1;
-    for (int k = k0; k < steps.total; k += stride_k) {
+    uint32_t phase = 0;
+    for (int k = k0, i = 0; k < steps.total; k += stride_k, ++i) {
+        if ((i & 31) == 0) {
+            if (i > 0) cur = nxt;
+            nxt = batch_of(i + 32);
+        }
         __syncwarp();                                 // the warp has read the stage that is filled now
-        issue(k + (D - 1) * stride_k, ahead, id);
-        pages_of(k + D * stride_k, id);
-        cp_async_wait<D - 1>();
-        __syncwarp();
-        const uint8_t* st = ring_p + stage * F::STAGE;
-        const float* scales = reinterpret_cast<const float*>(st + 2 * F::HALF);
-        const int* ok = reinterpret_cast<const int*>(st + 2 * F::HALF + 16);
+        issue(i + D - 1, ahead, (i & 31) + D - 1 < 32 ? cur : nxt);
+        float ks[H], vsc[H];
+        bool ok[H];
+#pragma unroll
+        for (int z = 0; z < H; ++z) {
+            ks[z] = z == 0 || two ? __shfl_sync(0xffffffffu, cur.k[z], i & 31) : ks[0];
+            vsc[z] = z == 0 || two ? __shfl_sync(0xffffffffu, cur.v[z], i & 31) : vsc[0];
+            ok[z] = (cur.there[z] >> (i & 31)) & 1u;
+        }
+        if (!__all_sync(0xffffffffu, ptx::mbar_wait(full + 8 * stage, phase, abort_flag))) {
+            // given up: the copies on their way land before the ring is something else's (or are given up too)
+            for (int z = 0; z < D && k + z * stride_k < steps.total; ++z) {
+                volatile int no = 0;
+                ptx::mbar_wait(full + 8 * stage, phase, &no);
+                if (++stage == D) { stage = 0; phase ^= 1u; }
+            }
+            break;
+        }
+        const uint8_t* st = ring + stage * F::STAGE;
         const int t = steps.at(k, STEP);
-        // scores of 32 tokens
-        float x[2][NT][4];
+        // scores
+        float x[H][NT][4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < H; ++half) {
+            // (16 rows at a time, for the registers' sake; K is read again for others)
+            constexpr int NG = NT < 2 ? NT : 2;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) x[half][n][0] = x[half][n][1] = x[half][n][2] = x[half][n][3] = 0.0f;
+            for (int n0 = 0; n0 < NT; n0 += NG) {
+                int sum[NG][DIG][4];
 #pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-                const uint4 lo = *reinterpret_cast<const uint4*>(st + ((half * 2) * (DP / 64) + j) * 512 + lane * 16);
-                const uint4 hi = *reinterpret_cast<const uint4*>(st + ((half * 2 + 1) * (DP / 64) + j) * 512 + lane * 16);
-                const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+                for (int j = 0; j < DP / 64; ++j) {
+                    const uint4 lo = *reinterpret_cast<const uint4*>(k_at(st, 2 * half, j)), hi = *reinterpret_cast<const uint4*>(k_at(st, 2 * half + 1, j));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t frag[4] = {codes_f16(wl[i]), codes_f16(wh[i]), codes_f16(wl[i] >> 8), codes_f16(wh[i] >> 8)};
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t frag[4] = {i ? lo.z : lo.x, i ? hi.z : hi.x, i ? lo.w : lo.y, i ? hi.w : hi.y};
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const uint2 b = q_at((j * 4 + i) * NT + n);
-                        mma_f16(x[half][n], frag, b.x, b.y);
-                        if (SPLIT) { const uint2 d = q_at((KS + j * 4 + i) * NT + n); mma_f16(x[half][n], frag, d.x, d.y); }
+                        for (int n = 0; n < NG; ++n)
+#pragma unroll
+                            for (int g = 0; g < DIG; ++g) mma_i8_16x8(sum[n][g], frag, q_at(((j * 2 + i) * NT + n0 + n) * DIG + g), j == 0 && i == 0);
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {     // (two digits' sums are below 2^29; the upper two, or the third, count 2^14)
+                        const float lower = (float)(sum[n][0][i] + 128 * sum[n][1][i]), upper = (float)(DIG == 4 ? sum[n][2][i] + 128 * sum[n][DIG - 1][i] : sum[n][2][i]);
+                        x[half][n0 + n][i] = fmaf(upper, 16384.0f, lower) * (factor[n0 + n][i & 1] * ks[half]);
+                    }
             }
         }
-        const float ks[2] = {scales[0], scales[2]}, vsc[2] = {scales[1], scales[3]};
-        const bool all = ok[0] && ok[1] && t + STEP - 1 <= low && (a.window == 0 || t > high - a.window || t + STEP <= a.sinks);
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[half][n][i] *= factor[n][i & 1] * ks[half];
+        const bool all = ok[0] && ok[H - 1] && t + STEP - 1 <= low && (a.window == 0 || t > high - a.window || t + STEP <= a.sinks);
         if (!all) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < H; ++half)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -340,14 +407,15 @@ __global__ void __launch_bounds__(128) kv_attention_kernel(const __grid_constant
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float v = fmaxf(fmaxf(x[0][n][i], x[0][n][i + 2]), fmaxf(x[1][n][i], x[1][n][i + 2]));
+                float v = fmaxf(x[0][n][i], x[0][n][i + 2]);
+                if (H > 1) v = fmaxf(v, fmaxf(x[H - 1][n][i], x[H - 1][n][i + 2]));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
                 to[n][i] = fmaxf(m[n][i], v);
                 raise |= to[n][i] > m[n][i];
             }
-        const float vs_to = fmaxf(vs, fmaxf(fabsf(vsc[0]), fabsf(vsc[1])));
+        const float vs_to = fmaxf(vs, fmaxf(fabsf(vsc[0]), fabsf(vsc[H - 1])));
         if (__any_sync(0xffffffffu, raise || vs_to > vs)) {
             const float fv = vs_to > 0.0f ? vs / vs_to : 1.0f;
 #pragma unroll
@@ -358,23 +426,30 @@ __global__ void __launch_bounds__(128) kv_attention_kernel(const __grid_constant
                     l[n][i] *= f;
                     m[n][i] = to[n][i];
 #pragma unroll
-                    for (int j = 0; j < F::MT; ++j) { o[j][n][i] *= f * fv; o[j][n][i + 2] *= f * fv; }
+                    for (int j = 0; j < MT; ++j) { o[j][n][i] *= f * fv; o[j][n][i + 2] *= f * fv; }
                 }
             vs = vs_to;
+            over = vs > 0.0f ? 16384.0f / vs : 0.0f;
         }
-        const float over = vs > 0.0f ? 16384.0f / vs : 0.0f;
+        float base[NT][2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) base[n][i] = m[n][i] == -INFINITY ? 0.0f : m[n][i];
+#pragma unroll
+        for (int half = 0; half < H; ++half) {
             const float vf = vsc[half] * over;
+            const bool plain = vf == vf;              // (a scale of NaN: only of what is seen)
             uint32_t b[NT][2], d[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float p[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = ex2(x[half][n][i] - (m[n][i & 1] == -INFINITY ? 0.0f : m[n][i & 1]));
+                    const float e = ex2(x[half][n][i] - base[n][i & 1]);
                     l[n][i & 1] += e;
-                    p[i] = e == 0.0f ? 0.0f : e * vf;
+                    p[i] = e * vf;
+                    if (!plain) p[i] = e == 0.0f ? 0.0f : p[i];
                 }
                 b[n][0] = pack_f16(p[0], p[1]);
                 b[n][1] = pack_f16(p[2], p[3]);
@@ -389,15 +464,16 @@ __global__ void __launch_bounds__(128) kv_attention_kernel(const __grid_constant
                 b[n][1] = transpose8x8(b[n][1]);
             }
 #pragma unroll
-            for (int j = 0; j < F::CH; ++j) {
+            for (int j = 0; j < F::BOXES; ++j) {
                 uint32_t w[4][F::VB / 4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    const uint8_t* at = v_at(st + F::HALF, 2 * half + (i >> 1), i & 1, j);
                     if constexpr (F::VB == 16) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(st + F::HALF + ((half * 4 + i) * F::CH + j) * 512 + lane * 16);
+                        const uint4 v = *reinterpret_cast<const uint4*>(at);
                         w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
                     } else {
-                        const uint2 v = *reinterpret_cast<const uint2*>(st + F::HALF + (half * 4 + i) * 256 + lane * 8);
+                        const uint2 v = *reinterpret_cast<const uint2*>(at);
                         w[i][0] = v.x; w[i][1] = v.y;
                     }
                 }
@@ -415,15 +491,12 @@ __global__ void __launch_bounds__(128) kv_attention_kernel(const __grid_constant
                 }
             }
         }
-        stage = stage + 1 == D ? 0 : stage + 1;
+        if (++stage == D) { stage = 0; phase ^= 1u; }
         ahead = ahead + 1 == D ? 0 : ahead + 1;
     }
-    cp_async_wait<0>();
-    __syncthreads();                                  // the ring becomes the place of the warps' sums
+    __syncthreads();                                  // the ring becomes the place of the warps' sums (every copy has been waited for)
 
     float* sums = reinterpret_cast<float*>(smem);     // [warp][row][dimension]
-    float* stat = reinterpret_cast<float*>(smem + F::OFF_STAT);       // [warp][row]: m, l, scale
-    float* joined = stat + 3 * F::WARPS * F::ROWS;    // [row]: m, l of the CTA
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -439,81 +512,93 @@ __global__ void __launch_bounds__(128) kv_attention_kernel(const __grid_constant
             }
             float* to = sums + (warp * F::ROWS + r) * F::PITCH;
 #pragma unroll
-            for (int j = 0; j < F::MT; ++j) {
+            for (int j = 0; j < MT; ++j) {
                 const int d = (j / 8) * 128 + l4 * F::VB + 2 * (j % 8);
-                to[d] = o[j][n][i];
-                to[d + 1] = o[j][n][i + 2];
+                *reinterpret_cast<float2*>(to + d) = make_float2(o[j][n][i], o[j][n][i + 2]);
             }
         }
     __syncthreads();
-    for (int r = warp; r < F::ROWS; r += F::WARPS) {
-        float top = -INFINITY, total = 0.0f, f[F::WARPS];
-#pragma unroll
-        for (int w = 0; w < F::WARPS; ++w) top = fmaxf(top, stat[(w * F::ROWS + r) * 3]);
-#pragma unroll
-        for (int w = 0; w < F::WARPS; ++w) {
-            const float* s = stat + (w * F::ROWS + r) * 3;
-            const float e = s[0] == -INFINITY ? 0.0f : ex2(s[0] - top);
-            total += s[0] == -INFINITY && s[1] == 0.0f ? 0.0f : s[1] * (s[0] == -INFINITY ? 1.0f : e);
-            f[w] = e * s[2];
+    if (threadIdx.x < F::ROWS) {
+        const int r = threadIdx.x;
+        float top = -INFINITY, total = 0.0f;
+        for (int w = 0; w < W; ++w) top = fmaxf(top, stat[(w * F::ROWS + r) * 3]);
+        for (int w = 0; w < W; ++w) {
+            float* s = stat + (w * F::ROWS + r) * 3;
+            const float f = join_factor(s[0], s[1], top);
+            total += times(s[1], f);
+            s[2] *= f;
         }
-        for (int d = lane; d < DP; d += 32) {
-            float v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < F::WARPS; ++w) {
-                const float part = sums[(w * F::ROWS + r) * F::PITCH + d];
-                v += part == 0.0f ? 0.0f : part * f[w];
-            }
-            sums[r * F::PITCH + d] = v;               // (only this warp reads row r of any warp)
+        joined[2 * r] = top; joined[2 * r + 1] = total;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < F::ROWS * (DP / 4); e += blockDim.x) {
+        const int r = e / (DP / 4), d = (e % (DP / 4)) * 4;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int w = 0; w < W; ++w) {
+            const float f = stat[(w * F::ROWS + r) * 3 + 2];
+            const float4 p = *reinterpret_cast<const float4*>(sums + (w * F::ROWS + r) * F::PITCH + d);
+            v.x = fmaf(p.x, f, v.x); v.y = fmaf(p.y, f, v.y); v.z = fmaf(p.z, f, v.z); v.w = fmaf(p.w, f, v.w);
         }
-        if (lane == 0) { joined[2 * r] = top; joined[2 * r + 1] = total; }
+        *reinterpret_cast<float4*>(sums + r * F::PITCH + d) = v;       // (of warp 0's, which only this thread reads)
     }
     if (P > 1) {
         __syncwarp();
         ptx::cluster_arrive();
         ptx::cluster_wait();
     } else __syncthreads();
-    const uint32_t peer_sums = ptx::smem_u32(sums), peer_joined = ptx::smem_u32(joined);
-    auto peer = [&](uint32_t addr, int r) {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::cluster_addr(addr, (uint32_t)r)) : "memory");
-        return v;
-    };
-    // each CTA of the cluster finishes every so many'th row
-    for (int r = rank + P * warp; r < rows; r += P * F::WARPS) {
-        float top = -INFINITY, total = 0.0f, f = 0.0f;
-        float mine_m = -INFINITY, mine_l = 0.0f;
-        if (P > 1) {
-            if (lane < P) { mine_m = peer(peer_joined + 8 * r, lane); mine_l = peer(peer_joined + 8 * r + 4, lane); }
-        } else if (lane == 0) { mine_m = joined[2 * r]; mine_l = joined[2 * r + 1]; }
-        top = mine_m;
+    const uint32_t my_sums = ptx::smem_u32(sums), my_joined = ptx::smem_u32(joined);
+    const int quads = c.dim / 4;
+    for (int e = rank * (int)blockDim.x + threadIdx.x; e < rows * quads; e += P * (int)blockDim.x) {
+        const int r = e / quads, d = (e % quads) * 4;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float top = -INFINITY, total = 0.0f;
+        if (P == 1) {
+            v = *reinterpret_cast<const float4*>(sums + r * F::PITCH + d);
+            top = joined[2 * r]; total = joined[2 * r + 1];
+        } else {
+            for (int p0 = 0; p0 < P; p0 += 2) {       // (P is even; two parts' loads at once)
+                float2 ml[2]; float4 part[2];
 #pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        f = mine_m == -INFINITY ? (mine_l == 0.0f ? 0.0f : 1.0f) : ex2(mine_m - top);
-        total = mine_l == 0.0f ? 0.0f : mine_l * f;
+                for (int i = 0; i < 2; ++i) {
+                    ml[i] = ld_cluster2(ptx::cluster_addr(my_joined + 8 * r, (uint32_t)(p0 + i)));
+                    part[i] = ld_cluster4(ptx::cluster_addr(my_sums + 4 * (r * F::PITCH + d), (uint32_t)(p0 + i)));
+                }
+                const float to = fmaxf(top, fmaxf(ml[0].x, ml[1].x)), f = join_factor(top, total, to);
+                total = times(total, f);
+                v.x = times(v.x, f); v.y = times(v.y, f); v.z = times(v.z, f); v.w = times(v.w, f);
 #pragma unroll
-        for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+                for (int i = 0; i < 2; ++i) {
+                    const float fp = join_factor(ml[i].x, ml[i].y, to);
+                    total += times(ml[i].y, fp);
+                    v.x += times(part[i].x, fp); v.y += times(part[i].y, fp); v.z += times(part[i].z, fp); v.w += times(part[i].w, fp);
+                }
+                top = to;
+            }
+        }
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         const int row = row0 + r;
-        const long long at = (long long)(q.row + row / a.group) * a.out_stride + (long long)(h * a.group + row % a.group) * c.dim;
-        for (int d0 = 0; d0 < c.dim; d0 += 32) {      // (whole warps: the parts' factors come by shuffles)
-            const int d = d0 + lane;
-            float v = 0.0f;
-            for (int p = 0; p < P; ++p) {
-                const float fp = __shfl_sync(0xffffffffu, f, p);
-                const float part = d < c.dim ? (P > 1 ? peer(peer_sums + 4 * (r * F::PITCH + d), p) : sums[r * F::PITCH + d]) : 0.0f;
-                v += part == 0.0f ? 0.0f : part * fp;
-            }
-            if (total != total) v = total;
-            if (d < c.dim) kv_store(a.out, a.q_type, at + d, v * inv);
-        }
-        if (a.lse && lane == 0) a.lse[(long long)(q.row + row / a.group) * a.heads + h * a.group + row % a.group] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+        const long long token = q.row + row / a.group, head = h * a.group + row % a.group, at = token * a.out_stride + head * c.dim + d;
+        kv_store(a.out, a.q_type, at, v.x * inv); kv_store(a.out, a.q_type, at + 1, v.y * inv);
+        kv_store(a.out, a.q_type, at + 2, v.z * inv); kv_store(a.out, a.q_type, at + 3, v.w * inv);
+        if (a.lse && d == 0) a.lse[token * a.heads + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
     }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, (int)DEV_ERR_WAIT_TIMEOUT);
     if (P > 1) {
         __syncwarp();
         ptx::cluster_arrive();
         ptx::cluster_wait();                          // nobody leaves while its sums are read
     }
+}
+
+// Codes as boxes of `rows` tokens of a page and head, `box` bytes each, zeros behind the head's end.
+inline int32_t encode_kv_map(CUtensorMap* map, const void* p, const KvArgs& c, int box, int rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return fail(ZANT_E_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t dims[3] = {(cuuint64_t)c.dim, (cuuint64_t)c.page, (cuuint64_t)c.pages * c.heads}, strides[2] = {(cuuint64_t)c.dim, (cuuint64_t)c.dim * c.page};
+    const cuuint32_t sides[3] = {(cuuint32_t)box, (cuuint32_t)rows, 1}, ones[3] = {1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(p), dims, strides, sides, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              box == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? ZANT_OK : fail(ZANT_E_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
 }
 
 template <int DP, int NT, bool SPLIT>
@@ -523,18 +608,26 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     if (items > 0x7fffffffLL / 16) return fail(ZANT_E_TOO_LARGE, "%lld tiles of attention", items);
     // CTAs that share a tile: while they find room side by side and each warp has steps left to take
     const long long reach = std::min((long long)a.c.width << a.c.page_log2, a.window > 0 ? (long long)a.window + a.sinks + 2 * F::STEP : 0x7fffffffffLL);
-    int parts = 1;
-    while (parts < 16 && items * parts * 2 <= 2LL * ctx->sm_count && reach >= (long long)parts * 2 * F::WARPS * F::STEP) parts *= 2;
-    a.parts = parts; a.tiles = (int)tiles;
+    const long long steps = (reach + F::STEP - 1) / F::STEP;
+    const long long slots = (long long)ctx->sm_count * (F::MOST_WARPS / 4);
+    int warps = 4, parts = 1;
+    while (parts < 16 && ((items * parts * 2 <= slots && steps >= 8LL * parts) || (items * parts * 2 <= 3 * slots && steps >= 64LL * parts))) parts *= 2;
+    if (items * parts <= ctx->sm_count && parts < 16 && steps >= (long long)parts * F::MOST_WARPS) warps = F::MOST_WARPS;
+    a.parts = parts;
+    a.status = ctx->status_word;
+    alignas(64) CUtensorMap k_map{}, v_map{};
+    const int box_rows = std::min(a.c.page, F::STEP);
+    ZB_TRY(encode_kv_map(&k_map, a.c.k, a.c, F::BOX, box_rows));
+    ZB_TRY(encode_kv_map(&v_map, a.c.v, a.c, F::BOX, box_rows));
     auto kernel = kv_attention_kernel<DP, NT, SPLIT>;
-    ZB_SMEM_ATTR(ctx, kernel, F::SMEM);
+    ZB_SMEM_ATTR(ctx, kernel, F::smem(F::MOST_WARPS));
     static std::atomic<unsigned long long> wide{0ull};
     const unsigned long long bit = 1ull << (ctx->device & 63);
     if (parts > 8 && !(wide.load(std::memory_order_acquire) & bit)) {
         ZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         wide.fetch_or(bit, std::memory_order_release);
     }
-    launch_cluster(ctx, kernel, dim3((unsigned)(items * parts)), F::THREADS, F::SMEM, (unsigned)parts, a);
+    launch_cluster(ctx, kernel, dim3((unsigned)(items * parts)), 32 * warps, F::smem(warps), (unsigned)parts, a, k_map, v_map);
     return check_launch(ctx, "kv_attention_kernel");
 }
 
