@@ -224,3 +224,22 @@ def test_host_arrays(ctx, zb):
     got = ctx.kv_cache_attention(held, q, table, [70, 40], offsets=[0, 4, 5], lse=ls)
     within(got.reshape(5, 4, 32).astype(np.float64), want, off)
     within(ls.astype(np.float64), lse, lse_off)
+
+
+@pytest.mark.parametrize("cta", [0, 3, 10007])
+def test_a_prompts_cta_gives_up(ctx, zb, cta):
+    """A CTA whose first wait runs out: every warp of it comes to the kernel's end, the call reports the time-out, and the calls behind it are right."""
+    import torch
+    rng = np.random.default_rng(8)
+    cache = ref.Cache(20, 2, 64, 128, rng)
+    table = tables(rng, 20, 64, [600, 300])
+    q = as_kind(torch, rng.standard_normal((600, 4, 128)), "bf16")
+    args = (ctx, zb, torch, cache, q, table, [600, 300], [0, 500, 600], "bf16")
+    want = run(*args)
+    ctx.selftest_give_up(cta)
+    with pytest.raises(zb.ZantError) as e:
+        run(*args)
+    assert e.value.name == "DeviceTimeout"
+    for _ in range(2):
+        got = run(*args)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])

@@ -8,6 +8,7 @@
 #include "context.cuh"
 #include "kv_attention.cuh"
 #include "kv_cache.cuh"
+#include "kv_prompt.cuh"
 #include "row_checks.cuh"
 #include "status.hpp"
 #include "verify_drafts.cuh"
@@ -160,7 +161,7 @@ int32_t zant_b200_kv_cache_attention(zant_ctx* ctx, const zant_kv_cache* cache, 
         a.q = s.ptr<void>(iq); a.q_stride = (long long)q_stride; a.heads = (int)heads; a.group = (int)group; a.q_type = dtype;
         a.out = s.ptr<void>(io); a.out_stride = (long long)out_stride; a.lse = s.ptr<float>(il);
         a.scale_log2 = scale * kLog2e; a.window = window; a.sinks = sinks;
-        a.wide_q = whole_blocks(a.q, q_stride, esz);
+        a.wide_q = whole_blocks(a.q, q_stride, esz); a.wide_out = whole_blocks(a.out, out_stride, esz);
         ZB_TRY(run_kv_attention(ctx, a));
         return s.finish();
     });

@@ -39,9 +39,10 @@ struct KvAttendArgs {
     void* out; long long out_stride; float* lse;
     float scale_log2;                                 // scale log2(e)
     int window, sinks;
-    bool wide_q;                                      // q in whole 16-byte blocks
-    int parts;                                        // CTAs of a tile
-    int* status;
+    bool wide_q, wide_out;                            // q, out in whole 16-byte blocks
+    int more_rows_than, rows_up_to;                   // sequences with more rows of a key head than the first, up to the second, are the kernel's
+    int parts, tiles_each;                            // CTAs of a tile; tiles of each sequence (0: by its rows)
+    int* status; long long wait_budget; int give_up;  // give_up: self test, a CTA whose first wait counts as run out (-1: none)
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -118,6 +119,8 @@ struct KvSteps {
     }
     __device__ __forceinline__ int at(int k, int S) const { return (k < sink ? k : k - sink + first) * S; }
 };
+// Some row at positions [low, high] sees one of the 16 tokens from t on.  (What the table says of others, and their pages' scales, is nobody's business.)
+__device__ __forceinline__ bool kv_seen16(int t, int low, int high, int window, int sinks) { return t <= high && (window == 0 || t + 15 > low - window || t < sinks); }
 
 template <int DP_, int NT_, bool SPLIT_>
 struct KvAttendCfg {
@@ -182,8 +185,13 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
     ptx::grid_start();
     const int work = (int)(blockIdx.x / (unsigned)P), h = work % c.heads;
     KvSeq q; int unit;
-    const bool any = kv_locate(c, work / c.heads, a.group, F::ROWS, 1, q, unit);
-    const int row0 = unit * F::ROWS, rows = any ? min(F::ROWS, q.n * a.group - row0) : 0;
+    bool any;
+    if (a.tiles_each > 0) {
+        unit = work / c.heads % a.tiles_each;
+        q = kv_seq(c, min(work / c.heads / a.tiles_each, c.seqs - 1));
+        any = q.n > 0;
+    } else any = kv_locate(c, work / c.heads, a.group, F::ROWS, 1, q, unit);
+    const int row0 = unit * F::ROWS, rows = any && q.n * a.group > a.more_rows_than && q.n * a.group <= a.rows_up_to ? min(F::ROWS, q.n * a.group - row0) : 0;
     if (rows <= 0) return;                            // (all CTAs of a cluster)
     const int low = max(q.first + row0 / a.group, -1), high = max(q.first + (row0 + rows - 1) / a.group, -1);      // (below zero: nothing is seen)
     const KvSteps steps(low, high, a.window, a.sinks, STEP);
@@ -199,10 +207,10 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
     };
     auto batch_of = [&](int i) {
         Batch b;
-        const int k = k0 + (i + lane) * stride_k, t = k < steps.total ? steps.at(k, STEP) >> pl : -1;
+        const int k = k0 + (i + lane) * stride_k, t = k < steps.total ? steps.at(k, STEP) : -1;
 #pragma unroll
         for (int z = 0; z < H; ++z) {
-            b.page[z] = z == 0 || two ? (int)kv_page(c, q.s, t < 0 ? -1 : t + z) : b.page[0];
+            b.page[z] = z == 0 || two ? (int)kv_page(c, q.s, t < 0 || (two && !kv_seen16(t + 16 * z, low, high, a.window, a.sinks)) ? -1 : (t >> pl) + z) : b.page[0];
             b.there[z] = __ballot_sync(0xffffffffu, b.page[z] >= 0);
             const long long at = (long long)max(b.page[z], 0) * c.heads + h;
             b.k[z] = z == 0 || two ? (b.page[z] >= 0 ? c.k_scale[at] : 0.0f) : b.k[0];
@@ -604,7 +612,12 @@ inline int32_t encode_kv_map(CUtensorMap* map, const void* p, const KvArgs& c, i
 template <int DP, int NT, bool SPLIT>
 inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     using F = KvAttendCfg<DP, NT, SPLIT>;
-    const long long tiles = kv_units(a.c, a.group, F::ROWS, 1), items = tiles * a.c.heads;
+    long long tiles = kv_units(a.c, a.group, F::ROWS, 1);
+    if (a.c.offsets && a.rows_up_to < 0x7fffffff) {       // others take the sequences with more rows: tiles for those with as many as are left
+        const int each = (a.rows_up_to + F::ROWS - 1) / F::ROWS;
+        if ((long long)each * a.c.seqs < tiles) { a.tiles_each = each; tiles = (long long)each * a.c.seqs; }
+    }
+    const long long items = tiles * a.c.heads;
     if (items > 0x7fffffffLL / 16) return fail(ZANT_E_TOO_LARGE, "%lld tiles of attention", items);
     // CTAs that share a tile: while they find room side by side and each warp has steps left to take
     const long long reach = std::min((long long)a.c.width << a.c.page_log2, a.window > 0 ? (long long)a.window + a.sinks + 2 * F::STEP : 0x7fffffffffLL);
@@ -633,14 +646,15 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
 
 template <int DP, bool SPLIT>
 inline int32_t choose_kv_attention(zant_ctx* ctx, const KvAttendArgs& a) {
-    const long long rows = ((long long)a.c.rows + a.c.seqs - 1) / a.c.seqs * a.group;
+    // (where others take the sequences with many rows, what is left has a token or a few)
+    const long long rows = a.rows_up_to < 0x7fffffff ? a.group : ((long long)a.c.rows + a.c.seqs - 1) / a.c.seqs * a.group;
     if (rows <= 8) return launch_kv_attention<DP, 1, SPLIT>(ctx, a);
     if constexpr (DP <= 128 && !SPLIT)
         if (rows > 16) return launch_kv_attention<DP, 4, SPLIT>(ctx, a);
     return launch_kv_attention<DP, 2, SPLIT>(ctx, a);
 }
 
-inline int32_t run_kv_attention(zant_ctx* ctx, const KvAttendArgs& a) {
+inline int32_t run_kv_few(zant_ctx* ctx, const KvAttendArgs& a) {
     const bool split = a.q_type == ZANT_F32;
     if (a.c.dim <= 64) return split ? choose_kv_attention<64, true>(ctx, a) : choose_kv_attention<64, false>(ctx, a);
     if (a.c.dim <= 128) return split ? choose_kv_attention<128, true>(ctx, a) : choose_kv_attention<128, false>(ctx, a);

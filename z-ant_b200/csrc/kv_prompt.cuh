@@ -1,0 +1,527 @@
+// Attention of many new tokens (prompts, parts of them) over the cache of kv_cache.cuh on tcgen05: the formulas and masks of kv_attention.cuh for results in 16 bits.
+//
+// A CTA has 256 rows, (new token, head) pairs that share a key head, as two tiles of 128 that take turns: while the tensor core multiplies for one, the other one's
+// exponentials are taken.  Steps of 128 tokens.  Codes become f16 (exactly) once for all 256 rows; q is f16 times a power of two for each row, so that its largest value lies in
+// [2^14, 2^15) (f16 and bf16 values lose nothing down to 2^-28 of that one).  Scores are 128 x 128 x dim products into tensor memory; each thread has a row of them, finds its maximum, and
+// writes the weights back over them as f16, where they are the next product's operand.
+//
+// A page's scale of K multiplies its columns' scores; its scale of V, over the largest of the pages that the CTA sees, goes into the exponent: weights are 2^(x - m + lv + 10) with
+// lv = log2(vs / VS) in [-24, 0], so that what is rounded to f16 is at most 2^14 (the maximum is raised when it has grown by 2^4, and then what has been summed is rescaled), and
+// what is lost below f16's least numbers is 2^-35 of the largest weight.  The sum of the weights takes the factor out again, once for 16 tokens.
+//
+//   warps 0 .. 3, 4 .. 7  rows of the first and the second tile      8 .. 11  codes to f16      12  TMEM owner, MMA issuer
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "context.cuh"
+#include "kv_attention.cuh"
+#include "kv_cache.cuh"
+#include "ptx_sm100.cuh"
+#include "row_codes.cuh"
+
+namespace zb {
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+          "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Waits for the thread's loads; the registers of one of them are only read behind it.
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+}
+
+// f16 operands, fp32 sums, K-major A; B K-major, or with its N index the contiguous one.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) {
+    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// One lane of a whole warp (`leader`): D (+)= A B with A in shared memory, or in tensor memory.
+__device__ __forceinline__ void mma_f16_ss_if(uint32_t leader, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%6, %6, %6, %6}, p;\n\t}\n"
+                 ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts_if(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%6, %6, %6, %6}, p;\n\t}\n"
+                 ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader), "r"(0u) : "memory");
+}
+// Rows of 128 bytes in the 128-byte swizzle, 8 rows 1024 bytes: K index in the row (K-major); N index in the row, the next 64 of them `block` bytes further.
+__device__ __forceinline__ uint64_t kv_desc(uint32_t addr, uint32_t block) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)((block >> 4) & 0x3fffu) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <int DP_>
+struct KvPromptCfg {
+    static constexpr int DP = DP_, TILE = 128, ROWS = 2 * TILE, STEP = 128, WARPS = 13, THREADS = 32 * WARPS;
+    static constexpr int BLOCK = TILE * 128;          // 128 rows of 64 f16 numbers
+    static constexpr int OPERAND = BLOCK * (DP / 64); // Q of a tile, K or V of a step
+    static constexpr int OFF_K = 2 * OPERAND, OFF_V = 4 * OPERAND, OFF_REST = 6 * OPERAND;
+    static constexpr int LPR = DP / 16;               // lanes of a row of codes
+    static constexpr int LOADS = DP / 16;             // 16-byte loads of a thread for 128 tokens
+    static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 10) of 16 tokens each, which of them there are
+    // factors of rows, info of 4 steps, maxima of scales, barriers, address of TMEM, flag
+    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 16, OFF_TMEM = OFF_BAR + 16 * 8, SMEM = OFF_TMEM + 16;
+};
+struct KvPromptBars {
+    uint32_t at;
+    __device__ __forceinline__ uint32_t k_full(int s) const { return at + 8 * s; }
+    __device__ __forceinline__ uint32_t v_full(int s) const { return at + 16 + 8 * s; }
+    __device__ __forceinline__ uint32_t k_empty(int s) const { return at + 32 + 8 * s; }
+    __device__ __forceinline__ uint32_t v_empty(int s) const { return at + 48 + 8 * s; }
+    __device__ __forceinline__ uint32_t s_full(int x) const { return at + 64 + 8 * x; }
+    __device__ __forceinline__ uint32_t p_full(int x) const { return at + 80 + 8 * x; }
+    __device__ __forceinline__ uint32_t o_full(int x) const { return at + 96 + 8 * x; }
+    __device__ __forceinline__ uint32_t q_full() const { return at + 112; }
+    __device__ __forceinline__ uint32_t drained() const { return at + 120; }
+};
+
+// What all roles know of the CTA's rows.
+struct KvPromptTile {
+    int s, row, first, row0, rows, h;                 // sequence, its first row, position of its first new token, first of the CTA's rows, how many, key head
+    int low[2], high[2];                              // positions of either tile's first and last row (high < 0: the tile has none, or sees nothing)
+    __device__ __forceinline__ bool active(int x, int t, int window, int sinks) const {
+        return t <= high[x] && (window == 0 || t + 127 > low[x] - window || t < sinks);
+    }
+    // every row sees all of the step
+    __device__ __forceinline__ bool whole(int x, int t, int window, int sinks) const {
+        return t + 127 <= low[x] && (window == 0 || t > high[x] - window || t + 128 <= sinks);
+    }
+};
+
+__device__ __forceinline__ bool kv_wait(const KvAttendArgs& a, uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag, a.wait_budget));
+}
+
+// ---- warps 8 .. 11
+template <typename F>
+__device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
+    constexpr int LPR = F::LPR, N = F::LOADS;
+    const KvArgs& c = a.c;
+    const int tid = threadIdx.x - 256, lane = tid & 31, warp = tid >> 5, pl = c.page_log2, inpage = c.page - 1;
+    float* row_factor = reinterpret_cast<float*>(smem + F::OFF_REST);
+    float* info = reinterpret_cast<float*>(smem + F::OFF_INFO);
+    float* part = reinterpret_cast<float*>(smem + F::OFF_MAX);
+    const int mine = tid % LPR, token0 = tid / LPR;   // the thread's 16 dimensions, and its token of each 128 / LPR
+    constexpr int TOKENS = 128 / LPR;                 // tokens of one load of all threads: 16 (32)
+    // the place of 16 f16 numbers, two chunks, in row r of an operand
+    auto place = [&](int r, int half) { return (mine >> 2) * F::BLOCK + r * 128 + ((((mine & 3) * 2 + half) ^ (r & 7)) << 4); };
+
+    // pages of 16 tokens each of a step: lane i (of 8) has the i-th
+    const int low = tile.low[0], high = max(tile.high[0], tile.high[1]);
+    auto page_of = [&](int k) {
+        if (k >= steps.total) return -1;
+        const int t = steps.at(k, 128) + 16 * (lane & 7);
+        return kv_seen16(t, low, high, a.window, a.sinks) ? (int)kv_page(c, tile.s, t >> pl) : -1;
+    };
+    uint4 w[N];
+    auto load = [&](const int8_t* codes, int page, int k) {
+        const int t = k < steps.total ? steps.at(k, 128) : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int token = i * TOKENS + token0, id = __shfl_sync(0xffffffffu, page, token >> 4);
+            const bool in = id >= 0 && mine * 16 < c.dim;
+            const int8_t* p = codes + (((long long)(in ? id : 0) * c.heads + tile.h) * c.page + ((t + token) & inpage)) * c.dim + mine * 16;
+            w[i] = in ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    auto convert = [&](uint8_t* to) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t r[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            uint32_t f[8];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) { f[2 * z] = codes_f16(r[z]); f[2 * z + 1] = codes_f16(r[z] >> 8); }       // (numbers 0, 2, 1, 3 of each four)
+            const int row = i * TOKENS + token0, first = (mine >> 2) & 1;              // (the upper 64 dimensions the other way round: no bank twice)
+            *reinterpret_cast<uint4*>(to + place(row, first)) = make_uint4(f[4 * first], f[4 * first + 1], f[4 * first + 2], f[4 * first + 3]);
+            *reinterpret_cast<uint4*>(to + place(row, 1 - first)) = make_uint4(f[4 - 4 * first], f[5 - 4 * first], f[6 - 4 * first], f[7 - 4 * first]);
+        }
+    };
+    auto done = [&](uint32_t b) {
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(b);
+    };
+    int page = page_of(0);
+    load(c.k, page, 0);
+
+    // the largest scale of V that any row sees
+    float top = 0.0f;
+    if (steps.total > 0) {
+        const int from = a.window > 0 ? max(low - a.window + 1, 0) >> pl : 0, to = (high >> pl) + 1;
+        const int sink_pages = a.sinks > 0 ? min(((a.sinks - 1) >> pl) + 1, from) : 0;
+#pragma unroll 4
+        for (int i = tid; i < sink_pages + to - from; i += 128) {
+            const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
+            if (id >= 0) top = fmaxf(top, fabsf(c.v_scale[id * c.heads + tile.h]));
+        }
+    }
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if (lane == 0) part[warp] = top;
+
+    // q
+    constexpr int RPP = 4 * (32 / LPR);               // rows that four warps take at once
+#pragma unroll 2
+    for (int r0 = 0; r0 < F::ROWS; r0 += RPP) {
+        const int r = r0 + tid / LPR, row = tile.row0 + r;
+        const bool there = r < tile.rows && mine * 16 < c.dim;
+        float v[16];
+        if (there) kv_values16(a.q, a.q_type, a.wide_q, (long long)(tile.row + row / a.group) * a.q_stride + (long long)(tile.h * a.group + row % a.group) * c.dim + mine * 16, v);
+        else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+        }
+        float big = 0.0f;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { big = fmaxf(big, fabsf(v[i])); odd |= !(fabsf(v[i]) < INFINITY); }
+#pragma unroll
+        for (int d = LPR / 2; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+        odd = (__ballot_sync(0xffffffffu, odd) >> (lane / LPR * LPR)) & ((1u << LPR) - 1u);
+        const int e = min(max((int)(__float_as_uint(big) >> 23) - 127 - 14, -114), 127);
+        const float down = odd ? 0.0f : __uint_as_float((uint32_t)(127 - e) << 23), up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(127 + e, 1) << 23);
+        if (mine == 0) row_factor[r] = up * a.scale_log2;
+        uint32_t f[8];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = odd ? 0.0f : v[4 * z + i] * down;
+            f[2 * z] = pack_f16(x[0], x[2]);
+            f[2 * z + 1] = pack_f16(x[1], x[3]);
+        }
+        uint8_t* to = smem + (r >> 7) * F::OPERAND;
+        *reinterpret_cast<uint4*>(to + place(r & 127, 0)) = make_uint4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<uint4*>(to + place(r & 127, 1)) = make_uint4(f[4], f[5], f[6], f[7]);
+    }
+    done(bar.q_full());
+    ptx::named_barrier_sync(1, 128);                  // (in front of any wait that may be given up)
+    const float vs = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+
+    for (int k = 0; k < steps.total; ++k) {
+        const int s = k & 1;
+        const uint32_t free_parity = ((uint32_t)(k >> 1) & 1u) ^ 1u;
+        if (!kv_wait(a, bar.k_empty(s), free_parity, abort_flag)) return;
+        convert(smem + F::OFF_K + s * F::OPERAND);
+        done(bar.k_full(s));
+        load(c.v, page, k);
+        if (warp == 0 && lane < 8) {
+            float* i = info + (k & 3) * F::INFO;
+            const long long at = (long long)max(page, 0) * c.heads + tile.h;
+            const float ks = page >= 0 ? c.k_scale[at] : 0.0f, mine_v = page >= 0 ? c.v_scale[at] : 0.0f;
+            float lv = vs > 0.0f ? __log2f(fabsf(mine_v) / vs) : 0.0f;
+            lv = lv < -24.0f ? -24.0f : (lv > 0.0f ? 0.0f : lv);       // (NaN stays)
+            i[lane] = ks; i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 10.0f);
+            const unsigned there = __ballot_sync(0xffu, page >= 0);
+            if (lane == 0) reinterpret_cast<int*>(i)[24] = (int)there;
+        }
+        __syncwarp();
+        const int next = page_of(k + 1);
+        if (!kv_wait(a, bar.v_empty(s), free_parity, abort_flag)) return;
+        convert(smem + F::OFF_V + s * F::OPERAND);
+        done(bar.v_full(s));
+        page = next;
+        load(c.k, page, k + 1);
+    }
+}
+
+// ---- warp 12
+template <typename F>
+__device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint32_t s0, uint32_t tmem, volatile int* abort_flag) {
+    constexpr int DP = F::DP;
+    constexpr uint32_t idesc_s = idesc_f16(128, 128, false), idesc_o = idesc_f16(128, DP, true);
+    const uint32_t leader = ptx::elect_one() ? 1u : 0u;
+    int count[2] = {0, 0};                            // products P V so far
+    int last[2] = {-1, -1};                           // a tile's last step
+    for (int k = 0; k < steps.total; ++k)
+        for (int x = 0; x < 2; ++x)
+            if (tile.active(x, steps.at(k, 128), a.window, a.sinks)) last[x] = k;
+    auto scores = [&](int x, int k) {
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const uint32_t at = (i >> 2) * F::BLOCK + (i & 3) * 32;
+            mma_f16_ss_if(leader, tmem + x * 128, kv_desc(s0 + x * F::OPERAND + at, 16), kv_desc(s0 + F::OFF_K + (k & 1) * F::OPERAND + at, 16), idesc_s, i > 0);
+        }
+        ptx::mma_commit_if(leader, bar.s_full(x));
+    };
+    auto values = [&](int x, int k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            mma_f16_ts_if(leader, tmem + 256 + x * DP, tmem + x * 128 + i * 8, kv_desc(s0 + F::OFF_V + (k & 1) * F::OPERAND + i * 2048, F::BLOCK), idesc_o, (count[x] | i) != 0);
+        ++count[x];
+        if (k == last[x]) ptx::mma_commit_if(leader, bar.o_full(x));
+    };
+    auto active = [&](int x, int k) { return k < steps.total && tile.active(x, steps.at(k, 128), a.window, a.sinks); };
+    if (steps.total > 0) {
+        if (!kv_wait(a, bar.q_full(), 0, abort_flag) || !kv_wait(a, bar.k_full(0), 0, abort_flag)) return;
+        ptx::tc_fence_after();
+        for (int x = 0; x < 2; ++x) if (active(x, 0)) scores(x, 0);
+        ptx::mma_commit_if(leader, bar.k_empty(0));
+    }
+    for (int k = 0; k < steps.total; ++k) {
+        const uint32_t parity = (uint32_t)(k >> 1) & 1u, next_parity = (uint32_t)((k + 1) >> 1) & 1u;
+        if (!kv_wait(a, bar.v_full(k & 1), parity, abort_flag)) return;
+        bool k_there = false;
+        for (int x = 0; x < 2; ++x) {
+            if (active(x, k)) {
+                if (!kv_wait(a, bar.p_full(x), (uint32_t)count[x] & 1u, abort_flag)) return;
+                ptx::tc_fence_after();
+                values(x, k);
+            }
+            if (x == 1) ptx::mma_commit_if(leader, bar.v_empty(k & 1));
+            if (k + 1 < steps.total) {
+                if (!k_there && !kv_wait(a, bar.k_full((k + 1) & 1), next_parity, abort_flag)) return;
+                k_there = true;
+                ptx::tc_fence_after();
+                if (active(x, k + 1)) scores(x, k + 1);
+            }
+        }
+        if (k + 1 < steps.total) ptx::mma_commit_if(leader, bar.k_empty((k + 1) & 1));
+    }
+}
+
+// ---- warps 0 .. 7, a row each thread
+template <typename F>
+__device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, uint32_t tmem, volatile int* abort_flag) {
+    constexpr int DP = F::DP;
+    const KvArgs& c = a.c;
+    const int x = threadIdx.x >> 7, r = threadIdx.x & 127, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = x * 128 + r;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + x * 128 + lanes, to = tmem + 256 + x * DP + lanes;
+    const float* info = reinterpret_cast<const float*>(smem + F::OFF_INFO);
+    const int row = tile.row0 + min(mine, tile.rows - 1), pos = max(tile.first + row / a.group, -1);
+    float factor = 0.0f, m = -INFINITY, l = 0.0f;
+    int count = 0;
+    for (int k = 0; k < steps.total; ++k) {
+        const int t = steps.at(k, 128);
+        if (!tile.active(x, t, a.window, a.sinks)) continue;
+        if (!kv_wait(a, bar.v_full(k & 1), (uint32_t)(k >> 1) & 1u, abort_flag)) return;       // what the step's pages say
+        if (!kv_wait(a, bar.s_full(x), (uint32_t)count & 1u, abort_flag)) return;
+        ptx::tc_fence_after();
+        if (count == 0) factor = reinterpret_cast<const float*>(smem + F::OFF_REST)[mine];
+        const float* i = info + (k & 3) * F::INFO;
+        const int there = reinterpret_cast<const int*>(i)[24];
+        const bool whole = there == 255 && tile.whole(x, t, a.window, a.sinks);
+        const int upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
+        auto seen = [&](int col) { return col <= upto && (col > behind || col < sunk) && ((there >> (col >> 4)) & 1); };
+        // the row's maximum
+        float top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint32_t v[32];
+            ptx::tmem_ld32(ts + g * 32, v);
+            ptx::tmem_wait_ld32(v);
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const float f = factor * i[2 * g + z];
+                if (whole) {
+                    float b = __uint_as_float(v[16 * z]);
+#pragma unroll
+                    for (int y = 1; y < 16; ++y) b = fmaxf(b, __uint_as_float(v[16 * z + y]));
+                    top = fmaxf(top, b * f);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) top = fmaxf(top, seen(32 * g + 16 * z + y) ? __uint_as_float(v[16 * z + y]) * f : -INFINITY);
+                }
+            }
+        }
+        const bool raise = top > m + 4.0f;            // (also from minus infinity)
+        if (__any_sync(0xffffffffu, raise)) {
+            const float f = raise ? (m == -INFINITY ? 0.0f : ex2(m - top)) : 1.0f;
+            if (raise) { l *= f; m = top; }
+            if (count > 0) {
+#pragma unroll
+                for (int g = 0; g < DP / 16; ++g) {
+                    uint32_t v[16];
+                    ptx::tmem_ld16(to + g * 16, v);
+                    tmem_wait_ld16(v);
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) * f);
+                    tmem_st16(to + g * 16, v);
+                }
+            }
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint32_t v[32], p[16];
+            ptx::tmem_ld32(ts + g * 32, v);
+            ptx::tmem_wait_ld32(v);
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const float f = factor * i[2 * g + z], b = i[8 + 2 * g + z] + 10.0f - base;
+                const unsigned long long f2 = ptx::pack2(f, f), b2 = ptx::pack2(b, b);
+                unsigned long long sum = 0;
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    const int at = 16 * z + 2 * y;
+                    const float2 e = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), f2, b2));
+                    float2 w = make_float2(ex2(e.x), ex2(e.y));
+                    if (!whole) {
+                        if (!seen(32 * g + at)) w.x = 0.0f;
+                        if (!seen(32 * g + at + 1)) w.y = 0.0f;
+                    }
+                    sum = ptx::add2(sum, ptx::pack2(w.x, w.y));
+                    p[8 * z + y] = pack_f16(w.x, w.y);
+                }
+                const float2 s2 = ptx::unpack2(sum);
+                const float s1 = s2.x + s2.y;
+                l = s1 == 0.0f ? l : fmaf(s1, i[16 + 2 * g + z], l);       // (the factor of a page that the row does not see may be NaN)
+            }
+            tmem_st16(ts + g * 16, p);
+        }
+        tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar.p_full(x));
+        ++count;
+    }
+    if (count > 0) {
+        if (!kv_wait(a, bar.o_full(x), 0, abort_flag)) return;
+        ptx::tc_fence_after();
+    }
+    const float* part = reinterpret_cast<const float*>(smem + F::OFF_MAX);
+    float vs = 0.0f;
+    if (count > 0) vs = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    const bool mine_there = mine < tile.rows;
+    const float out_scale = l == 0.0f ? 0.0f : vs * (1.0f / 1024.0f) / l;
+    const long long token = tile.row + row / a.group, head = tile.h * a.group + row % a.group, at = token * a.out_stride + head * c.dim;
+#pragma unroll
+    for (int g = 0; g < DP / 16; ++g) {
+        uint32_t v[16];
+        if (count > 0) {                              // (the same for the whole warp)
+            ptx::tmem_ld16(to + g * 16, v);
+            tmem_wait_ld16(v);
+        } else {
+#pragma unroll
+            for (int y = 0; y < 16; ++y) v[y] = 0;
+        }
+        if (mine_there && g * 16 < c.dim) {
+            uint32_t w[8];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {             // numbers 0, 2, 1, 3 of each four
+                const float d0 = __uint_as_float(v[4 * y]) * out_scale, d2 = __uint_as_float(v[4 * y + 1]) * out_scale, d1 = __uint_as_float(v[4 * y + 2]) * out_scale,
+                            d3 = __uint_as_float(v[4 * y + 3]) * out_scale;
+                if (a.q_type == ZANT_F16) { w[2 * y] = pack_f16(d0, d1); w[2 * y + 1] = pack_f16(d2, d3); }
+                else {
+                    const __nv_bfloat162 b0 = __floats2bfloat162_rn(d0, d1), b1 = __floats2bfloat162_rn(d2, d3);
+                    w[2 * y] = *reinterpret_cast<const uint32_t*>(&b0); w[2 * y + 1] = *reinterpret_cast<const uint32_t*>(&b1);
+                }
+            }
+            uint16_t* o = static_cast<uint16_t*>(a.out) + at + g * 16;
+            if (a.wide_out) {
+                reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+#pragma unroll
+                for (int y = 0; y < 16; ++y) o[y] = (uint16_t)(w[y >> 1] >> (16 * (y & 1)));
+            }
+        }
+    }
+    if (a.lse && mine_there) a.lse[token * a.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(const __grid_constant__ KvAttendArgs a) {
+    using F = KvPromptCfg<DP>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const KvArgs& c = a.c;
+    const int warp = threadIdx.x >> 5;
+    const uint32_t s0 = ptx::smem_u32(smem);
+    const KvPromptBars bar{s0 + F::OFF_BAR};
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + F::OFF_TMEM + 8);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(bar.k_full(i), 4); ptx::mbar_init(bar.v_full(i), 4);
+            ptx::mbar_init(bar.k_empty(i), 1); ptx::mbar_init(bar.v_empty(i), 1);
+            ptx::mbar_init(bar.s_full(i), 1); ptx::mbar_init(bar.p_full(i), 4); ptx::mbar_init(bar.o_full(i), 1);
+        }
+        ptx::mbar_init(bar.q_full(), 4); ptx::mbar_init(bar.drained(), 1);
+        ptx::mbar_fence_init();
+        *abort_flag = (int)blockIdx.x == a.give_up ? 1 : 0;
+    }
+    if (warp == 12) {
+        ptx::tmem_alloc(s0 + F::OFF_TMEM, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + F::OFF_TMEM);
+    ptx::grid_start();
+
+    // late tiles see the most tokens: they go first
+    const int units = (int)(gridDim.x / (unsigned)c.heads), work = units - 1 - (int)(blockIdx.x / (unsigned)c.heads);
+    KvPromptTile tile;
+    KvSeq q; int unit;
+    const bool any = kv_locate(c, work, a.group, F::ROWS, 1, q, unit);
+    tile.h = (int)(blockIdx.x % (unsigned)c.heads);
+    tile.row0 = unit * F::ROWS;
+    tile.rows = any && q.n * a.group > a.more_rows_than ? min(F::ROWS, q.n * a.group - tile.row0) : 0;
+    if (tile.rows > 0) {                              // (the same for the whole CTA)
+        tile.s = q.s; tile.row = q.row; tile.first = q.first;
+        for (int x = 0; x < 2; ++x) {
+            const int b = tile.row0 + x * 128, e = tile.row0 + min(tile.rows, (x + 1) * 128) - 1;
+            tile.low[x] = max(q.first + b / a.group, -1);
+            tile.high[x] = e < b ? -1 : max(q.first + e / a.group, -1);
+        }
+        const KvSteps steps(tile.low[0], max(tile.high[0], tile.high[1]), a.window, a.sinks, 128);
+        if (warp < 8) kv_prompt_rows<F>(a, tile, steps, bar, smem, tmem, abort_flag);
+        else if (warp < 12) kv_prompt_convert<F>(a, tile, steps, bar, smem, abort_flag);
+        else {
+            kv_prompt_mma<F>(a, tile, steps, bar, s0, tmem, abort_flag);
+            // what the tensor core still does ends before its operands' memory is another kernel's, also where a wait was given up
+            const uint32_t leader = ptx::elect_one() ? 1u : 0u;
+            ptx::mma_commit_if(leader, bar.drained());
+            volatile int no = 0;
+            ptx::mbar_wait(bar.drained(), 0, &no);
+        }
+    }
+    __syncwarp();
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, (int)DEV_ERR_WAIT_TIMEOUT);
+}
+
+template <int DP>
+inline int32_t launch_kv_prompt(zant_ctx* ctx, KvAttendArgs a) {
+    using F = KvPromptCfg<DP>;
+    const long long grid = kv_units(a.c, a.group, F::ROWS, 1) * a.c.heads;
+    if (grid > 0x7fffffffLL) return fail(ZANT_E_TOO_LARGE, "%lld tiles of attention", grid);
+    a.status = ctx->status_word;
+    a.give_up = ctx->give_up_cta < 0 ? -1 : (int)(ctx->give_up_cta % grid);
+    ctx->give_up_cta = -1;
+    a.wait_budget = a.give_up < 0 ? ptx::kWaitBudgetCycles : 4000000;
+    ZB_SMEM_ATTR(ctx, kv_prompt_kernel<DP>, F::SMEM);
+    launch(ctx, kv_prompt_kernel<DP>, dim3((unsigned)grid), F::THREADS, F::SMEM, a);
+    return check_launch(ctx, "kv_prompt_kernel");
+}
+
+// Rows of a key head from which on a sequence is a prompt.
+constexpr int kPromptRows = 64;
+
+inline int32_t run_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
+    a.more_rows_than = 0; a.rows_up_to = 0x7fffffff;
+    if (a.q_type == ZANT_F32 || a.c.dim > 128) return run_kv_few(ctx, a);
+    // Which sequences have many rows is known on the device only, unless all have the same number: both kernels run then, and each takes its own.
+    const bool uniform = !a.c.offsets;
+    const long long most = uniform ? (long long)a.c.per * a.group : (long long)a.c.rows * a.group;
+    if (most > kPromptRows) {
+        KvAttendArgs p = a;
+        p.more_rows_than = kPromptRows;
+        ZB_TRY(a.c.dim <= 64 ? launch_kv_prompt<64>(ctx, p) : launch_kv_prompt<128>(ctx, p));
+        if (uniform) return ZANT_OK;
+        a.rows_up_to = kPromptRows;
+    }
+    return run_kv_few(ctx, a);
+}
+
+}  // namespace zb
