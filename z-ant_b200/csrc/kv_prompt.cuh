@@ -285,14 +285,55 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
     }
 }
 
+// Weights of a row's 128 scores in tensor memory at `ts`, in pairs, under the base `base` (log2): p, their sum with each page's factor taken out, and the largest exponent.
+// WHOLE: the row sees all of them; else columns up to `upto`, and behind `behind` or in front of `sunk`, on pages that are there.
+template <bool WHOLE>
+__device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* info, float factor, float base, int there, int upto, int behind, int sunk, uint32_t (&p)[64], float& sum) {
+    uint32_t v[2][16];
+    float top = -INFINITY;
+    sum = 0.0f;
+    ptx::tmem_ld16(ts, v[0]);
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {                     // 16 tokens, which are on one page
+        tmem_wait_ld16(v[g & 1]);
+        if (g < 7) ptx::tmem_ld16(ts + 16 * (g + 1), v[(g + 1) & 1]);
+        const float f = factor * info[g], lv = info[8 + g], b = lv + 10.0f - base;
+        const unsigned long long f2 = ptx::pack2(f, f), b2 = ptx::pack2(b, b);
+        unsigned long long s2 = 0;
+        float most = -INFINITY;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            float2 e = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(v[g & 1][2 * y]), __uint_as_float(v[g & 1][2 * y + 1])), f2, b2));
+            if (!WHOLE) {
+                const int at = 16 * g + 2 * y;
+                const bool on = (there >> g) & 1;
+                if (!(on && at <= upto && (at > behind || at < sunk))) e.x = -INFINITY;
+                if (!(on && at + 1 <= upto && (at + 1 > behind || at + 1 < sunk))) e.y = -INFINITY;
+            }
+            most = fmaxf(most, fmaxf(e.x, e.y));
+            const float2 w = make_float2(ex2(e.x), ex2(e.y));
+            s2 = ptx::add2(s2, ptx::pack2(w.x, w.y));
+            p[8 * g + y] = pack_f16(w.x, w.y);
+        }
+        top = fmaxf(top, most - lv);
+        const float2 s1 = ptx::unpack2(s2);
+        const float add = (s1.x + s1.y) * info[16 + g];
+        sum += WHOLE || s1.x + s1.y != 0.0f ? add : 0.0f;              // (the factor of a page that the row does not see may be NaN)
+    }
+    return top - 10.0f;
+}
+
 // ---- warps 0 .. 7, a row each thread
+//
+// The base of the exponents is the maximum of earlier steps: one pass over the scores gives weights and their maximum, and only where that has grown by 2^4 (a row's first step, and few
+// others) it is taken again.  (A pass for the maximum in front: twice the time.)
 template <typename F>
 __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, uint32_t tmem, volatile int* abort_flag) {
     constexpr int DP = F::DP;
     const KvArgs& c = a.c;
     const int x = threadIdx.x >> 7, r = threadIdx.x & 127, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = x * 128 + r;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + x * 128 + lanes, to = tmem + 256 + x * DP + lanes;
-    const float* info = reinterpret_cast<const float*>(smem + F::OFF_INFO);
+    const float* all_info = reinterpret_cast<const float*>(smem + F::OFF_INFO);
     const int row = tile.row0 + min(mine, tile.rows - 1), pos = max(tile.first + row / a.group, -1);
     float factor = 0.0f, m = -INFINITY, l = 0.0f;
     int count = 0;
@@ -303,38 +344,22 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
         if (!kv_wait(a, bar.s_full(x), (uint32_t)count & 1u, abort_flag)) return;
         ptx::tc_fence_after();
         if (count == 0) factor = reinterpret_cast<const float*>(smem + F::OFF_REST)[mine];
-        const float* i = info + (k & 3) * F::INFO;
-        const int there = reinterpret_cast<const int*>(i)[24];
+        const float* info = all_info + (k & 3) * F::INFO;
+        const int there = reinterpret_cast<const int*>(info)[24];
         const bool whole = there == 255 && tile.whole(x, t, a.window, a.sinks);
         const int upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
-        auto seen = [&](int col) { return col <= upto && (col > behind || col < sunk) && ((there >> (col >> 4)) & 1); };
-        // the row's maximum
-        float top = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            uint32_t v[32];
-            ptx::tmem_ld32(ts + g * 32, v);
-            ptx::tmem_wait_ld32(v);
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                const float f = factor * i[2 * g + z];
-                if (whole) {
-                    float b = __uint_as_float(v[16 * z]);
-#pragma unroll
-                    for (int y = 1; y < 16; ++y) b = fmaxf(b, __uint_as_float(v[16 * z + y]));
-                    top = fmaxf(top, b * f);
-                } else {
-#pragma unroll
-                    for (int y = 0; y < 16; ++y) top = fmaxf(top, seen(32 * g + 16 * z + y) ? __uint_as_float(v[16 * z + y]) * f : -INFINITY);
-                }
-            }
-        }
-        const bool raise = top > m + 4.0f;            // (also from minus infinity)
-        if (__any_sync(0xffffffffu, raise)) {
-            const float f = raise ? (m == -INFINITY ? 0.0f : ex2(m - top)) : 1.0f;
-            if (raise) { l *= f; m = top; }
+        uint32_t p[64];
+        float sum;
+        for (int again = 0; again < 2; ++again) {
+            const float base = m == -INFINITY ? 0.0f : m;
+            const float top = whole ? kv_prompt_weights<true>(ts, info, factor, base, there, upto, behind, sunk, p, sum)
+                                    : kv_prompt_weights<false>(ts, info, factor, base, there, upto, behind, sunk, p, sum);
+            const bool raise = m == -INFINITY ? top > -INFINITY : top > 4.0f;
+            if (again || !__any_sync(0xffffffffu, raise)) break;
+            const float to_m = base + top, f = raise ? (m == -INFINITY ? 0.0f : ex2(m - to_m)) : 1.0f;
+            if (raise) { l *= f; m = to_m; }
             if (count > 0) {
-#pragma unroll
+#pragma unroll 1
                 for (int g = 0; g < DP / 16; ++g) {
                     uint32_t v[16];
                     ptx::tmem_ld16(to + g * 16, v);
@@ -345,35 +370,9 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
                 }
             }
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        l += sum;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            uint32_t v[32], p[16];
-            ptx::tmem_ld32(ts + g * 32, v);
-            ptx::tmem_wait_ld32(v);
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                const float f = factor * i[2 * g + z], b = i[8 + 2 * g + z] + 10.0f - base;
-                const unsigned long long f2 = ptx::pack2(f, f), b2 = ptx::pack2(b, b);
-                unsigned long long sum = 0;
-#pragma unroll
-                for (int y = 0; y < 8; ++y) {
-                    const int at = 16 * z + 2 * y;
-                    const float2 e = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), f2, b2));
-                    float2 w = make_float2(ex2(e.x), ex2(e.y));
-                    if (!whole) {
-                        if (!seen(32 * g + at)) w.x = 0.0f;
-                        if (!seen(32 * g + at + 1)) w.y = 0.0f;
-                    }
-                    sum = ptx::add2(sum, ptx::pack2(w.x, w.y));
-                    p[8 * z + y] = pack_f16(w.x, w.y);
-                }
-                const float2 s2 = ptx::unpack2(sum);
-                const float s1 = s2.x + s2.y;
-                l = s1 == 0.0f ? l : fmaf(s1, i[16 + 2 * g + z], l);       // (the factor of a page that the row does not see may be NaN)
-            }
-            tmem_st16(ts + g * 16, p);
-        }
+        for (int g = 0; g < 4; ++g) tmem_st16(ts + g * 16, p + 16 * g);
         tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();
