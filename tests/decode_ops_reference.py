@@ -88,8 +88,8 @@ def attention(cache, q, table, lengths, offsets, kind, scale=None, window=0, sin
     A score x is a sum of dim products of exact codes with q, which is exact or (few rows) rounded to whole numbers of which the row's largest is 2^19 (2^26 for f32) at least,
     half a step of which is 2^-20 (2^-27) of that value; added exactly or in fp32 with at most one step (2 U) of the sum of magnitudes for each, times three factors: off by
     dx = 2 U (dim + 2) scale sum |q k| + 2^-20 scale max |q| sum |k| and, with the difference to the maximum and the power of two, by 6 U |x - max| + 8 U relative to the weight.  A weight in f16 is
-    off by 2**-11, in two f16 numbers by 2**-22, and by 2**-35 of the largest weight times the largest value where it is tiny
-    (the rounding below f16's least numbers, of weights that are at least 2**10 at the largest).  Sums over n tokens are
+    off by 2**-11, in two f16 numbers by 2**-22, and by 2**-31 of the largest weight times the largest value where it is tiny
+    (the rounding below f16's least numbers, of weights that are at least 2**6 at the largest).  Sums over n tokens are
     added in fp32, 16 at a time, and rescaled at most every 32: n / 4 + 64 steps in all."""
     rows, heads, dim = q.shape
     group = heads // cache.heads
@@ -128,7 +128,7 @@ def attention(cache, q, table, lengths, offsets, kind, scale=None, window=0, sin
                         dw = 2 * (dx + 8 * U + 6 * U * np.abs(x - top))
                         mean = w @ np.abs(v[j])
                         wide = 2 * U * (len(j) / 4 + 64)
-                        o = (w * (dw + h16)) @ np.abs(v[j]) + mean * (w @ dw + 2 * wide) + 2.0 ** -35 * w.max() * np.abs(v[j]).max() * len(j)
+                        o = (w * (dw + h16)) @ np.abs(v[j]) + mean * (w @ dw + 2 * wide) + 2.0 ** -31 * w.max() * np.abs(v[j]).max() * len(j)
                         off[row + i, g] = o + HALF_STEP[kind] * (np.abs(out[row + i, g]) + o) + LEAST[kind]
                         lse[row + i, g] = top + np.log(e.sum())
                         lse_off[row + i, g] = (w @ dw) + wide + 8 * U * (1 + abs(lse[row + i, g]) + abs(top))

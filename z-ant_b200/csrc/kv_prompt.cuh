@@ -5,9 +5,9 @@
 // [2^14, 2^15) (f16 and bf16 values lose nothing down to 2^-28 of that one).  Scores are 128 x 128 x dim products into tensor memory; each thread has a row of them, finds its maximum, and
 // writes the weights back over them as f16, where they are the next product's operand.
 //
-// A page's scale of K multiplies its columns' scores; its scale of V, over the largest of the pages that the CTA sees, goes into the exponent: weights are 2^(x - m + lv + 10) with
-// lv = log2(vs / VS) in [-24, 0], so that what is rounded to f16 is at most 2^14 (the maximum is raised when it has grown by 2^4, and then what has been summed is rescaled), and
-// what is lost below f16's least numbers is 2^-35 of the largest weight.  The sum of the weights takes the factor out again, once for 16 tokens.
+// A page's scale of K multiplies its columns' scores; its scale of V, over the largest of the pages that the CTA sees, goes into the exponent: weights are 2^(x - m + lv + 6) with
+// lv = log2(vs / VS) in [-24, 0], so that what is rounded to f16 is at most 2^14 (the maximum is raised when one of a warp's rows has grown by 2^8, and then what has been summed is
+// rescaled), and what is lost below f16's least numbers is 2^-31 of the largest weight.  The sum of the weights takes the factor out again, once for 16 tokens.
 //
 //   warps 0 .. 3, 4 .. 7  rows of the first and the second tile      8 .. 11  codes to f16      12  TMEM owner, MMA issuer
 #pragma once
@@ -64,7 +64,7 @@ struct KvPromptCfg {
     static constexpr int OFF_K = 2 * OPERAND, OFF_V = 4 * OPERAND, OFF_REST = 6 * OPERAND;
     static constexpr int LPR = DP / 16;               // lanes of a row of codes
     static constexpr int LOADS = DP / 16;             // 16-byte loads of a thread for 128 tokens
-    static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 10) of 16 tokens each, which of them there are
+    static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are
     // factors of rows, info of 4 steps, maxima of scales, barriers, address of TMEM, flag
     static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 16, OFF_TMEM = OFF_BAR + 16 * 8, SMEM = OFF_TMEM + 16;
 };
@@ -119,8 +119,8 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         const int t = steps.at(k, 128) + 16 * (lane & 7);
         return kv_seen16(t, low, high, a.window, a.sinks) ? (int)kv_page(c, tile.s, t >> pl) : -1;
     };
-    uint4 w[N];
-    auto load = [&](const int8_t* codes, int page, int k) {
+    uint4 wk[N], wv[N];
+    auto load = [&](uint4 (&w)[N], const int8_t* codes, int page, int k) {
         const int t = k < steps.total ? steps.at(k, 128) : 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -130,16 +130,17 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
             w[i] = in ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
         }
     };
-    auto convert = [&](uint8_t* to) {
+    auto convert = [&](const uint4 (&w)[N], uint8_t* to) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t r[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
             uint32_t f[8];
 #pragma unroll
             for (int z = 0; z < 4; ++z) { f[2 * z] = codes_f16(r[z]); f[2 * z + 1] = codes_f16(r[z] >> 8); }       // (numbers 0, 2, 1, 3 of each four)
-            const int row = i * TOKENS + token0, first = (mine >> 2) & 1;              // (the upper 64 dimensions the other way round: no bank twice)
-            *reinterpret_cast<uint4*>(to + place(row, first)) = make_uint4(f[4 * first], f[4 * first + 1], f[4 * first + 2], f[4 * first + 3]);
-            *reinterpret_cast<uint4*>(to + place(row, 1 - first)) = make_uint4(f[4 - 4 * first], f[5 - 4 * first], f[6 - 4 * first], f[7 - 4 * first]);
+            const int row = i * TOKENS + token0;
+            const bool upper = (mine >> 2) & 1;       // (the upper 64 dimensions the other way round: no bank twice)
+            *reinterpret_cast<uint4*>(to + place(row, upper)) = upper ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(to + place(row, !upper)) = upper ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
         }
     };
     auto done = [&](uint32_t b) {
@@ -147,8 +148,12 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(b);
     };
-    int page = page_of(0);
-    load(c.k, page, 0);
+    // everything is on its way a step ahead, the pages two
+    int page = page_of(0), page1 = page_of(1);
+    load(wk, c.k, page, 0);
+    load(wv, c.v, page, 0);
+    auto scale_of = [&](const float* scales, int p) { return warp == 0 && p >= 0 ? scales[(long long)p * c.heads + tile.h] : 0.0f; };
+    float ks = scale_of(c.k_scale, page), vsc = scale_of(c.v_scale, page);
 
     // the largest scale of V that any row sees
     float top = 0.0f;
@@ -206,27 +211,27 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
     for (int k = 0; k < steps.total; ++k) {
         const int s = k & 1;
         const uint32_t free_parity = ((uint32_t)(k >> 1) & 1u) ^ 1u;
+        const int page2 = page_of(k + 2);
+        const float next_ks = scale_of(c.k_scale, page1), next_vsc = scale_of(c.v_scale, page1);
         if (!kv_wait(a, bar.k_empty(s), free_parity, abort_flag)) return;
-        convert(smem + F::OFF_K + s * F::OPERAND);
+        convert(wk, smem + F::OFF_K + s * F::OPERAND);
         done(bar.k_full(s));
-        load(c.v, page, k);
-        if (warp == 0 && lane < 8) {
+        load(wk, c.k, page1, k + 1);
+        if (warp == 0) {
             float* i = info + (k & 3) * F::INFO;
-            const long long at = (long long)max(page, 0) * c.heads + tile.h;
-            const float ks = page >= 0 ? c.k_scale[at] : 0.0f, mine_v = page >= 0 ? c.v_scale[at] : 0.0f;
-            float lv = vs > 0.0f ? __log2f(fabsf(mine_v) / vs) : 0.0f;
+            float lv = vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f;
             lv = lv < -24.0f ? -24.0f : (lv > 0.0f ? 0.0f : lv);       // (NaN stays)
-            i[lane] = ks; i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 10.0f);
-            const unsigned there = __ballot_sync(0xffu, page >= 0);
-            if (lane == 0) reinterpret_cast<int*>(i)[24] = (int)there;
+            if (lane < 8) { i[lane] = ks; i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 6.0f); }
+            const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane == 0) reinterpret_cast<int*>(i)[24] = (int)(there & 255u);
+            __syncwarp();
         }
-        __syncwarp();
-        const int next = page_of(k + 1);
         if (!kv_wait(a, bar.v_empty(s), free_parity, abort_flag)) return;
-        convert(smem + F::OFF_V + s * F::OPERAND);
+        convert(wv, smem + F::OFF_V + s * F::OPERAND);
         done(bar.v_full(s));
-        page = next;
-        load(c.k, page, k + 1);
+        load(wv, c.v, page1, k + 1);
+        page = page1; page1 = page2;
+        ks = next_ks; vsc = next_vsc;
     }
 }
 
@@ -297,7 +302,7 @@ __device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* inf
     for (int g = 0; g < 8; ++g) {                     // 16 tokens, which are on one page
         tmem_wait_ld16(v[g & 1]);
         if (g < 7) ptx::tmem_ld16(ts + 16 * (g + 1), v[(g + 1) & 1]);
-        const float f = factor * info[g], lv = info[8 + g], b = lv + 10.0f - base;
+        const float f = factor * info[g], lv = info[8 + g], b = lv + 6.0f - base;
         const unsigned long long f2 = ptx::pack2(f, f), b2 = ptx::pack2(b, b);
         unsigned long long s2 = 0;
         float most = -INFINITY;
@@ -320,12 +325,12 @@ __device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* inf
         const float add = (s1.x + s1.y) * info[16 + g];
         sum += WHOLE || s1.x + s1.y != 0.0f ? add : 0.0f;              // (the factor of a page that the row does not see may be NaN)
     }
-    return top - 10.0f;
+    return top - 6.0f;
 }
 
 // ---- warps 0 .. 7, a row each thread
 //
-// The base of the exponents is the maximum of earlier steps: one pass over the scores gives weights and their maximum, and only where that has grown by 2^4 (a row's first step, and few
+// The base of the exponents is the maximum of earlier steps: one pass over the scores gives weights and their maximum, and only where that has grown by 2^8 (a row's first step, and few
 // others) it is taken again.  (A pass for the maximum in front: twice the time.)
 template <typename F>
 __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, uint32_t tmem, volatile int* abort_flag) {
@@ -354,10 +359,11 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
             const float base = m == -INFINITY ? 0.0f : m;
             const float top = whole ? kv_prompt_weights<true>(ts, info, factor, base, there, upto, behind, sunk, p, sum)
                                     : kv_prompt_weights<false>(ts, info, factor, base, there, upto, behind, sunk, p, sum);
-            const bool raise = m == -INFINITY ? top > -INFINITY : top > 4.0f;
+            const bool raise = m == -INFINITY ? top > -INFINITY : top > 8.0f;
             if (again || !__any_sync(0xffffffffu, raise)) break;
-            const float to_m = base + top, f = raise ? (m == -INFINITY ? 0.0f : ex2(m - to_m)) : 1.0f;
-            if (raise) { l *= f; m = to_m; }
+            const bool more = raise || top > 0.0f;    // (a row that has grown at all goes along)
+            const float to_m = base + top, f = more ? (m == -INFINITY ? 0.0f : ex2(m - to_m)) : 1.0f;
+            if (more) { l *= f; m = to_m; }
             if (count > 0) {
 #pragma unroll 1
                 for (int g = 0; g < DP / 16; ++g) {
@@ -387,7 +393,7 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     float vs = 0.0f;
     if (count > 0) vs = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
     const bool mine_there = mine < tile.rows;
-    const float out_scale = l == 0.0f ? 0.0f : vs * (1.0f / 1024.0f) / l;
+    const float out_scale = l == 0.0f ? 0.0f : vs * (1.0f / 64.0f) / l;
     const long long token = tile.row + row / a.group, head = tile.h * a.group + row % a.group, at = token * a.out_stride + head * c.dim;
 #pragma unroll
     for (int g = 0; g < DP / 16; ++g) {
