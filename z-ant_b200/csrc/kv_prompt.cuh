@@ -9,7 +9,8 @@
 // lv = log2(vs / VS) in [-24, 0], so that what is rounded to f16 is at most 2^14 (the maximum is raised when one of a warp's rows has grown by 2^8, and then what has been summed is
 // rescaled), and what is lost below f16's least numbers is 2^-31 of the largest weight.  The sum of the weights takes the factor out again, once for 16 tokens.
 //
-//   warps 0 .. 3, 4 .. 7  rows of the first and the second tile      8 .. 11  codes to f16      12  TMEM owner, MMA issuer
+//   warps 0 .. 3, 4 .. 7  rows of the first and the second tile      8 .. 11  q and K to f16      12  TMEM owner, MMA issuer      13 .. 15  V to f16, scales
+// Registers: 152 for the rows' threads, 104 for others (setmaxnreg; 128 each at launch).
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -40,31 +41,35 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) {
     return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-// One lane of a whole warp (`leader`): D (+)= A B with A in shared memory, or in tensor memory.
-__device__ __forceinline__ void mma_f16_ss_if(uint32_t leader, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%6, %6, %6, %6}, p;\n\t}\n"
-                 ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader), "r"(0u) : "memory");
+// One lane of a whole warp (`leader`): D (+)= A B with A in shared memory, or in tensor memory.  Operands in shared memory are rows of 128 bytes in the 128-byte swizzle, 8 rows
+// 1024 bytes: K index in the row (K-major), or N index in the row and the next 64 of them `block` bytes further.  Descriptors as halves: the upper one is the same for all.
+constexpr uint32_t kKvDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t kv_desc_lo(uint32_t addr, uint32_t block) { return (addr >> 4) | ((block >> 4) << 16); }
+__device__ __forceinline__ void mma_f16_ss_if(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.b64 da, {%1, %7};\n\tmov.b64 db, {%2, %7};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n\t}\n"
+                 ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(leader), "r"(0u), "r"(kKvDescHi) : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts_if(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%6, %6, %6, %6}, p;\n\t}\n"
-                 ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader), "r"(0u) : "memory");
+__device__ __forceinline__ void mma_f16_ts_if(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.b64 db, {%2, %7};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%6, %6, %6, %6}, p;\n\t}\n"
+                 ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(leader), "r"(0u), "r"(kKvDescHi) : "memory");
 }
-// Rows of 128 bytes in the 128-byte swizzle, 8 rows 1024 bytes: K index in the row (K-major); N index in the row, the next 64 of them `block` bytes further.
-__device__ __forceinline__ uint64_t kv_desc(uint32_t addr, uint32_t block) {
-    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)((block >> 4) & 0x3fffu) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+
+// A warpgroup's registers a thread; the shares of all warpgroups add up to what the CTA was launched with.
+template <int N> __device__ __forceinline__ void set_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void set_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int DP_>
 struct KvPromptCfg {
-    static constexpr int DP = DP_, TILE = 128, ROWS = 2 * TILE, STEP = 128, WARPS = 13, THREADS = 32 * WARPS;
+    static constexpr int DP = DP_, TILE = 128, ROWS = 2 * TILE, STEP = 128, WARPS = 16, THREADS = 32 * WARPS;
     static constexpr int BLOCK = TILE * 128;          // 128 rows of 64 f16 numbers
     static constexpr int OPERAND = BLOCK * (DP / 64); // Q of a tile, K or V of a step
     static constexpr int OFF_K = 2 * OPERAND, OFF_V = 4 * OPERAND, OFF_REST = 6 * OPERAND;
     static constexpr int LPR = DP / 16;               // lanes of a row of codes
-    static constexpr int LOADS = DP / 16;             // 16-byte loads of a thread for 128 tokens
-    static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are
+    static constexpr int TPL = 32 / LPR;              // tokens of a warp's load
+    static constexpr int ROWS_REGS = 152, OTHER_REGS = 104;       // 256 x 152 + 256 x 104 = 512 x 128
+    static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN
     // factors of rows, info of 4 steps, maxima of scales, barriers, address of TMEM, flag
     static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 16, OFF_TMEM = OFF_BAR + 16 * 8, SMEM = OFF_TMEM + 16;
 };
@@ -84,13 +89,16 @@ struct KvPromptBars {
 // What all roles know of the CTA's rows.
 struct KvPromptTile {
     int s, row, first, row0, rows, h;                 // sequence, its first row, position of its first new token, first of the CTA's rows, how many, key head
-    int low[2], high[2];                              // positions of either tile's first and last row (high < 0: the tile has none, or sees nothing)
+    int low0, low1, high0, high1;                     // positions of either tile's first and last row (high < 0: the tile has none, or sees nothing)
+    __device__ __forceinline__ int low(int x) const { return x ? low1 : low0; }
+    __device__ __forceinline__ int high(int x) const { return x ? high1 : high0; }
+    __device__ __forceinline__ int last() const { return max(high0, high1); }
     __device__ __forceinline__ bool active(int x, int t, int window, int sinks) const {
-        return t <= high[x] && (window == 0 || t + 127 > low[x] - window || t < sinks);
+        return t <= high(x) && (window == 0 || t + 127 > low(x) - window || t < sinks);
     }
     // every row sees all of the step
     __device__ __forceinline__ bool whole(int x, int t, int window, int sinks) const {
-        return t + 127 <= low[x] && (window == 0 || t > high[x] - window || t + 128 <= sinks);
+        return t + 127 <= low(x) && (window == 0 || t > high(x) - window || t + 128 <= sinks);
     }
 };
 
@@ -98,80 +106,66 @@ __device__ __forceinline__ bool kv_wait(const KvAttendArgs& a, uint32_t bar, uin
     return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag, a.wait_budget));
 }
 
-// ---- warps 8 .. 11
-template <typename F>
-__device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
-    constexpr int LPR = F::LPR, N = F::LOADS;
-    const KvArgs& c = a.c;
-    const int tid = threadIdx.x - 256, lane = tid & 31, warp = tid >> 5, pl = c.page_log2, inpage = c.page - 1;
-    float* row_factor = reinterpret_cast<float*>(smem + F::OFF_REST);
-    float* info = reinterpret_cast<float*>(smem + F::OFF_INFO);
-    float* part = reinterpret_cast<float*>(smem + F::OFF_MAX);
-    const int mine = tid % LPR, token0 = tid / LPR;   // the thread's 16 dimensions, and its token of each 128 / LPR
-    constexpr int TOKENS = 128 / LPR;                 // tokens of one load of all threads: 16 (32)
-    // the place of 16 f16 numbers, two chunks, in row r of an operand
-    auto place = [&](int r, int half) { return (mine >> 2) * F::BLOCK + r * 128 + ((((mine & 3) * 2 + half) ^ (r & 7)) << 4); };
-
-    // pages of 16 tokens each of a step: lane i (of 8) has the i-th
-    const int low = tile.low[0], high = max(tile.high[0], tile.high[1]);
-    auto page_of = [&](int k) {
-        if (k >= steps.total) return -1;
-        const int t = steps.at(k, 128) + 16 * (lane & 7);
-        return kv_seen16(t, low, high, a.window, a.sinks) ? (int)kv_page(c, tile.s, t >> pl) : -1;
-    };
-    uint4 wk[N], wv[N];
-    auto load = [&](uint4 (&w)[N], const int8_t* codes, int page, int k) {
-        const int t = k < steps.total ? steps.at(k, 128) : 0;
+// Codes on their way to f16 operands: warp `warp` of WARPS that do it takes every so many'th TPL tokens of a step's 128.
+template <typename F, int WARPS>
+struct KvConvert {
+    static constexpr int LPR = F::LPR, GROUPS = 128 / F::TPL, N = (GROUPS + WARPS - 1) / WARPS;
+    uint4 w[N];
+    int lane, warp, mine, in_group;                   // mine: the lane's 16 dimensions of its token
+    __device__ __forceinline__ KvConvert(int lane_, int warp_) : lane(lane_), warp(warp_), mine(lane_ % LPR), in_group(lane_ / LPR) {}
+    __device__ __forceinline__ int token(int i) const { return (i * WARPS + warp) * F::TPL + in_group; }
+    // page: of 16 tokens each, in lanes 0 .. 7; t: the step's first token
+    __device__ __forceinline__ void load(const KvArgs& c, const int8_t* codes, int h, int page, int t) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int token = i * TOKENS + token0, id = __shfl_sync(0xffffffffu, page, token >> 4);
-            const bool in = id >= 0 && mine * 16 < c.dim;
-            const int8_t* p = codes + (((long long)(in ? id : 0) * c.heads + tile.h) * c.page + ((t + token) & inpage)) * c.dim + mine * 16;
+            const int tok = token(i), id = __shfl_sync(0xffffffffu, page, (tok >> 4) & 7);
+            const bool in = id >= 0 && mine * 16 < c.dim && (GROUPS % WARPS == 0 || tok < 128);
+            const int8_t* p = codes + (((long long)(in ? id : 0) * c.heads + h) * c.page + (in ? (t + tok) & (c.page - 1) : 0)) * c.dim + (in ? mine * 16 : 0);
             w[i] = in ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
         }
-    };
-    auto convert = [&](const uint4 (&w)[N], uint8_t* to) {
+    }
+    // the place of 8 f16 numbers of the lane's 16 in row r of an operand
+    static __device__ __forceinline__ int place(int mine, int r, int half) { return (mine >> 2) * F::BLOCK + r * 128 + ((((mine & 3) * 2 + half) ^ (r & 7)) << 4); }
+    __device__ __forceinline__ void store(uint8_t* to) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            if (GROUPS % WARPS != 0 && i == N - 1 && token(i) >= 128) continue;        // (whole warps)
             const uint32_t r[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
             uint32_t f[8];
 #pragma unroll
             for (int z = 0; z < 4; ++z) { f[2 * z] = codes_f16(r[z]); f[2 * z + 1] = codes_f16(r[z] >> 8); }       // (numbers 0, 2, 1, 3 of each four)
-            const int row = i * TOKENS + token0;
             const bool upper = (mine >> 2) & 1;       // (the upper 64 dimensions the other way round: no bank twice)
-            *reinterpret_cast<uint4*>(to + place(row, upper)) = upper ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<uint4*>(to + place(row, !upper)) = upper ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
-        }
-    };
-    auto done = [&](uint32_t b) {
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(b);
-    };
-    // everything is on its way a step ahead, the pages two
-    int page = page_of(0), page1 = page_of(1);
-    load(wk, c.k, page, 0);
-    load(wv, c.v, page, 0);
-    auto scale_of = [&](const float* scales, int p) { return warp == 0 && p >= 0 ? scales[(long long)p * c.heads + tile.h] : 0.0f; };
-    float ks = scale_of(c.k_scale, page), vsc = scale_of(c.v_scale, page);
-
-    // the largest scale of V that any row sees
-    float top = 0.0f;
-    if (steps.total > 0) {
-        const int from = a.window > 0 ? max(low - a.window + 1, 0) >> pl : 0, to = (high >> pl) + 1;
-        const int sink_pages = a.sinks > 0 ? min(((a.sinks - 1) >> pl) + 1, from) : 0;
-#pragma unroll 4
-        for (int i = tid; i < sink_pages + to - from; i += 128) {
-            const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
-            if (id >= 0) top = fmaxf(top, fabsf(c.v_scale[id * c.heads + tile.h]));
+            *reinterpret_cast<uint4*>(to + place(mine, token(i), upper)) = upper ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(to + place(mine, token(i), !upper)) = upper ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
         }
     }
-    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-    if (lane == 0) part[warp] = top;
+};
+__device__ __forceinline__ void kv_written(uint32_t bar) {
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
+}
+// Pages of 16 tokens each of step k: lane i (of 8) has the i-th.
+__device__ __forceinline__ int kv_prompt_page(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, int k) {
+    if (k >= steps.total) return -1;
+    const int t = steps.at(k, 128) + 16 * (threadIdx.x & 7);
+    return kv_seen16(t, tile.low0, tile.last(), a.window, a.sinks) ? (int)kv_page(a.c, tile.s, t >> a.c.page_log2) : -1;
+}
 
-    // q
-    constexpr int RPP = 4 * (32 / LPR);               // rows that four warps take at once
-#pragma unroll 2
+// ---- warps 8 .. 11: q, then K.  Codes are on their way a step ahead, pages two.
+template <typename F>
+__device__ __forceinline__ void kv_prompt_keys(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
+    constexpr int LPR = F::LPR;
+    const KvArgs& c = a.c;
+    const int tid = threadIdx.x - 256, lane = tid & 31;
+    float* row_factor = reinterpret_cast<float*>(smem + F::OFF_REST);
+    KvConvert<F, 4> codes(lane, tid >> 5);
+    const int mine = codes.mine;
+    int page1 = kv_prompt_page(a, tile, steps, 1);
+    codes.load(c, c.k, tile.h, kv_prompt_page(a, tile, steps, 0), steps.total > 0 ? steps.at(0, 128) : 0);
+
+    constexpr int RPP = 4 * F::TPL;                   // rows that four warps take at once
+#pragma unroll 1
     for (int r0 = 0; r0 < F::ROWS; r0 += RPP) {
         const int r = r0 + tid / LPR, row = tile.row0 + r;
         const bool there = r < tile.rows && mine * 16 < c.dim;
@@ -189,8 +183,8 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         for (int d = LPR / 2; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
         odd = (__ballot_sync(0xffffffffu, odd) >> (lane / LPR * LPR)) & ((1u << LPR) - 1u);
         const int e = min(max((int)(__float_as_uint(big) >> 23) - 127 - 14, -114), 127);
-        const float down = odd ? 0.0f : __uint_as_float((uint32_t)(127 - e) << 23), up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(127 + e, 1) << 23);
-        if (mine == 0) row_factor[r] = up * a.scale_log2;
+        const float down = odd ? 0.0f : copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2), up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(127 + e, 1) << 23);
+        if (mine == 0) row_factor[r] = up * fabsf(a.scale_log2);
         uint32_t f[8];
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
@@ -201,35 +195,65 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
             f[2 * z + 1] = pack_f16(x[1], x[3]);
         }
         uint8_t* to = smem + (r >> 7) * F::OPERAND;
-        *reinterpret_cast<uint4*>(to + place(r & 127, 0)) = make_uint4(f[0], f[1], f[2], f[3]);
-        *reinterpret_cast<uint4*>(to + place(r & 127, 1)) = make_uint4(f[4], f[5], f[6], f[7]);
+        *reinterpret_cast<uint4*>(to + codes.place(mine, r & 127, 0)) = make_uint4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<uint4*>(to + codes.place(mine, r & 127, 1)) = make_uint4(f[4], f[5], f[6], f[7]);
     }
-    done(bar.q_full());
-    ptx::named_barrier_sync(1, 128);                  // (in front of any wait that may be given up)
-    const float vs = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    kv_written(bar.q_full());
 
     for (int k = 0; k < steps.total; ++k) {
-        const int s = k & 1;
-        const uint32_t free_parity = ((uint32_t)(k >> 1) & 1u) ^ 1u;
-        const int page2 = page_of(k + 2);
+        const int page2 = kv_prompt_page(a, tile, steps, k + 2);
+        if (!kv_wait(a, bar.k_empty(k & 1), ((uint32_t)(k >> 1) & 1u) ^ 1u, abort_flag)) return;
+        codes.store(smem + F::OFF_K + (k & 1) * F::OPERAND);
+        kv_written(bar.k_full(k & 1));
+        codes.load(c, c.k, tile.h, page1, k + 1 < steps.total ? steps.at(k + 1, 128) : 0);
+        page1 = page2;
+    }
+}
+
+// ---- warps 13 .. 15: the largest scale of V, then V and what each step's pages say
+template <typename F>
+__device__ __forceinline__ void kv_prompt_values(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
+    const KvArgs& c = a.c;
+    const int tid = threadIdx.x - 13 * 32, lane = tid & 31, warp = tid >> 5, pl = c.page_log2;
+    float* info = reinterpret_cast<float*>(smem + F::OFF_INFO);
+    float* part = reinterpret_cast<float*>(smem + F::OFF_MAX);
+    const int low = tile.low0, high = tile.last();
+    KvConvert<F, 3> codes(lane, warp);
+    int page = kv_prompt_page(a, tile, steps, 0), page1 = kv_prompt_page(a, tile, steps, 1);
+    codes.load(c, c.v, tile.h, page, steps.total > 0 ? steps.at(0, 128) : 0);
+    auto scale_of = [&](const float* scales, int p) { return warp == 0 && p >= 0 ? scales[(long long)p * c.heads + tile.h] : 0.0f; };
+    float ks = scale_of(c.k_scale, page), vsc = scale_of(c.v_scale, page);
+    float top = 0.0f;
+    if (steps.total > 0) {
+        const int from = a.window > 0 ? max(low - a.window + 1, 0) >> pl : 0, to = (high >> pl) + 1;
+        const int sink_pages = a.sinks > 0 ? min(((a.sinks - 1) >> pl) + 1, from) : 0;
+#pragma unroll 4
+        for (int i = tid; i < sink_pages + to - from; i += 96) {
+            const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
+            if (id >= 0) top = fmaxf(top, fabsf(c.v_scale[id * c.heads + tile.h]));
+        }
+    }
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if (lane == 0) part[warp] = top;
+    ptx::named_barrier_sync(1, 96);                   // (in front of any wait that may be given up)
+    const float vs = fmaxf(fmaxf(part[0], part[1]), part[2]);
+
+    for (int k = 0; k < steps.total; ++k) {
+        const int page2 = kv_prompt_page(a, tile, steps, k + 2);
         const float next_ks = scale_of(c.k_scale, page1), next_vsc = scale_of(c.v_scale, page1);
-        if (!kv_wait(a, bar.k_empty(s), free_parity, abort_flag)) return;
-        convert(wk, smem + F::OFF_K + s * F::OPERAND);
-        done(bar.k_full(s));
-        load(wk, c.k, page1, k + 1);
+        if (!kv_wait(a, bar.v_empty(k & 1), ((uint32_t)(k >> 1) & 1u) ^ 1u, abort_flag)) return;
         if (warp == 0) {
             float* i = info + (k & 3) * F::INFO;
-            float lv = vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f;
-            lv = lv < -24.0f ? -24.0f : (lv > 0.0f ? 0.0f : lv);       // (NaN stays)
-            if (lane < 8) { i[lane] = ks; i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 6.0f); }
-            const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
-            if (lane == 0) reinterpret_cast<int*>(i)[24] = (int)(there & 255u);
+            const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
+            const bool k_nan = ks != ks, v_nan = vsc != vsc;
+            if (lane < 8) { i[lane] = k_nan ? 0.0f : fabsf(ks); i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 6.0f); }
+            const unsigned there = __ballot_sync(0xffffffffu, page >= 0), bad_k = __ballot_sync(0xffffffffu, k_nan), bad_v = __ballot_sync(0xffffffffu, v_nan);
+            if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8)); }
             __syncwarp();
         }
-        if (!kv_wait(a, bar.v_empty(s), free_parity, abort_flag)) return;
-        convert(wv, smem + F::OFF_V + s * F::OPERAND);
-        done(bar.v_full(s));
-        load(wv, c.v, page1, k + 1);
+        codes.store(smem + F::OFF_V + (k & 1) * F::OPERAND);
+        kv_written(bar.v_full(k & 1));
+        codes.load(c, c.v, tile.h, page1, k + 1 < steps.total ? steps.at(k + 1, 128) : 0);
         page = page1; page1 = page2;
         ks = next_ks; vsc = next_vsc;
     }
@@ -244,20 +268,22 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
     int count[2] = {0, 0};                            // products P V so far
     int last[2] = {-1, -1};                           // a tile's last step
     for (int k = 0; k < steps.total; ++k)
+#pragma unroll
         for (int x = 0; x < 2; ++x)
             if (tile.active(x, steps.at(k, 128), a.window, a.sinks)) last[x] = k;
     auto scores = [&](int x, int k) {
+        const uint32_t qa = kv_desc_lo(s0 + x * F::OPERAND, 16), kb = kv_desc_lo(s0 + F::OFF_K + (k & 1) * F::OPERAND, 16);
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            const uint32_t at = (i >> 2) * F::BLOCK + (i & 3) * 32;
-            mma_f16_ss_if(leader, tmem + x * 128, kv_desc(s0 + x * F::OPERAND + at, 16), kv_desc(s0 + F::OFF_K + (k & 1) * F::OPERAND + at, 16), idesc_s, i > 0);
+            const uint32_t at = ((i >> 2) * F::BLOCK + (i & 3) * 32) >> 4;
+            mma_f16_ss_if(leader, tmem + x * 128, qa + at, kb + at, idesc_s, i > 0);
         }
         ptx::mma_commit_if(leader, bar.s_full(x));
     };
     auto values = [&](int x, int k) {
+        const uint32_t vb = kv_desc_lo(s0 + F::OFF_V + (k & 1) * F::OPERAND, F::BLOCK);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            mma_f16_ts_if(leader, tmem + 256 + x * DP, tmem + x * 128 + i * 8, kv_desc(s0 + F::OFF_V + (k & 1) * F::OPERAND + i * 2048, F::BLOCK), idesc_o, (count[x] | i) != 0);
+        for (int i = 0; i < 8; ++i) mma_f16_ts_if(leader, tmem + 256 + x * DP, tmem + x * 128 + i * 8, vb + i * (2048 >> 4), idesc_o, (count[x] | i) != 0);
         ++count[x];
         if (k == last[x]) ptx::mma_commit_if(leader, bar.o_full(x));
     };
@@ -265,6 +291,7 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
     if (steps.total > 0) {
         if (!kv_wait(a, bar.q_full(), 0, abort_flag) || !kv_wait(a, bar.k_full(0), 0, abort_flag)) return;
         ptx::tc_fence_after();
+#pragma unroll
         for (int x = 0; x < 2; ++x) if (active(x, 0)) scores(x, 0);
         ptx::mma_commit_if(leader, bar.k_empty(0));
     }
@@ -272,6 +299,7 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
         const uint32_t parity = (uint32_t)(k >> 1) & 1u, next_parity = (uint32_t)((k + 1) >> 1) & 1u;
         if (!kv_wait(a, bar.v_full(k & 1), parity, abort_flag)) return;
         bool k_there = false;
+#pragma unroll
         for (int x = 0; x < 2; ++x) {
             if (active(x, k)) {
                 if (!kv_wait(a, bar.p_full(x), (uint32_t)count[x] & 1u, abort_flag)) return;
@@ -290,10 +318,9 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
     }
 }
 
-// Weights of a row's 128 scores in tensor memory at `ts`, in pairs, under the base `base` (log2): p, their sum with each page's factor taken out, and the largest exponent.
-// WHOLE: the row sees all of them; else columns up to `upto`, and behind `behind` or in front of `sunk`, on pages that are there.
-template <bool WHOLE>
-__device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* info, float factor, float base, int there, int upto, int behind, int sunk, uint32_t (&p)[64], float& sum) {
+// Weights of a row's 128 scores in tensor memory at `ts` (minus infinity: not seen), in pairs, under the base `base` (log2): p, their sum with each page's factor taken out, and
+// the largest exponent.
+__device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* info, float factor, float base, uint32_t (&p)[64], float& sum) {
     uint32_t v[2][16];
     float top = -INFINITY;
     sum = 0.0f;
@@ -302,19 +329,15 @@ __device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* inf
     for (int g = 0; g < 8; ++g) {                     // 16 tokens, which are on one page
         tmem_wait_ld16(v[g & 1]);
         if (g < 7) ptx::tmem_ld16(ts + 16 * (g + 1), v[(g + 1) & 1]);
-        const float f = factor * info[g], lv = info[8 + g], b = lv + 6.0f - base;
+        float f = factor * info[g];
+        f = f == 0.0f ? 1e-38f : f;                   // (minus infinity stays what it is)
+        const float lv = info[8 + g], b = lv + 6.0f - base;
         const unsigned long long f2 = ptx::pack2(f, f), b2 = ptx::pack2(b, b);
         unsigned long long s2 = 0;
         float most = -INFINITY;
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
-            float2 e = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(v[g & 1][2 * y]), __uint_as_float(v[g & 1][2 * y + 1])), f2, b2));
-            if (!WHOLE) {
-                const int at = 16 * g + 2 * y;
-                const bool on = (there >> g) & 1;
-                if (!(on && at <= upto && (at > behind || at < sunk))) e.x = -INFINITY;
-                if (!(on && at + 1 <= upto && (at + 1 > behind || at + 1 < sunk))) e.y = -INFINITY;
-            }
+            const float2 e = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(v[g & 1][2 * y]), __uint_as_float(v[g & 1][2 * y + 1])), f2, b2));
             most = fmaxf(most, fmaxf(e.x, e.y));
             const float2 w = make_float2(ex2(e.x), ex2(e.y));
             s2 = ptx::add2(s2, ptx::pack2(w.x, w.y));
@@ -322,16 +345,19 @@ __device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* inf
         }
         top = fmaxf(top, most - lv);
         const float2 s1 = ptx::unpack2(s2);
-        const float add = (s1.x + s1.y) * info[16 + g];
-        sum += WHOLE || s1.x + s1.y != 0.0f ? add : 0.0f;              // (the factor of a page that the row does not see may be NaN)
+        sum = fmaf(s1.x + s1.y, info[16 + g], sum);
     }
     return top - 6.0f;
 }
+// The first n of 32 columns.
+__device__ __forceinline__ uint32_t first_columns(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
 // ---- warps 0 .. 7, a row each thread
 //
 // The base of the exponents is the maximum of earlier steps: one pass over the scores gives weights and their maximum, and only where that has grown by 2^8 (a row's first step, and few
-// others) it is taken again.  (A pass for the maximum in front: twice the time.)
+// others) it is taken again.  (A pass for the maximum in front: twice the time.)  Steps that a row sees in part have minus infinity written over the other scores first, so that there is one
+// form of the pass, which is what the instruction cache has to hold (with a second form for such steps beside it: 7000 clocks a step where this one takes 3300).  Pages with a scale of NaN count as
+// zeros; the rows that see them are noted and get their NaN at the end.
 template <typename F>
 __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, uint32_t tmem, volatile int* abort_flag) {
     constexpr int DP = F::DP;
@@ -341,24 +367,43 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     const float* all_info = reinterpret_cast<const float*>(smem + F::OFF_INFO);
     const int row = tile.row0 + min(mine, tile.rows - 1), pos = max(tile.first + row / a.group, -1);
     float factor = 0.0f, m = -INFINITY, l = 0.0f;
-    int count = 0;
+    int count = 0, spoilt = 0;                        // spoilt: 1 by a page's scale of K, 2 of V
     for (int k = 0; k < steps.total; ++k) {
         const int t = steps.at(k, 128);
         if (!tile.active(x, t, a.window, a.sinks)) continue;
         if (!kv_wait(a, bar.v_full(k & 1), (uint32_t)(k >> 1) & 1u, abort_flag)) return;       // what the step's pages say
         if (!kv_wait(a, bar.s_full(x), (uint32_t)count & 1u, abort_flag)) return;
         ptx::tc_fence_after();
-        if (count == 0) factor = reinterpret_cast<const float*>(smem + F::OFF_REST)[mine];
+        if (count == 0) {
+            if (!kv_wait(a, bar.q_full(), 0, abort_flag)) return;
+            factor = reinterpret_cast<const float*>(smem + F::OFF_REST)[mine];
+        }
         const float* info = all_info + (k & 3) * F::INFO;
-        const int there = reinterpret_cast<const int*>(info)[24];
-        const bool whole = there == 255 && tile.whole(x, t, a.window, a.sinks);
-        const int upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
+        const int there = reinterpret_cast<const int*>(info)[24], nan = reinterpret_cast<const int*>(info)[25];
+        if (there != 255 || nan != 0 || !tile.whole(x, t, a.window, a.sinks)) {
+            const int upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
+#pragma unroll 1
+            for (int g = 0; g < 4; ++g) {
+                uint32_t seen = first_columns(upto + 1 - 32 * g) & (~first_columns(behind + 1 - 32 * g) | first_columns(sunk - 32 * g));
+                seen &= ((there >> (2 * g)) & 1 ? 0xffffu : 0u) | ((there >> (2 * g + 1)) & 1 ? 0xffff0000u : 0u);
+                if (((seen & 0xffffu) && ((nan >> (2 * g)) & 1)) || ((seen >> 16) && ((nan >> (2 * g + 1)) & 1))) spoilt |= 1;
+                if (((seen & 0xffffu) && ((nan >> (2 * g + 8)) & 1)) || ((seen >> 16) && ((nan >> (2 * g + 9)) & 1))) spoilt |= 2;
+                if (__all_sync(0xffffffffu, seen == 0xffffffffu)) continue;
+                uint32_t v[32];
+                ptx::tmem_ld32(ts + 32 * g, v);
+                ptx::tmem_wait_ld32(v);
+#pragma unroll
+                for (int y = 0; y < 32; ++y) v[y] = (seen >> y) & 1u ? v[y] : 0xff800000u;
+                tmem_st16(ts + 32 * g, v);
+                tmem_st16(ts + 32 * g + 16, v + 16);
+            }
+            tmem_wait_st();
+        }
         uint32_t p[64];
         float sum;
+#pragma unroll 1
         for (int again = 0; again < 2; ++again) {
-            const float base = m == -INFINITY ? 0.0f : m;
-            const float top = whole ? kv_prompt_weights<true>(ts, info, factor, base, there, upto, behind, sunk, p, sum)
-                                    : kv_prompt_weights<false>(ts, info, factor, base, there, upto, behind, sunk, p, sum);
+            const float base = m == -INFINITY ? 0.0f : m, top = kv_prompt_weights(ts, info, factor, base, p, sum);
             const bool raise = m == -INFINITY ? top > -INFINITY : top > 8.0f;
             if (again || !__any_sync(0xffffffffu, raise)) break;
             const bool more = raise || top > 0.0f;    // (a row that has grown at all goes along)
@@ -391,9 +436,10 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     }
     const float* part = reinterpret_cast<const float*>(smem + F::OFF_MAX);
     float vs = 0.0f;
-    if (count > 0) vs = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    if (count > 0) vs = fmaxf(fmaxf(part[0], part[1]), part[2]);
     const bool mine_there = mine < tile.rows;
-    const float out_scale = l == 0.0f ? 0.0f : vs * (1.0f / 64.0f) / l;
+    if (spoilt & 1) l = __uint_as_float(0x7fffffffu);
+    const float out_scale = spoilt ? __uint_as_float(0x7fffffffu) : (l == 0.0f ? 0.0f : vs * (1.0f / 64.0f) / l);
     const long long token = tile.row + row / a.group, head = tile.h * a.group + row % a.group, at = token * a.out_stride + head * c.dim;
 #pragma unroll
     for (int g = 0; g < DP / 16; ++g) {
@@ -441,7 +487,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + F::OFF_TMEM + 8);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(bar.k_full(i), 4); ptx::mbar_init(bar.v_full(i), 4);
+            ptx::mbar_init(bar.k_full(i), 4); ptx::mbar_init(bar.v_full(i), 3);
             ptx::mbar_init(bar.k_empty(i), 1); ptx::mbar_init(bar.v_empty(i), 1);
             ptx::mbar_init(bar.s_full(i), 1); ptx::mbar_init(bar.p_full(i), 4); ptx::mbar_init(bar.o_full(i), 1);
         }
@@ -469,21 +515,28 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
     tile.rows = any && q.n * a.group > a.more_rows_than ? min(F::ROWS, q.n * a.group - tile.row0) : 0;
     if (tile.rows > 0) {                              // (the same for the whole CTA)
         tile.s = q.s; tile.row = q.row; tile.first = q.first;
-        for (int x = 0; x < 2; ++x) {
-            const int b = tile.row0 + x * 128, e = tile.row0 + min(tile.rows, (x + 1) * 128) - 1;
-            tile.low[x] = max(q.first + b / a.group, -1);
-            tile.high[x] = e < b ? -1 : max(q.first + e / a.group, -1);
-        }
-        const KvSteps steps(tile.low[0], max(tile.high[0], tile.high[1]), a.window, a.sinks, 128);
-        if (warp < 8) kv_prompt_rows<F>(a, tile, steps, bar, smem, tmem, abort_flag);
-        else if (warp < 12) kv_prompt_convert<F>(a, tile, steps, bar, smem, abort_flag);
-        else {
-            kv_prompt_mma<F>(a, tile, steps, bar, s0, tmem, abort_flag);
-            // what the tensor core still does ends before its operands' memory is another kernel's, also where a wait was given up
-            const uint32_t leader = ptx::elect_one() ? 1u : 0u;
-            ptx::mma_commit_if(leader, bar.drained());
-            volatile int no = 0;
-            ptx::mbar_wait(bar.drained(), 0, &no);
+        tile.low0 = max(q.first + tile.row0 / a.group, -1);
+        tile.high0 = max(q.first + (tile.row0 + min(tile.rows, 128) - 1) / a.group, -1);
+        tile.low1 = max(q.first + (tile.row0 + 128) / a.group, -1);
+        tile.high1 = tile.rows <= 128 ? -1 : max(q.first + (tile.row0 + tile.rows - 1) / a.group, -1);
+        const KvSteps steps(tile.low0, tile.last(), a.window, a.sinks, 128);
+        if (warp < 8) {
+            set_registers_up<F::ROWS_REGS>();
+            kv_prompt_rows<F>(a, tile, steps, bar, smem, tmem, abort_flag);
+        } else if (warp < 12) {
+            set_registers_down<F::OTHER_REGS>();
+            kv_prompt_keys<F>(a, tile, steps, bar, smem, abort_flag);
+        } else {
+            set_registers_down<F::OTHER_REGS>();
+            if (warp > 12) kv_prompt_values<F>(a, tile, steps, bar, smem, abort_flag);
+            else {
+                kv_prompt_mma<F>(a, tile, steps, bar, s0, tmem, abort_flag);
+                // what the tensor core still does ends before its operands' memory is another kernel's, also where a wait was given up
+                const uint32_t leader = ptx::elect_one() ? 1u : 0u;
+                ptx::mma_commit_if(leader, bar.drained());
+                volatile int no = 0;
+                ptx::mbar_wait(bar.drained(), 0, &no);
+            }
         }
     }
     __syncwarp();
