@@ -9,7 +9,7 @@
 // lv = log2(vs / VS) in [-24, 0], so that what is rounded to f16 is at most 2^14 (the maximum is raised when one of a warp's rows has grown by 2^8, and then what has been summed is
 // rescaled), and what is lost below f16's least numbers is 2^-31 of the largest weight.  The sum of the weights takes the factor out again, once for 16 tokens.
 //
-//   warps 0 .. 3, 4 .. 7  rows of the first and the second tile      8 .. 11  q and K to f16      12  TMEM owner, MMA issuer      13 .. 15  V to f16, scales
+//   warps 0 .. 3, 4 .. 7  rows of the first and the second tile      12  TMEM owner, MMA issuer      8 .. 11, 13 .. 15  q and codes to f16, scales
 // Registers: 152 for the rows' threads, 104 for others (setmaxnreg; 128 each at launch).
 #pragma once
 #include <cuda_fp16.h>
@@ -71,7 +71,7 @@ struct KvPromptCfg {
     static constexpr int ROWS_REGS = 152, OTHER_REGS = 104;       // 256 x 152 + 256 x 104 = 512 x 128
     static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN
     // factors of rows, info of 4 steps, maxima of scales, barriers, address of TMEM, flag
-    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 16, OFF_TMEM = OFF_BAR + 16 * 8, SMEM = OFF_TMEM + 16;
+    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 16 * 8, SMEM = OFF_TMEM + 16;
 };
 struct KvPromptBars {
     uint32_t at;
@@ -102,41 +102,49 @@ struct KvPromptTile {
     }
 };
 
+// The largest of the seven warps' numbers.
+__device__ __forceinline__ float kv_prompt_top(const float* part) {
+    float v = part[0];
+#pragma unroll
+    for (int i = 1; i < 7; ++i) v = fmaxf(v, part[i]);
+    return v;
+}
+
 __device__ __forceinline__ bool kv_wait(const KvAttendArgs& a, uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag, a.wait_budget));
 }
 
-// Codes on their way to f16 operands: warp `warp` of WARPS that do it takes every so many'th TPL tokens of a step's 128.
-template <typename F, int WARPS>
+// Codes on their way to f16 operands: warp `warp` of the seven takes every seventh TPL tokens of a step's 128.
+template <typename F>
 struct KvConvert {
-    static constexpr int LPR = F::LPR, GROUPS = 128 / F::TPL, N = (GROUPS + WARPS - 1) / WARPS;
+    static constexpr int WARPS = 7, LPR = F::LPR, GROUPS = 128 / F::TPL, N = (GROUPS + WARPS - 1) / WARPS;
     uint4 w[N];
-    int lane, warp, mine, in_group;                   // mine: the lane's 16 dimensions of its token
-    __device__ __forceinline__ KvConvert(int lane_, int warp_) : lane(lane_), warp(warp_), mine(lane_ % LPR), in_group(lane_ / LPR) {}
-    __device__ __forceinline__ int token(int i) const { return (i * WARPS + warp) * F::TPL + in_group; }
-    // page: of 16 tokens each, in lanes 0 .. 7; t: the step's first token
-    __device__ __forceinline__ void load(const KvArgs& c, const int8_t* codes, int h, int page, int t) {
+    // blocks: where 16 tokens each lie in the cache, in units of 16 tokens, in lanes 0 .. 7 (-1: nowhere); at: the lane's place in the 16 tokens of even (and, where a load has 8
+    // tokens, of any) groups, in bytes; mine: there are such dimensions
+    __device__ __forceinline__ void load(const int8_t* codes, int blocks, int warp, int dim, int in_group, int column, bool mine) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int tok = token(i), id = __shfl_sync(0xffffffffu, page, (tok >> 4) & 7);
-            const bool in = id >= 0 && mine * 16 < c.dim && (GROUPS % WARPS == 0 || tok < 128);
-            const int8_t* p = codes + (((long long)(in ? id : 0) * c.heads + h) * c.page + (in ? (t + tok) & (c.page - 1) : 0)) * c.dim + (in ? mine * 16 : 0);
-            w[i] = in ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+            const int group = i * WARPS + warp, tok = group * F::TPL;
+            const int block = __shfl_sync(0xffffffffu, blocks, (tok >> 4) & 7);
+            const bool in = mine && block >= 0 && (GROUPS % WARPS == 0 || group < GROUPS);
+            const int8_t* p = codes + (unsigned long long)(unsigned)block * (unsigned)(16 * dim) + (unsigned)(((tok & 15) + in_group) * dim + column);
+            w[i] = make_uint4(0, 0, 0, 0);
+            if (in) w[i] = *reinterpret_cast<const uint4*>(p);
         }
     }
-    // the place of 8 f16 numbers of the lane's 16 in row r of an operand
-    static __device__ __forceinline__ int place(int mine, int r, int half) { return (mine >> 2) * F::BLOCK + r * 128 + ((((mine & 3) * 2 + half) ^ (r & 7)) << 4); }
-    __device__ __forceinline__ void store(uint8_t* to) const {
+    // to: the operand, and the lane's place in row in_group of it
+    __device__ __forceinline__ void store(uint8_t* to, int warp, int in_group, int chunk) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (GROUPS % WARPS != 0 && i == N - 1 && token(i) >= 128) continue;        // (whole warps)
+            const int group = i * WARPS + warp, row = group * F::TPL + in_group;
+            if (GROUPS % WARPS != 0 && group >= GROUPS) continue;      // (whole warps)
             const uint32_t r[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
             uint32_t f[8];
 #pragma unroll
             for (int z = 0; z < 4; ++z) { f[2 * z] = codes_f16(r[z]); f[2 * z + 1] = codes_f16(r[z] >> 8); }       // (numbers 0, 2, 1, 3 of each four)
-            const bool upper = (mine >> 2) & 1;       // (the upper 64 dimensions the other way round: no bank twice)
-            *reinterpret_cast<uint4*>(to + place(mine, token(i), upper)) = upper ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<uint4*>(to + place(mine, token(i), !upper)) = upper ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
+            uint8_t* at = to + row * 128;
+            *reinterpret_cast<uint4*>(at + ((chunk ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(at + (((chunk + 1) ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
         }
     }
 };
@@ -151,26 +159,53 @@ __device__ __forceinline__ int kv_prompt_page(const KvAttendArgs& a, const KvPro
     const int t = steps.at(k, 128) + 16 * (threadIdx.x & 7);
     return kv_seen16(t, tile.low0, tile.last(), a.window, a.sinks) ? (int)kv_page(a.c, tile.s, t >> a.c.page_log2) : -1;
 }
+// Where these 16 tokens lie in the cache, in units of 16 tokens (below 2^31: 16 tokens are 256 bytes at least).
+__device__ __forceinline__ int kv_prompt_block(const KvArgs& c, const KvPromptTile& tile, const KvSteps& steps, int k, int page) {
+    if (page < 0) return -1;
+    const int t = steps.at(k, 128) + 16 * (threadIdx.x & 7);
+    return (int)((((unsigned)page * (unsigned)c.heads + (unsigned)tile.h) << (c.page_log2 - 4)) + (unsigned)((t & (c.page - 1)) >> 4));
+}
 
-// ---- warps 8 .. 11: q, then K.  Codes are on their way a step ahead, pages two.
+// ---- warps 8 .. 11 and 13 .. 15: the largest scale of V; q; K, V and what each step's pages say.  Codes are on their way a step ahead, pages two.
 template <typename F>
-__device__ __forceinline__ void kv_prompt_keys(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
-    constexpr int LPR = F::LPR;
+__device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
+    constexpr int LPR = F::LPR, TPL = F::TPL;
     const KvArgs& c = a.c;
-    const int tid = threadIdx.x - 256, lane = tid & 31;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - ((threadIdx.x >> 5) < 12 ? 8 : 9), pl = c.page_log2;
     float* row_factor = reinterpret_cast<float*>(smem + F::OFF_REST);
-    KvConvert<F, 4> codes(lane, tid >> 5);
-    const int mine = codes.mine;
-    int page1 = kv_prompt_page(a, tile, steps, 1);
-    codes.load(c, c.k, tile.h, kv_prompt_page(a, tile, steps, 0), steps.total > 0 ? steps.at(0, 128) : 0);
+    float* info = reinterpret_cast<float*>(smem + F::OFF_INFO);
+    float* part = reinterpret_cast<float*>(smem + F::OFF_MAX);
+    // the lane's 16 dimensions of a token: their place in its row of codes, and in an operand's
+    const int which = lane % LPR, in_group = lane / LPR, column = which * 16, chunk = (which & 3) * 2;
+    const bool mine = column < c.dim;
+    uint8_t* operand = smem + (which >> 2) * F::BLOCK;
+    KvConvert<F> kc, vc;
+    int page = kv_prompt_page(a, tile, steps, 0), page1 = kv_prompt_page(a, tile, steps, 1);
+    const int first_block = kv_prompt_block(c, tile, steps, 0, page);
+    kc.load(c.k, first_block, warp, c.dim, in_group, column, mine);
+    vc.load(c.v, first_block, warp, c.dim, in_group, column, mine);
+    auto scale_of = [&](const float* scales, int p) { return warp == 0 && p >= 0 ? scales[(long long)p * c.heads + tile.h] : 0.0f; };
+    float ks = scale_of(c.k_scale, page), vsc = scale_of(c.v_scale, page);
 
-    constexpr int RPP = 4 * F::TPL;                   // rows that four warps take at once
+    float top = 0.0f;
+    if (steps.total > 0) {
+        const int low = tile.low0, high = tile.last(), from = a.window > 0 ? max(low - a.window + 1, 0) >> pl : 0, to = (high >> pl) + 1;
+        const int sink_pages = a.sinks > 0 ? min(((a.sinks - 1) >> pl) + 1, from) : 0;
+#pragma unroll 2
+        for (int i = warp * 32 + lane; i < sink_pages + to - from; i += 224) {
+            const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
+            if (id >= 0) top = fmaxf(top, fabsf(c.v_scale[id * c.heads + tile.h]));
+        }
+    }
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if (lane == 0) part[warp] = top;
+
 #pragma unroll 1
-    for (int r0 = 0; r0 < F::ROWS; r0 += RPP) {
-        const int r = r0 + tid / LPR, row = tile.row0 + r;
-        const bool there = r < tile.rows && mine * 16 < c.dim;
+    for (int g = warp; g < F::ROWS / TPL; g += 7) {
+        const int r = g * TPL + in_group, row = tile.row0 + r;
+        const bool there = r < tile.rows && mine;
         float v[16];
-        if (there) kv_values16(a.q, a.q_type, a.wide_q, (long long)(tile.row + row / a.group) * a.q_stride + (long long)(tile.h * a.group + row % a.group) * c.dim + mine * 16, v);
+        if (there) kv_values16(a.q, a.q_type, a.wide_q, (long long)(tile.row + row / a.group) * a.q_stride + (long long)(tile.h * a.group + row % a.group) * c.dim + column, v);
         else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = 0.0f;
@@ -183,8 +218,10 @@ __device__ __forceinline__ void kv_prompt_keys(const KvAttendArgs& a, const KvPr
         for (int d = LPR / 2; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
         odd = (__ballot_sync(0xffffffffu, odd) >> (lane / LPR * LPR)) & ((1u << LPR) - 1u);
         const int e = min(max((int)(__float_as_uint(big) >> 23) - 127 - 14, -114), 127);
-        const float down = odd ? 0.0f : copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2), up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(127 + e, 1) << 23);
-        if (mine == 0) row_factor[r] = up * fabsf(a.scale_log2);
+        // (a negative scale's sign goes into q: scores are multiplied by positive numbers only)
+        const float down = odd ? 0.0f : copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);
+        const float up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(127 + e, 1) << 23);
+        if (which == 0) row_factor[r] = up * fabsf(a.scale_log2);
         uint32_t f[8];
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
@@ -194,54 +231,23 @@ __device__ __forceinline__ void kv_prompt_keys(const KvAttendArgs& a, const KvPr
             f[2 * z] = pack_f16(x[0], x[2]);
             f[2 * z + 1] = pack_f16(x[1], x[3]);
         }
-        uint8_t* to = smem + (r >> 7) * F::OPERAND;
-        *reinterpret_cast<uint4*>(to + codes.place(mine, r & 127, 0)) = make_uint4(f[0], f[1], f[2], f[3]);
-        *reinterpret_cast<uint4*>(to + codes.place(mine, r & 127, 1)) = make_uint4(f[4], f[5], f[6], f[7]);
+        uint8_t* to = operand + (r >> 7) * F::OPERAND + (r & 127) * 128;
+        *reinterpret_cast<uint4*>(to + ((chunk ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<uint4*>(to + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
     }
     kv_written(bar.q_full());
+    ptx::named_barrier_sync(1, 224);                  // (in front of any wait that may be given up)
+    const float vs = kv_prompt_top(part);
 
+#pragma unroll 1
     for (int k = 0; k < steps.total; ++k) {
-        const int page2 = kv_prompt_page(a, tile, steps, k + 2);
-        if (!kv_wait(a, bar.k_empty(k & 1), ((uint32_t)(k >> 1) & 1u) ^ 1u, abort_flag)) return;
-        codes.store(smem + F::OFF_K + (k & 1) * F::OPERAND);
-        kv_written(bar.k_full(k & 1));
-        codes.load(c, c.k, tile.h, page1, k + 1 < steps.total ? steps.at(k + 1, 128) : 0);
-        page1 = page2;
-    }
-}
-
-// ---- warps 13 .. 15: the largest scale of V, then V and what each step's pages say
-template <typename F>
-__device__ __forceinline__ void kv_prompt_values(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
-    const KvArgs& c = a.c;
-    const int tid = threadIdx.x - 13 * 32, lane = tid & 31, warp = tid >> 5, pl = c.page_log2;
-    float* info = reinterpret_cast<float*>(smem + F::OFF_INFO);
-    float* part = reinterpret_cast<float*>(smem + F::OFF_MAX);
-    const int low = tile.low0, high = tile.last();
-    KvConvert<F, 3> codes(lane, warp);
-    int page = kv_prompt_page(a, tile, steps, 0), page1 = kv_prompt_page(a, tile, steps, 1);
-    codes.load(c, c.v, tile.h, page, steps.total > 0 ? steps.at(0, 128) : 0);
-    auto scale_of = [&](const float* scales, int p) { return warp == 0 && p >= 0 ? scales[(long long)p * c.heads + tile.h] : 0.0f; };
-    float ks = scale_of(c.k_scale, page), vsc = scale_of(c.v_scale, page);
-    float top = 0.0f;
-    if (steps.total > 0) {
-        const int from = a.window > 0 ? max(low - a.window + 1, 0) >> pl : 0, to = (high >> pl) + 1;
-        const int sink_pages = a.sinks > 0 ? min(((a.sinks - 1) >> pl) + 1, from) : 0;
-#pragma unroll 4
-        for (int i = tid; i < sink_pages + to - from; i += 96) {
-            const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
-            if (id >= 0) top = fmaxf(top, fabsf(c.v_scale[id * c.heads + tile.h]));
-        }
-    }
-    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-    if (lane == 0) part[warp] = top;
-    ptx::named_barrier_sync(1, 96);                   // (in front of any wait that may be given up)
-    const float vs = fmaxf(fmaxf(part[0], part[1]), part[2]);
-
-    for (int k = 0; k < steps.total; ++k) {
-        const int page2 = kv_prompt_page(a, tile, steps, k + 2);
+        const uint32_t free_parity = ((uint32_t)(k >> 1) & 1u) ^ 1u;
+        const int page2 = kv_prompt_page(a, tile, steps, k + 2), block = kv_prompt_block(c, tile, steps, k + 1, page1);
         const float next_ks = scale_of(c.k_scale, page1), next_vsc = scale_of(c.v_scale, page1);
-        if (!kv_wait(a, bar.v_empty(k & 1), ((uint32_t)(k >> 1) & 1u) ^ 1u, abort_flag)) return;
+        if (!kv_wait(a, bar.k_empty(k & 1), free_parity, abort_flag)) return;
+        kc.store(operand + F::OFF_K + (k & 1) * F::OPERAND, warp, in_group, chunk);
+        kv_written(bar.k_full(k & 1));
+        kc.load(c.k, block, warp, c.dim, in_group, column, mine);
         if (warp == 0) {
             float* i = info + (k & 3) * F::INFO;
             const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
@@ -251,9 +257,10 @@ __device__ __forceinline__ void kv_prompt_values(const KvAttendArgs& a, const Kv
             if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8)); }
             __syncwarp();
         }
-        codes.store(smem + F::OFF_V + (k & 1) * F::OPERAND);
+        if (!kv_wait(a, bar.v_empty(k & 1), free_parity, abort_flag)) return;
+        vc.store(operand + F::OFF_V + (k & 1) * F::OPERAND, warp, in_group, chunk);
         kv_written(bar.v_full(k & 1));
-        codes.load(c, c.v, tile.h, page1, k + 1 < steps.total ? steps.at(k + 1, 128) : 0);
+        vc.load(c.v, block, warp, c.dim, in_group, column, mine);
         page = page1; page1 = page2;
         ks = next_ks; vsc = next_vsc;
     }
@@ -435,8 +442,7 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
         ptx::tc_fence_after();
     }
     const float* part = reinterpret_cast<const float*>(smem + F::OFF_MAX);
-    float vs = 0.0f;
-    if (count > 0) vs = fmaxf(fmaxf(part[0], part[1]), part[2]);
+    const float vs = count > 0 ? kv_prompt_top(part) : 0.0f;
     const bool mine_there = mine < tile.rows;
     if (spoilt & 1) l = __uint_as_float(0x7fffffffu);
     const float out_scale = spoilt ? __uint_as_float(0x7fffffffu) : (l == 0.0f ? 0.0f : vs * (1.0f / 64.0f) / l);
@@ -487,11 +493,11 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + F::OFF_TMEM + 8);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(bar.k_full(i), 4); ptx::mbar_init(bar.v_full(i), 3);
+            ptx::mbar_init(bar.k_full(i), 7); ptx::mbar_init(bar.v_full(i), 7);
             ptx::mbar_init(bar.k_empty(i), 1); ptx::mbar_init(bar.v_empty(i), 1);
             ptx::mbar_init(bar.s_full(i), 1); ptx::mbar_init(bar.p_full(i), 4); ptx::mbar_init(bar.o_full(i), 1);
         }
-        ptx::mbar_init(bar.q_full(), 4); ptx::mbar_init(bar.drained(), 1);
+        ptx::mbar_init(bar.q_full(), 7); ptx::mbar_init(bar.drained(), 1);
         ptx::mbar_fence_init();
         *abort_flag = (int)blockIdx.x == a.give_up ? 1 : 0;
     }
@@ -523,12 +529,9 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
         if (warp < 8) {
             set_registers_up<F::ROWS_REGS>();
             kv_prompt_rows<F>(a, tile, steps, bar, smem, tmem, abort_flag);
-        } else if (warp < 12) {
-            set_registers_down<F::OTHER_REGS>();
-            kv_prompt_keys<F>(a, tile, steps, bar, smem, abort_flag);
         } else {
             set_registers_down<F::OTHER_REGS>();
-            if (warp > 12) kv_prompt_values<F>(a, tile, steps, bar, smem, abort_flag);
+            if (warp != 12) kv_prompt_convert<F>(a, tile, steps, bar, smem, abort_flag);
             else {
                 kv_prompt_mma<F>(a, tile, steps, bar, s0, tmem, abort_flag);
                 // what the tensor core still does ends before its operands' memory is another kernel's, also where a wait was given up
