@@ -71,7 +71,7 @@ struct KvPromptCfg {
     static constexpr int ROWS_REGS = 152, OTHER_REGS = 104;       // 256 x 152 + 256 x 104 = 512 x 128
     static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN
     // factors of rows, info of 4 steps, maxima of scales, barriers, address of TMEM, flag
-    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 16 * 8, SMEM = OFF_TMEM + 16;
+    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 20 * 8, SMEM = OFF_TMEM + 16;
 };
 struct KvPromptBars {
     uint32_t at;
@@ -84,6 +84,7 @@ struct KvPromptBars {
     __device__ __forceinline__ uint32_t o_full(int x) const { return at + 96 + 8 * x; }
     __device__ __forceinline__ uint32_t q_full() const { return at + 112; }
     __device__ __forceinline__ uint32_t drained() const { return at + 120; }
+    __device__ __forceinline__ uint32_t info_full(int s) const { return at + 128 + 8 * s; }
 };
 
 // What all roles know of the CTA's rows.
@@ -244,11 +245,7 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         const uint32_t free_parity = ((uint32_t)(k >> 1) & 1u) ^ 1u;
         const int page2 = kv_prompt_page(a, tile, steps, k + 2), block = kv_prompt_block(c, tile, steps, k + 1, page1);
         const float next_ks = scale_of(c.k_scale, page1), next_vsc = scale_of(c.v_scale, page1);
-        if (!kv_wait(a, bar.k_empty(k & 1), free_parity, abort_flag)) return;
-        kc.store(operand + F::OFF_K + (k & 1) * F::OPERAND, warp, in_group, chunk);
-        kv_written(bar.k_full(k & 1));
-        kc.load(c.k, block, warp, c.dim, in_group, column, mine);
-        if (warp == 0) {
+        if (warp == 0) {                              // (in the place of step k - 4: its weights have been taken, or step k - 1's K would not have had room)
             float* i = info + (k & 3) * F::INFO;
             const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
             const bool k_nan = ks != ks, v_nan = vsc != vsc;
@@ -256,7 +253,12 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
             const unsigned there = __ballot_sync(0xffffffffu, page >= 0), bad_k = __ballot_sync(0xffffffffu, k_nan), bad_v = __ballot_sync(0xffffffffu, v_nan);
             if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8)); }
             __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar.info_full(k & 3));
         }
+        if (!kv_wait(a, bar.k_empty(k & 1), free_parity, abort_flag)) return;
+        kc.store(operand + F::OFF_K + (k & 1) * F::OPERAND, warp, in_group, chunk);
+        kv_written(bar.k_full(k & 1));
+        kc.load(c.k, block, warp, c.dim, in_group, column, mine);
         if (!kv_wait(a, bar.v_empty(k & 1), free_parity, abort_flag)) return;
         vc.store(operand + F::OFF_V + (k & 1) * F::OPERAND, warp, in_group, chunk);
         kv_written(bar.v_full(k & 1));
@@ -378,7 +380,7 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     for (int k = 0; k < steps.total; ++k) {
         const int t = steps.at(k, 128);
         if (!tile.active(x, t, a.window, a.sinks)) continue;
-        if (!kv_wait(a, bar.v_full(k & 1), (uint32_t)(k >> 1) & 1u, abort_flag)) return;       // what the step's pages say
+        if (!kv_wait(a, bar.info_full(k & 3), (uint32_t)(k >> 2) & 1u, abort_flag)) return;    // what the step's pages say
         if (!kv_wait(a, bar.s_full(x), (uint32_t)count & 1u, abort_flag)) return;
         ptx::tc_fence_after();
         if (count == 0) {
@@ -497,6 +499,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
             ptx::mbar_init(bar.k_empty(i), 1); ptx::mbar_init(bar.v_empty(i), 1);
             ptx::mbar_init(bar.s_full(i), 1); ptx::mbar_init(bar.p_full(i), 4); ptx::mbar_init(bar.o_full(i), 1);
         }
+        for (int i = 0; i < 4; ++i) ptx::mbar_init(bar.info_full(i), 1);
         ptx::mbar_init(bar.q_full(), 7); ptx::mbar_init(bar.drained(), 1);
         ptx::mbar_fence_init();
         *abort_flag = (int)blockIdx.x == a.give_up ? 1 : 0;
