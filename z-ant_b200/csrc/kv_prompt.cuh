@@ -10,7 +10,7 @@
 // rescaled), and what is lost below f16's least numbers is 2^-31 of the largest weight.  The sum of the weights takes the factor out again, once for 16 tokens.
 //
 //   warps 0 .. 3, 4 .. 7  rows of the first and the second tile      12  TMEM owner, MMA issuer      8 .. 11, 13 .. 15  q and codes to f16, scales
-// Registers: 152 for the rows' threads, 104 for others (setmaxnreg; 128 each at launch).
+// Registers: 136 for the rows' threads, 120 for others (setmaxnreg; 128 each at launch).
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -68,7 +68,7 @@ struct KvPromptCfg {
     static constexpr int OFF_K = 2 * OPERAND, OFF_V = 4 * OPERAND, OFF_REST = 6 * OPERAND;
     static constexpr int LPR = DP / 16;               // lanes of a row of codes
     static constexpr int TPL = 32 / LPR;              // tokens of a warp's load
-    static constexpr int ROWS_REGS = 152, OTHER_REGS = 104;       // 256 x 152 + 256 x 104 = 512 x 128
+    static constexpr int ROWS_REGS = 136, OTHER_REGS = 120;       // 256 x 136 + 256 x 120 = 512 x 128
     static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN
     // factors of rows, info of 4 steps, maxima of scales, barriers, address of TMEM, flag
     static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 20 * 8, SMEM = OFF_TMEM + 16;
@@ -111,8 +111,23 @@ __device__ __forceinline__ float kv_prompt_top(const float* part) {
     return v;
 }
 
+// A whole warp's wait: polls in turns of 64, one vote and one branch each (mbar_wait's lanes branch by themselves: the waiting warps took a third of all instructions).
 __device__ __forceinline__ bool kv_wait(const KvAttendArgs& a, uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag, a.wait_budget));
+    long long t0 = 0;
+    while (true) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred P, Q, R;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
+                     "KV_WAIT_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\tvote.sync.all.pred Q, P, 0xffffffff;\n\t@Q bra.uni KV_DONE_%=;\n\t"
+                     "add.u32 n, n, 1;\n\tsetp.lt.u32 R, n, 64;\n\t@R bra.uni KV_WAIT_%=;\n"
+                     "KV_DONE_%=:\n\tselp.u32 %0, 1, 0, Q;\n\t}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        const bool flag = *abort_flag != 0;
+        const long long now = clock64();
+        if (t0 == 0) t0 = now;
+        const bool late = now - t0 > a.wait_budget;
+        if (late) *abort_flag = 1;
+        if (__any_sync(0xffffffffu, flag || late)) return false;
+    }
 }
 
 // Codes on their way to f16 operands: warp `warp` of the seven takes every seventh TPL tokens of a step's 128.
@@ -130,7 +145,7 @@ struct KvConvert {
             const bool in = mine && block >= 0 && (GROUPS % WARPS == 0 || group < GROUPS);
             const int8_t* p = codes + (unsigned long long)(unsigned)block * (unsigned)(16 * dim) + (unsigned)(((tok & 15) + in_group) * dim + column);
             w[i] = make_uint4(0, 0, 0, 0);
-            if (in) w[i] = *reinterpret_cast<const uint4*>(p);
+            if (in) w[i] = ptx::ld_global_once(reinterpret_cast<const uint4*>(p));     // (past L1)
         }
     }
     // to: the operand, and the lane's place in row in_group of it
@@ -167,7 +182,7 @@ __device__ __forceinline__ int kv_prompt_block(const KvArgs& c, const KvPromptTi
     return (int)((((unsigned)page * (unsigned)c.heads + (unsigned)tile.h) << (c.page_log2 - 4)) + (unsigned)((t & (c.page - 1)) >> 4));
 }
 
-// ---- warps 8 .. 11 and 13 .. 15: the largest scale of V; q; K, V and what each step's pages say.  Codes are on their way a step ahead, pages two.
+// ---- warps 8 .. 11 and 13 .. 15 (the last one has the fewest tokens and says what pages are like): the largest scale of V; q; K, V and what each step's pages say.  Codes are on their way a step ahead, pages two.
 template <typename F>
 __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
     constexpr int LPR = F::LPR, TPL = F::TPL;
@@ -185,7 +200,7 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
     const int first_block = kv_prompt_block(c, tile, steps, 0, page);
     kc.load(c.k, first_block, warp, c.dim, in_group, column, mine);
     vc.load(c.v, first_block, warp, c.dim, in_group, column, mine);
-    auto scale_of = [&](const float* scales, int p) { return warp == 0 && p >= 0 ? scales[(long long)p * c.heads + tile.h] : 0.0f; };
+    auto scale_of = [&](const float* scales, int p) { return warp == 6 && p >= 0 ? scales[(long long)p * c.heads + tile.h] : 0.0f; };
     float ks = scale_of(c.k_scale, page), vsc = scale_of(c.v_scale, page);
 
     float top = 0.0f;
@@ -245,7 +260,7 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         const uint32_t free_parity = ((uint32_t)(k >> 1) & 1u) ^ 1u;
         const int page2 = kv_prompt_page(a, tile, steps, k + 2), block = kv_prompt_block(c, tile, steps, k + 1, page1);
         const float next_ks = scale_of(c.k_scale, page1), next_vsc = scale_of(c.v_scale, page1);
-        if (warp == 0) {                              // (in the place of step k - 4: its weights have been taken, or step k - 1's K would not have had room)
+        if (warp == 6) {                              // (in the place of step k - 4: its weights have been taken, or step k - 1's K would not have had room)
             float* i = info + (k & 3) * F::INFO;
             const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
             const bool k_nan = ks != ks, v_nan = vsc != vsc;
