@@ -69,9 +69,9 @@ struct KvPromptCfg {
     static constexpr int LPR = DP / 16;               // lanes of a row of codes
     static constexpr int TPL = 32 / LPR;              // tokens of a warp's load
     static constexpr int ROWS_REGS = 136, OTHER_REGS = 120;       // 256 x 136 + 256 x 120 = 512 x 128
-    static constexpr int INFO = 28;                   // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN
-    // factors of rows, info of 4 steps, maxima of scales, barriers, address of TMEM, flag
-    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + 4 * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 20 * 8, SMEM = OFF_TMEM + 16;
+    static constexpr int INFO = 36, RING = 8;         // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN; where they lie
+    // factors of rows, info of RING steps, maxima of scales, barriers, address of TMEM, flag
+    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + RING * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 24 * 8, SMEM = OFF_TMEM + 16;
 };
 struct KvPromptBars {
     uint32_t at;
@@ -94,13 +94,23 @@ struct KvPromptTile {
     __device__ __forceinline__ int low(int x) const { return x ? low1 : low0; }
     __device__ __forceinline__ int high(int x) const { return x ? high1 : high0; }
     __device__ __forceinline__ int last() const { return max(high0, high1); }
-    __device__ __forceinline__ bool active(int x, int t, int window, int sinks) const {
-        return t <= high(x) && (window == 0 || t + 127 > low(x) - window || t < sinks);
+};
+
+// The steps of a tile: those behind the sinks' own from `from` on and before `to` are its (and all of the sinks' before `to`); of these it sees all of the tokens from
+// `whole_from` on and before `whole_to`.
+struct KvPromptSteps {
+    int sink, from, to, whole_from, whole_to;
+    __device__ __forceinline__ KvPromptSteps(const KvSteps& s, int low, int high, int window, int sinks) {
+        // a step k behind the sinks' begins at 128 (k + add)
+        const int add = s.first - s.sink;
+        sink = s.sink > 0 ? s.sink : (int)min(((long long)sinks + 127) / 128, (long long)s.total);      // (none of their own: they are in front of `from` all the same)
+        to = high < 0 ? 0 : min(s.total, high < 128 * s.first ? min(s.sink, high / 128 + 1) : high / 128 + 1 - add);
+        from = window > 0 && low - window + 1 > 0 ? (low - window + 1) / 128 - add : 0;
+        whole_to = min(to, low < 127 ? 0 : (low - 127) / 128 + 1 - add);
+        whole_from = max(s.sink, window > 0 && high - window + 1 > 0 ? (high - window + 1 + 127) / 128 - add : 0);
     }
-    // every row sees all of the step
-    __device__ __forceinline__ bool whole(int x, int t, int window, int sinks) const {
-        return t + 127 <= low(x) && (window == 0 || t > high(x) - window || t + 128 <= sinks);
-    }
+    __device__ __forceinline__ bool active(int k) const { return k < to && (k < sink || k >= from); }
+    __device__ __forceinline__ bool whole(int k) const { return k >= whole_from && k < whole_to; }
 };
 
 // The largest of the seven warps' numbers.
@@ -135,17 +145,15 @@ template <typename F>
 struct KvConvert {
     static constexpr int WARPS = 7, LPR = F::LPR, GROUPS = 128 / F::TPL, N = (GROUPS + WARPS - 1) / WARPS;
     uint4 w[N];
-    // blocks: where 16 tokens each lie in the cache, in units of 16 tokens, in lanes 0 .. 7 (-1: nowhere); at: the lane's place in the 16 tokens of even (and, where a load has 8
-    // tokens, of any) groups, in bytes; mine: there are such dimensions
-    __device__ __forceinline__ void load(const int8_t* codes, int blocks, int warp, int dim, int in_group, int column, bool mine) {
+    // blocks: where 16 tokens each lie in the cache, in units of 16 tokens (-1: nowhere); mine: the lane's 16 bytes are dimensions of the head
+    __device__ __forceinline__ void load(const int8_t* codes, const int* blocks, int warp, int dim, int in_group, int column, bool mine) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int group = i * WARPS + warp, tok = group * F::TPL;
-            const int block = __shfl_sync(0xffffffffu, blocks, (tok >> 4) & 7);
-            const bool in = mine && block >= 0 && (GROUPS % WARPS == 0 || group < GROUPS);
+            const int block = GROUPS % WARPS == 0 || group < GROUPS ? blocks[tok >> 4] : -1;
             const int8_t* p = codes + (unsigned long long)(unsigned)block * (unsigned)(16 * dim) + (unsigned)(((tok & 15) + in_group) * dim + column);
             w[i] = make_uint4(0, 0, 0, 0);
-            if (in) w[i] = ptx::ld_global_once(reinterpret_cast<const uint4*>(p));     // (past L1)
+            if (mine && block >= 0) w[i] = ptx::ld_global_once(reinterpret_cast<const uint4*>(p));     // (past L1)
         }
     }
     // to: the operand, and the lane's place in row in_group of it
@@ -182,7 +190,7 @@ __device__ __forceinline__ int kv_prompt_block(const KvArgs& c, const KvPromptTi
     return (int)((((unsigned)page * (unsigned)c.heads + (unsigned)tile.h) << (c.page_log2 - 4)) + (unsigned)((t & (c.page - 1)) >> 4));
 }
 
-// ---- warps 8 .. 11 and 13 .. 15 (the last one has the fewest tokens and says what pages are like): the largest scale of V; q; K, V and what each step's pages say.  Codes are on their way a step ahead, pages two.
+// ---- warps 8 .. 11 and 13 .. 15: the largest scale of V; q; K, V and what each step's pages say.  Codes are on their way a step ahead.
 template <typename F>
 __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
     constexpr int LPR = F::LPR, TPL = F::TPL;
@@ -196,12 +204,30 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
     const bool mine = column < c.dim;
     uint8_t* operand = smem + (which >> 2) * F::BLOCK;
     KvConvert<F> kc, vc;
-    int page = kv_prompt_page(a, tile, steps, 0), page1 = kv_prompt_page(a, tile, steps, 1);
-    const int first_block = kv_prompt_block(c, tile, steps, 0, page);
-    kc.load(c.k, first_block, warp, c.dim, in_group, column, mine);
-    vc.load(c.v, first_block, warp, c.dim, in_group, column, mine);
-    auto scale_of = [&](const float* scales, int p) { return warp == 6 && p >= 0 ? scales[(long long)p * c.heads + tile.h] : 0.0f; };
-    float ks = scale_of(c.k_scale, page), vsc = scale_of(c.v_scale, page);
+    // The last warp (it has the fewest tokens) says what a step's pages are like, two steps before the others ask: in the place of step k - 6 then, whose weights have been taken, or
+    // step k - 1's K would not have had room.
+    int page = -1;
+    float ks = 0.0f, vsc = 0.0f;
+    auto look = [&](int k) {                          // on their way
+        page = kv_prompt_page(a, tile, steps, k);
+        ks = page >= 0 ? c.k_scale[(long long)page * c.heads + tile.h] : 0.0f;
+        vsc = page >= 0 ? c.v_scale[(long long)page * c.heads + tile.h] : 0.0f;
+    };
+    auto tell = [&](int k, float vs) {
+        float* i = info + (k & (F::RING - 1)) * F::INFO;
+        const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
+        const bool k_nan = ks != ks, v_nan = vsc != vsc;
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0), bad_k = __ballot_sync(0xffffffffu, k_nan), bad_v = __ballot_sync(0xffffffffu, v_nan);
+        if (lane < 8) {
+            i[lane] = k_nan ? 0.0f : fabsf(ks); i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 6.0f);
+            reinterpret_cast<int*>(i)[28 + lane] = kv_prompt_block(c, tile, steps, k, page);
+        }
+        if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8)); }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar.info_full(k & (F::RING - 1)));
+    };
+    auto blocks = [&](int k) { return reinterpret_cast<const int*>(info + (k & (F::RING - 1)) * F::INFO) + 28; };
+    if (warp == 6) look(0);
 
     float top = 0.0f;
     if (steps.total > 0) {
@@ -254,32 +280,32 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
     kv_written(bar.q_full());
     ptx::named_barrier_sync(1, 224);                  // (in front of any wait that may be given up)
     const float vs = kv_prompt_top(part);
+    if (warp == 6) {
+        tell(0, vs);
+        look(1);
+        tell(1, vs);
+        look(2);
+    }
+    if (!kv_wait(a, bar.info_full(0), 0, abort_flag)) return;
+    kc.load(c.k, blocks(0), warp, c.dim, in_group, column, mine);
+    vc.load(c.v, blocks(0), warp, c.dim, in_group, column, mine);
 
 #pragma unroll 1
     for (int k = 0; k < steps.total; ++k) {
         const uint32_t free_parity = ((uint32_t)(k >> 1) & 1u) ^ 1u;
-        const int page2 = kv_prompt_page(a, tile, steps, k + 2), block = kv_prompt_block(c, tile, steps, k + 1, page1);
-        const float next_ks = scale_of(c.k_scale, page1), next_vsc = scale_of(c.v_scale, page1);
-        if (warp == 6) {                              // (in the place of step k - 4: its weights have been taken, or step k - 1's K would not have had room)
-            float* i = info + (k & 3) * F::INFO;
-            const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
-            const bool k_nan = ks != ks, v_nan = vsc != vsc;
-            if (lane < 8) { i[lane] = k_nan ? 0.0f : fabsf(ks); i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 6.0f); }
-            const unsigned there = __ballot_sync(0xffffffffu, page >= 0), bad_k = __ballot_sync(0xffffffffu, k_nan), bad_v = __ballot_sync(0xffffffffu, v_nan);
-            if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8)); }
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(bar.info_full(k & 3));
-        }
+        if (!kv_wait(a, bar.info_full((k + 1) & (F::RING - 1)), (uint32_t)((k + 1) / F::RING) & 1u, abort_flag)) return;
         if (!kv_wait(a, bar.k_empty(k & 1), free_parity, abort_flag)) return;
         kc.store(operand + F::OFF_K + (k & 1) * F::OPERAND, warp, in_group, chunk);
         kv_written(bar.k_full(k & 1));
-        kc.load(c.k, block, warp, c.dim, in_group, column, mine);
+        kc.load(c.k, blocks(k + 1), warp, c.dim, in_group, column, mine);
+        if (warp == 6) {
+            tell(k + 2, vs);
+            look(k + 3);
+        }
         if (!kv_wait(a, bar.v_empty(k & 1), free_parity, abort_flag)) return;
         vc.store(operand + F::OFF_V + (k & 1) * F::OPERAND, warp, in_group, chunk);
         kv_written(bar.v_full(k & 1));
-        vc.load(c.v, block, warp, c.dim, in_group, column, mine);
-        page = page1; page1 = page2;
-        ks = next_ks; vsc = next_vsc;
+        vc.load(c.v, blocks(k + 1), warp, c.dim, in_group, column, mine);
     }
 }
 
@@ -290,11 +316,7 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
     constexpr uint32_t idesc_s = idesc_f16(128, 128, false), idesc_o = idesc_f16(128, DP, true);
     const uint32_t leader = ptx::elect_one() ? 1u : 0u;
     int count[2] = {0, 0};                            // products P V so far
-    int last[2] = {-1, -1};                           // a tile's last step
-    for (int k = 0; k < steps.total; ++k)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-            if (tile.active(x, steps.at(k, 128), a.window, a.sinks)) last[x] = k;
+    const KvPromptSteps mine[2] = {KvPromptSteps(steps, tile.low0, tile.high0, a.window, a.sinks), KvPromptSteps(steps, tile.low1, tile.high1, a.window, a.sinks)};
     auto scores = [&](int x, int k) {
         const uint32_t qa = kv_desc_lo(s0 + x * F::OPERAND, 16), kb = kv_desc_lo(s0 + F::OFF_K + (k & 1) * F::OPERAND, 16);
 #pragma unroll
@@ -309,9 +331,9 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
 #pragma unroll
         for (int i = 0; i < 8; ++i) mma_f16_ts_if(leader, tmem + 256 + x * DP, tmem + x * 128 + i * 8, vb + i * (2048 >> 4), idesc_o, (count[x] | i) != 0);
         ++count[x];
-        if (k == last[x]) ptx::mma_commit_if(leader, bar.o_full(x));
+        if (k == mine[x].to - 1) ptx::mma_commit_if(leader, bar.o_full(x));      // its last step
     };
-    auto active = [&](int x, int k) { return k < steps.total && tile.active(x, steps.at(k, 128), a.window, a.sinks); };
+    auto active = [&](int x, int k) { return mine[x].active(k); };
     if (steps.total > 0) {
         if (!kv_wait(a, bar.q_full(), 0, abort_flag) || !kv_wait(a, bar.k_full(0), 0, abort_flag)) return;
         ptx::tc_fence_after();
@@ -391,21 +413,21 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     const float* all_info = reinterpret_cast<const float*>(smem + F::OFF_INFO);
     const int row = tile.row0 + min(mine, tile.rows - 1), pos = max(tile.first + row / a.group, -1);
     float factor = 0.0f, m = -INFINITY, l = 0.0f;
+    const KvPromptSteps own(steps, tile.low(x), tile.high(x), a.window, a.sinks);
     int count = 0, spoilt = 0;                        // spoilt: 1 by a page's scale of K, 2 of V
-    for (int k = 0; k < steps.total; ++k) {
-        const int t = steps.at(k, 128);
-        if (!tile.active(x, t, a.window, a.sinks)) continue;
-        if (!kv_wait(a, bar.info_full(k & 3), (uint32_t)(k >> 2) & 1u, abort_flag)) return;    // what the step's pages say
+    for (int k = 0; k < own.to; ++k) {
+        if (!own.active(k)) continue;
+        if (!kv_wait(a, bar.info_full(k & (F::RING - 1)), (uint32_t)(k / F::RING) & 1u, abort_flag)) return;       // what the step's pages say
         if (!kv_wait(a, bar.s_full(x), (uint32_t)count & 1u, abort_flag)) return;
         ptx::tc_fence_after();
         if (count == 0) {
             if (!kv_wait(a, bar.q_full(), 0, abort_flag)) return;
             factor = reinterpret_cast<const float*>(smem + F::OFF_REST)[mine];
         }
-        const float* info = all_info + (k & 3) * F::INFO;
+        const float* info = all_info + (k & (F::RING - 1)) * F::INFO;
         const int there = reinterpret_cast<const int*>(info)[24], nan = reinterpret_cast<const int*>(info)[25];
-        if (there != 255 || nan != 0 || !tile.whole(x, t, a.window, a.sinks)) {
-            const int upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
+        if (there != 255 || nan != 0 || !own.whole(k)) {
+            const int t = steps.at(k, 128), upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
 #pragma unroll 1
             for (int g = 0; g < 4; ++g) {
                 uint32_t seen = first_columns(upto + 1 - 32 * g) & (~first_columns(behind + 1 - 32 * g) | first_columns(sunk - 32 * g));
@@ -514,7 +536,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
             ptx::mbar_init(bar.k_empty(i), 1); ptx::mbar_init(bar.v_empty(i), 1);
             ptx::mbar_init(bar.s_full(i), 1); ptx::mbar_init(bar.p_full(i), 4); ptx::mbar_init(bar.o_full(i), 1);
         }
-        for (int i = 0; i < 4; ++i) ptx::mbar_init(bar.info_full(i), 1);
+        for (int i = 0; i < F::RING; ++i) ptx::mbar_init(bar.info_full(i), 1);
         ptx::mbar_init(bar.q_full(), 7); ptx::mbar_init(bar.drained(), 1);
         ptx::mbar_fence_init();
         *abort_flag = (int)blockIdx.x == a.give_up ? 1 : 0;
