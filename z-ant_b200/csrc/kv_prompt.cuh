@@ -1,8 +1,9 @@
 // Attention of many new tokens (prompts, parts of them) over the cache of kv_cache.cuh on tcgen05: the formulas and masks of kv_attention.cuh for results in 16 bits.
 //
-// A CTA has 256 rows, (new token, head) pairs that share a key head, as two tiles of 128 that take turns: while the tensor core multiplies for one, the other one's
-// exponentials are taken.  Steps of 128 tokens.  Codes become f16 (exactly) once for all 256 rows; q is f16 times a power of two for each row, so that its largest value lies in
-// [2^14, 2^15) (f16 and bf16 values lose nothing down to 2^-28 of that one).  Scores are 128 x 128 x dim products into tensor memory; each thread has a row of them, finds its maximum, and
+// A CTA has 256 rows, (new token, head) pairs that share a key head, as two tiles of 128.  Steps of 128 tokens, whose scores come in halves of 64 with a place each in tensor memory: while a
+// row's thread takes the exponentials of one half, the tensor core multiplies V with the other half's weights and takes the next step's scores in its place.  (Whole steps with one
+// place: the rows waited 1300 clocks of 4500 for their next scores.)  Codes become f16 (exactly) once for all 256 rows; q is f16 times a power of two for each row, so that its largest value lies in
+// [2^14, 2^15) (f16 and bf16 values lose nothing down to 2^-28 of that one).  Scores are 128 x 64 x dim products into tensor memory; each thread has a row of them, finds its maximum, and
 // writes the weights back over them as f16, where they are the next product's operand.
 //
 // A page's scale of K multiplies its columns' scores; its scale of V, over the largest of the pages that the CTA sees, goes into the exponent: weights are 2^(x - m + lv + 6) with
@@ -71,7 +72,7 @@ struct KvPromptCfg {
     static constexpr int ROWS_REGS = 136, OTHER_REGS = 120;       // 256 x 136 + 256 x 120 = 512 x 128
     static constexpr int INFO = 36, RING = 8;         // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN; where they lie
     // factors of rows, info of RING steps, maxima of scales, barriers, address of TMEM, flag
-    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + RING * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 24 * 8, SMEM = OFF_TMEM + 16;
+    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + RING * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 30 * 8, SMEM = OFF_TMEM + 16;
 };
 struct KvPromptBars {
     uint32_t at;
@@ -79,12 +80,13 @@ struct KvPromptBars {
     __device__ __forceinline__ uint32_t v_full(int s) const { return at + 16 + 8 * s; }
     __device__ __forceinline__ uint32_t k_empty(int s) const { return at + 32 + 8 * s; }
     __device__ __forceinline__ uint32_t v_empty(int s) const { return at + 48 + 8 * s; }
-    __device__ __forceinline__ uint32_t s_full(int x) const { return at + 64 + 8 * x; }
-    __device__ __forceinline__ uint32_t p_full(int x) const { return at + 80 + 8 * x; }
-    __device__ __forceinline__ uint32_t o_full(int x) const { return at + 96 + 8 * x; }
-    __device__ __forceinline__ uint32_t q_full() const { return at + 112; }
-    __device__ __forceinline__ uint32_t drained() const { return at + 120; }
-    __device__ __forceinline__ uint32_t info_full(int s) const { return at + 128 + 8 * s; }
+    __device__ __forceinline__ uint32_t s_full(int x, int b) const { return at + 64 + 16 * x + 8 * b; }
+    __device__ __forceinline__ uint32_t p_full(int x, int b) const { return at + 96 + 16 * x + 8 * b; }
+    __device__ __forceinline__ uint32_t pv_done(int x) const { return at + 128 + 8 * x; }
+    __device__ __forceinline__ uint32_t o_full(int x) const { return at + 144 + 8 * x; }
+    __device__ __forceinline__ uint32_t q_full() const { return at + 160; }
+    __device__ __forceinline__ uint32_t drained() const { return at + 168; }
+    __device__ __forceinline__ uint32_t info_full(int s) const { return at + 176 + 8 * s; }
 };
 
 // What all roles know of the CTA's rows.
@@ -313,68 +315,67 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
 template <typename F>
 __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint32_t s0, uint32_t tmem, volatile int* abort_flag) {
     constexpr int DP = F::DP;
-    constexpr uint32_t idesc_s = idesc_f16(128, 128, false), idesc_o = idesc_f16(128, DP, true);
+    constexpr uint32_t idesc_s = idesc_f16(128, 64, false), idesc_o = idesc_f16(128, DP, true);
     const uint32_t leader = ptx::elect_one() ? 1u : 0u;
-    int count[2] = {0, 0};                            // products P V so far
+    int count[2] = {0, 0};                            // a tile's steps so far
     const KvPromptSteps mine[2] = {KvPromptSteps(steps, tile.low0, tile.high0, a.window, a.sinks), KvPromptSteps(steps, tile.low1, tile.high1, a.window, a.sinks)};
-    auto scores = [&](int x, int k) {
-        const uint32_t qa = kv_desc_lo(s0 + x * F::OPERAND, 16), kb = kv_desc_lo(s0 + F::OFF_K + (k & 1) * F::OPERAND, 16);
+    auto scores = [&](int x, int k, int b) {
+        const uint32_t qa = kv_desc_lo(s0 + x * F::OPERAND, 16), kb = kv_desc_lo(s0 + F::OFF_K + (k & 1) * F::OPERAND + b * 64 * 128, 16);
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
             const uint32_t at = ((i >> 2) * F::BLOCK + (i & 3) * 32) >> 4;
-            mma_f16_ss_if(leader, tmem + x * 128, qa + at, kb + at, idesc_s, i > 0);
+            mma_f16_ss_if(leader, tmem + x * 128 + b * 64, qa + at, kb + at, idesc_s, i > 0);
         }
-        ptx::mma_commit_if(leader, bar.s_full(x));
+        ptx::mma_commit_if(leader, bar.s_full(x, b));
     };
-    auto values = [&](int x, int k) {
-        const uint32_t vb = kv_desc_lo(s0 + F::OFF_V + (k & 1) * F::OPERAND, F::BLOCK);
+    auto values = [&](int x, int k, int b) {
+        const uint32_t vb = kv_desc_lo(s0 + F::OFF_V + (k & 1) * F::OPERAND + b * 64 * 128, F::BLOCK);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mma_f16_ts_if(leader, tmem + 256 + x * DP, tmem + x * 128 + i * 8, vb + i * (2048 >> 4), idesc_o, (count[x] | i) != 0);
-        ++count[x];
-        if (k == mine[x].to - 1) ptx::mma_commit_if(leader, bar.o_full(x));      // its last step
+        for (int i = 0; i < 4; ++i) mma_f16_ts_if(leader, tmem + 256 + x * DP, tmem + x * 128 + b * 64 + i * 8, vb + i * (2048 >> 4), idesc_o, (count[x] | b | i) != 0);
+        ptx::mma_commit_if(leader, bar.pv_done(x));
+        if (b == 1 && k == mine[x].to - 1) ptx::mma_commit_if(leader, bar.o_full(x));      // its last step
     };
-    auto active = [&](int x, int k) { return mine[x].active(k); };
     if (steps.total > 0) {
         if (!kv_wait(a, bar.q_full(), 0, abort_flag) || !kv_wait(a, bar.k_full(0), 0, abort_flag)) return;
         ptx::tc_fence_after();
 #pragma unroll
-        for (int x = 0; x < 2; ++x) if (active(x, 0)) scores(x, 0);
+        for (int i = 0; i < 4; ++i) if (mine[i & 1].active(0)) scores(i & 1, 0, i >> 1);
         ptx::mma_commit_if(leader, bar.k_empty(0));
     }
     for (int k = 0; k < steps.total; ++k) {
         const uint32_t parity = (uint32_t)(k >> 1) & 1u, next_parity = (uint32_t)((k + 1) >> 1) & 1u;
         if (!kv_wait(a, bar.v_full(k & 1), parity, abort_flag)) return;
-        bool k_there = false;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            if (active(x, k)) {
-                if (!kv_wait(a, bar.p_full(x), (uint32_t)count[x] & 1u, abort_flag)) return;
+        for (int i = 0; i < 4; ++i) {                 // the first half of either tile, the second
+            const int x = i & 1, b = i >> 1;
+            if (mine[x].active(k)) {
+                if (!kv_wait(a, bar.p_full(x, b), (uint32_t)count[x] & 1u, abort_flag)) return;
                 ptx::tc_fence_after();
-                values(x, k);
+                values(x, k, b);
+                count[x] += b;
             }
-            if (x == 1) ptx::mma_commit_if(leader, bar.v_empty(k & 1));
+            if (i == 3) ptx::mma_commit_if(leader, bar.v_empty(k & 1));
             if (k + 1 < steps.total) {
-                if (!k_there && !kv_wait(a, bar.k_full((k + 1) & 1), next_parity, abort_flag)) return;
-                k_there = true;
+                if (i == 0 && !kv_wait(a, bar.k_full((k + 1) & 1), next_parity, abort_flag)) return;
                 ptx::tc_fence_after();
-                if (active(x, k + 1)) scores(x, k + 1);
+                if (mine[x].active(k + 1)) scores(x, k + 1, b);
             }
         }
         if (k + 1 < steps.total) ptx::mma_commit_if(leader, bar.k_empty((k + 1) & 1));
     }
 }
 
-// Weights of a row's 128 scores in tensor memory at `ts` (minus infinity: not seen), in pairs, under the base `base` (log2): p, their sum with each page's factor taken out, and
+// Weights of a row's 64 scores in tensor memory at `ts` (minus infinity: not seen), in pairs, under the base `base` (log2): p, their sum with each page's factor taken out, and
 // the largest exponent.
-__device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* info, float factor, float base, uint32_t (&p)[64], float& sum) {
+__device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* info, float factor, float base, uint32_t (&p)[32], float& sum) {
     uint32_t v[2][16];
     float top = -INFINITY;
     sum = 0.0f;
     ptx::tmem_ld16(ts, v[0]);
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {                     // 16 tokens, which are on one page
+    for (int g = 0; g < 4; ++g) {                     // 16 tokens, which are on one page
         tmem_wait_ld16(v[g & 1]);
-        if (g < 7) ptx::tmem_ld16(ts + 16 * (g + 1), v[(g + 1) & 1]);
+        if (g < 3) ptx::tmem_ld16(ts + 16 * (g + 1), v[(g + 1) & 1]);
         float f = factor * info[g];
         f = f == 0.0f ? 1e-38f : f;                   // (minus infinity stays what it is)
         const float lv = info[8 + g], b = lv + 6.0f - base;
@@ -409,31 +410,34 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     constexpr int DP = F::DP;
     const KvArgs& c = a.c;
     const int x = threadIdx.x >> 7, r = threadIdx.x & 127, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = x * 128 + r;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + x * 128 + lanes, to = tmem + 256 + x * DP + lanes;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, to = tmem + 256 + x * DP + lanes;
     const float* all_info = reinterpret_cast<const float*>(smem + F::OFF_INFO);
     const int row = tile.row0 + min(mine, tile.rows - 1), pos = max(tile.first + row / a.group, -1);
     float factor = 0.0f, m = -INFINITY, l = 0.0f;
     const KvPromptSteps own(steps, tile.low(x), tile.high(x), a.window, a.sinks);
-    int count = 0, spoilt = 0;                        // spoilt: 1 by a page's scale of K, 2 of V
-    for (int k = 0; k < own.to; ++k) {
+    int count = 0, spoilt = 0;                        // halves so far; 1: by a page's scale of K, 2: of V
+    if (own.to > 0) {
+        if (!kv_wait(a, bar.q_full(), 0, abort_flag)) return;
+        factor = reinterpret_cast<const float*>(smem + F::OFF_REST)[mine];
+    }
+    for (int j = 0; j < 2 * own.to; ++j) {            // halves of steps
+        const int k = j >> 1, b = j & 1;
         if (!own.active(k)) continue;
-        if (!kv_wait(a, bar.info_full(k & (F::RING - 1)), (uint32_t)(k / F::RING) & 1u, abort_flag)) return;       // what the step's pages say
-        if (!kv_wait(a, bar.s_full(x), (uint32_t)count & 1u, abort_flag)) return;
+        const uint32_t ts = tmem + x * 128 + b * 64 + lanes;
+        if (!kv_wait(a, bar.s_full(x, b), (uint32_t)(count >> 1) & 1u, abort_flag)) return;
         ptx::tc_fence_after();
-        if (count == 0) {
-            if (!kv_wait(a, bar.q_full(), 0, abort_flag)) return;
-            factor = reinterpret_cast<const float*>(smem + F::OFF_REST)[mine];
-        }
+        // (what the step's pages say was said before its K was there)
         const float* info = all_info + (k & (F::RING - 1)) * F::INFO;
-        const int there = reinterpret_cast<const int*>(info)[24], nan = reinterpret_cast<const int*>(info)[25];
-        if (there != 255 || nan != 0 || !own.whole(k)) {
-            const int t = steps.at(k, 128), upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
+        const int2 pages = *reinterpret_cast<const int2*>(info + 24);
+        if (pages.x != 255 || pages.y != 0 || !own.whole(k)) {
+            const int there = pages.x >> (4 * b), k_nan = pages.y >> (4 * b), v_nan = pages.y >> (8 + 4 * b);       // of the half's four 16 tokens
+            const int t = steps.at(k, 128) + 64 * b, upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
 #pragma unroll 1
-            for (int g = 0; g < 4; ++g) {
+            for (int g = 0; g < 2; ++g) {
                 uint32_t seen = first_columns(upto + 1 - 32 * g) & (~first_columns(behind + 1 - 32 * g) | first_columns(sunk - 32 * g));
                 seen &= ((there >> (2 * g)) & 1 ? 0xffffu : 0u) | ((there >> (2 * g + 1)) & 1 ? 0xffff0000u : 0u);
-                if (((seen & 0xffffu) && ((nan >> (2 * g)) & 1)) || ((seen >> 16) && ((nan >> (2 * g + 1)) & 1))) spoilt |= 1;
-                if (((seen & 0xffffu) && ((nan >> (2 * g + 8)) & 1)) || ((seen >> 16) && ((nan >> (2 * g + 9)) & 1))) spoilt |= 2;
+                if (((seen & 0xffffu) && ((k_nan >> (2 * g)) & 1)) || ((seen >> 16) && ((k_nan >> (2 * g + 1)) & 1))) spoilt |= 1;
+                if (((seen & 0xffffu) && ((v_nan >> (2 * g)) & 1)) || ((seen >> 16) && ((v_nan >> (2 * g + 1)) & 1))) spoilt |= 2;
                 if (__all_sync(0xffffffffu, seen == 0xffffffffu)) continue;
                 uint32_t v[32];
                 ptx::tmem_ld32(ts + 32 * g, v);
@@ -445,17 +449,20 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
             }
             tmem_wait_st();
         }
-        uint32_t p[64];
+        uint32_t p[32];
         float sum;
 #pragma unroll 1
         for (int again = 0; again < 2; ++again) {
-            const float base = m == -INFINITY ? 0.0f : m, top = kv_prompt_weights(ts, info, factor, base, p, sum);
+            const float base = m == -INFINITY ? 0.0f : m, top = kv_prompt_weights(ts, info + 4 * b, factor, base, p, sum);
             const bool raise = m == -INFINITY ? top > -INFINITY : top > 8.0f;
             if (again || !__any_sync(0xffffffffu, raise)) break;
             const bool more = raise || top > 0.0f;    // (a row that has grown at all goes along)
             const float to_m = base + top, f = more ? (m == -INFINITY ? 0.0f : ex2(m - to_m)) : 1.0f;
             if (more) { l *= f; m = to_m; }
             if (count > 0) {
+                // the half before is in the sums (the one before that was, or this one's scores would not have had room)
+                if (!kv_wait(a, bar.pv_done(x), (uint32_t)(count - 1) & 1u, abort_flag)) return;
+                ptx::tc_fence_after();
 #pragma unroll 1
                 for (int g = 0; g < DP / 16; ++g) {
                     uint32_t v[16];
@@ -469,11 +476,11 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
         }
         l += sum;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) tmem_st16(ts + g * 16, p + 16 * g);
+        for (int g = 0; g < 2; ++g) tmem_st16(ts + g * 16, p + 16 * g);
         tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar.p_full(x));
+        if (lane == 0) ptx::mbar_arrive(bar.p_full(x, b));
         ++count;
     }
     if (count > 0) {
@@ -534,7 +541,8 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(bar.k_full(i), 7); ptx::mbar_init(bar.v_full(i), 7);
             ptx::mbar_init(bar.k_empty(i), 1); ptx::mbar_init(bar.v_empty(i), 1);
-            ptx::mbar_init(bar.s_full(i), 1); ptx::mbar_init(bar.p_full(i), 4); ptx::mbar_init(bar.o_full(i), 1);
+            for (int b = 0; b < 2; ++b) { ptx::mbar_init(bar.s_full(i, b), 1); ptx::mbar_init(bar.p_full(i, b), 4); }
+            ptx::mbar_init(bar.pv_done(i), 1); ptx::mbar_init(bar.o_full(i), 1);
         }
         for (int i = 0; i < F::RING; ++i) ptx::mbar_init(bar.info_full(i), 1);
         ptx::mbar_init(bar.q_full(), 7); ptx::mbar_init(bar.drained(), 1);
