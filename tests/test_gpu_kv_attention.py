@@ -243,3 +243,21 @@ def test_a_prompts_cta_gives_up(ctx, zb, cta):
     for _ in range(2):
         got = run(*args)
         assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+LONG = [([1], [20000], 8, 2, 64, 16, "bf16"), ([1], [33000], 4, 1, 128, 32, "f16"), ([3], [17001], 16, 1, 128, 64, "bf16"), ([1], [16400], 3, 1, 80, 128, "f32"), ([1, 2], [40000, 100], 5, 1, 96, 256, "bf16"),
+        ([1], [18000], 2, 1, 256, 32, "f16"), ([2], [25000], 8, 1, 112, 16, "f32")]
+
+
+@pytest.mark.parametrize("new,lengths,heads,kv_heads,dim,page,kind", LONG)
+def test_long_contexts_with_and_without_a_workspace(ctx, zb, new, lengths, heads, kv_heads, dim, page, kind):
+    """Few tiles of long contexts go through the arena; a context whose arena must not grow has its clusters."""
+    check(ctx, zb, new, lengths, heads, kv_heads, dim, page, kind)
+    assert ctx.last_kernel() == "kv_attention_join_kernel"
+    tight = zb.Context(0, arena_bytes=4096)
+    try:
+        tight.set_arena_limit(4096)
+        check(tight, zb, new, lengths, heads, kv_heads, dim, page, kind)
+        assert tight.last_kernel() == "kv_attention_kernel"
+    finally:
+        tight.close()

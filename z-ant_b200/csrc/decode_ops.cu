@@ -155,12 +155,19 @@ int32_t zant_b200_kv_cache_attention(zant_ctx* ctx, const zant_kv_cache* cache, 
         Stager s(ctx);
         const KvSlots slots(s, cache, codes, scales, table, seqs, width, lengths, offsets, false);
         const int iq = s.in(q, q_bytes), io = s.inout(out, out_bytes), il = s.inout(lse, rows * heads * 4);
-        ZB_TRY(s.commit());
         KvAttendArgs a{};
+        a.c = slots.args(s, cache, rows, seqs, width);       // (sizes; pointers again when all is in place)
+        a.heads = (int)heads; a.group = (int)group; a.q_type = dtype; a.window = window; a.sinks = sinks;
+        // a workspace in the arena, unless the call is captured or the arena must not grow that far
+        size_t work = kv_work_bytes(ctx, a);
+        if (work && (stream_capturing(ctx) || (ctx->arena_limit && !s.holds(work + kArenaAlign)))) work = 0;
+        const int iw = work ? s.scratch(work) : -1;
+        ZB_TRY(s.commit());
         a.c = slots.args(s, cache, rows, seqs, width);
-        a.q = s.ptr<void>(iq); a.q_stride = (long long)q_stride; a.heads = (int)heads; a.group = (int)group; a.q_type = dtype;
+        a.q = s.ptr<void>(iq); a.q_stride = (long long)q_stride;
         a.out = s.ptr<void>(io); a.out_stride = (long long)out_stride; a.lse = s.ptr<float>(il);
-        a.scale_log2 = scale * kLog2e; a.window = window; a.sinks = sinks;
+        a.scale_log2 = scale * kLog2e;
+        a.work = work ? s.ptr<float>(iw) : nullptr; a.work_bytes = work;
         a.wide_q = whole_blocks(a.q, q_stride, esz); a.wide_out = whole_blocks(a.out, out_stride, esz);
         ZB_TRY(run_kv_attention(ctx, a));
         return s.finish();

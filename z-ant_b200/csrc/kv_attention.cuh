@@ -42,6 +42,7 @@ struct KvAttendArgs {
     bool wide_q, wide_out;                            // q, out in whole 16-byte blocks
     int more_rows_than, rows_up_to;                   // sequences with more rows of a key head than the first, up to the second, are the kernel's
     int parts, tiles_each;                            // CTAs of a tile; tiles of each sequence (0: by its rows)
+    float* work; size_t work_bytes;                   // a workspace, if there is one: a tile's CTAs leave their sums there, and need not be a cluster
     int* status; long long wait_budget; int give_up;  // give_up: self test, a CTA whose first wait counts as run out (-1: none)
 };
 
@@ -168,7 +169,7 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
     extern __shared__ __align__(1024) uint8_t smem[];
     const KvArgs& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l4 = lane >> 2, c4 = lane & 3, P = a.parts, W = blockDim.x >> 5;
-    const int rank = P > 1 ? (int)ptx::cluster_rank() : 0;
+    const int rank = a.work ? (int)(blockIdx.x % (unsigned)P) : (P > 1 ? (int)ptx::cluster_rank() : 0);
     uint2* qs = reinterpret_cast<uint2*>(smem + F::big(W));
     float* stat = reinterpret_cast<float*>(smem + F::big(W) + F::Q_BYTES);       // [warp][row]: m, l, scale
     float* joined = stat + 3 * W * F::ROWS;           // [row]: m, l of the CTA
@@ -549,6 +550,17 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         }
         *reinterpret_cast<float4*>(sums + r * F::PITCH + d) = v;       // (of warp 0's, which only this thread reads)
     }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, (int)DEV_ERR_WAIT_TIMEOUT);
+    if (a.work) {
+        __syncthreads();
+        float* to = a.work + (size_t)blockIdx.x * (F::ROWS * (DP + 2));
+        for (int e = threadIdx.x; e < rows * (DP / 4); e += blockDim.x) {
+            const int r = e / (DP / 4), d = (e % (DP / 4)) * 4;
+            if (joined[2 * r + 1] != 0.0f) *reinterpret_cast<float4*>(to + r * DP + d) = *reinterpret_cast<const float4*>(sums + r * F::PITCH + d);
+        }
+        if (threadIdx.x < 2 * rows) to[F::ROWS * DP + threadIdx.x] = joined[threadIdx.x];
+        return;
+    }
     if (P > 1) {
         __syncwarp();
         ptx::cluster_arrive();
@@ -590,12 +602,63 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         kv_store(a.out, a.q_type, at + 2, v.z * inv); kv_store(a.out, a.q_type, at + 3, v.w * inv);
         if (a.lse && d == 0) a.lse[token * a.heads + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
     }
-    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, (int)DEV_ERR_WAIT_TIMEOUT);
     if (P > 1) {
         __syncwarp();
         ptx::cluster_arrive();
         ptx::cluster_wait();                          // nobody leaves while its sums are read
     }
+}
+
+// The sums of a tile's CTAs in the workspace; a CTA has 4 dimensions of a row each thread.
+template <int DP, int NT>
+__global__ void __launch_bounds__(256) kv_attention_join_kernel(const __grid_constant__ KvAttendArgs a) {
+    constexpr int ROWS = 8 * NT, QUADS = DP / 4;
+    ptx::grid_start();
+    const KvArgs& c = a.c;
+    const int h = blockIdx.x % c.heads;
+    KvSeq q; int unit;
+    if (!kv_locate(c, blockIdx.x / c.heads, a.group, ROWS, 1, q, unit)) return;
+    const int row0 = unit * ROWS, rows = min(ROWS, q.n * a.group - row0);
+    const int e = blockIdx.y * 256 + threadIdx.x, r = e / QUADS, d = (e % QUADS) * 4;
+    if (r >= rows || d >= c.dim) return;
+    const float* part = a.work + (size_t)blockIdx.x * a.parts * (ROWS * (DP + 2));
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float top = -INFINITY, total = 0.0f;
+    constexpr int U = 8;                              // parts whose sums are under way
+    for (int p0 = 0; p0 < a.parts; p0 += U) {
+        float2 ml[U]; float4 s[U];
+        float to = top;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const float* from = part + (size_t)(p0 + i) * (ROWS * (DP + 2));
+            ml[i] = p0 + i < a.parts ? *reinterpret_cast<const float2*>(from + ROWS * DP + 2 * r) : make_float2(-INFINITY, 0.0f);
+            s[i] = ml[i].y != 0.0f ? *reinterpret_cast<const float4*>(from + r * DP + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            to = fmaxf(to, ml[i].x);
+        }
+        const float f = join_factor(top, total, to);
+        total = times(total, f);
+        v.x = times(v.x, f); v.y = times(v.y, f); v.z = times(v.z, f); v.w = times(v.w, f);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const float fp = join_factor(ml[i].x, ml[i].y, to);
+            total += times(ml[i].y, fp);
+            v.x += times(s[i].x, fp); v.y += times(s[i].y, fp); v.z += times(s[i].z, fp); v.w += times(s[i].w, fp);
+        }
+        top = to;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const int row = row0 + r;
+    const long long token = q.row + row / a.group, head = h * a.group + row % a.group, at = token * a.out_stride + head * c.dim + d;
+    kv_store(a.out, a.q_type, at, v.x * inv); kv_store(a.out, a.q_type, at + 1, v.y * inv);
+    kv_store(a.out, a.q_type, at + 2, v.z * inv); kv_store(a.out, a.q_type, at + 3, v.w * inv);
+    if (a.lse && d == 0) a.lse[token * a.heads + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+}
+
+// Bytes of a workspace that a call can use (0: none): few tiles, contexts of 16384 tokens and more.
+inline size_t kv_work_bytes(const zant_ctx* ctx, const KvAttendArgs& a) {
+    const long long reach = std::min((long long)a.c.width << a.c.page_log2, a.window > 0 ? (long long)a.window + a.sinks : 0x7fffffffffLL);
+    if (reach < 16384 || kv_units(a.c, a.group, 32, 1) * a.c.heads * 16 > 3LL * ctx->sm_count) return 0;
+    return (size_t)ctx->sm_count * 3 * 32 * ((a.c.dim <= 64 ? 64 : (a.c.dim <= 128 ? 128 : 256)) + 2) * 4;
 }
 
 // Codes as boxes of `rows` tokens of a page and head, `box` bytes each, zeros behind the head's end.
@@ -626,6 +689,13 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     int warps = 4, parts = 1;
     while (parts < 16 && ((items * parts * 2 <= slots && steps >= 8LL * parts) || (items * parts * 2 <= 3 * slots && steps >= 64LL * parts))) parts *= 2;
     if (items * parts <= ctx->sm_count && parts < 16 && steps >= (long long)parts * F::MOST_WARPS) warps = F::MOST_WARPS;
+    // Few tiles of long contexts: clusters of 16 leave most of the GPU idle (8 of them, one sequence of 131072: 113 us), so as many CTAs as it holds share a tile through the workspace and
+    // a second kernel joins them.
+    if (a.work) {
+        const long long most = std::min({slots / items, steps / (4 * 4), (long long)(a.work_bytes / (items * F::ROWS * (DP + 2) * 4))});
+        if (parts == 16 && most >= 24 && !a.tiles_each) { parts = (int)most; warps = 4; }
+        else a.work = nullptr;
+    }
     a.parts = parts;
     a.status = ctx->status_word;
     alignas(64) CUtensorMap k_map{}, v_map{};
@@ -636,12 +706,15 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     ZB_SMEM_ATTR(ctx, kernel, F::smem(F::MOST_WARPS));
     static std::atomic<unsigned long long> wide{0ull};
     const unsigned long long bit = 1ull << (ctx->device & 63);
-    if (parts > 8 && !(wide.load(std::memory_order_acquire) & bit)) {
+    if (parts > 8 && !a.work && !(wide.load(std::memory_order_acquire) & bit)) {
         ZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         wide.fetch_or(bit, std::memory_order_release);
     }
-    launch_cluster(ctx, kernel, dim3((unsigned)(items * parts)), 32 * warps, F::smem(warps), (unsigned)parts, a, k_map, v_map);
-    return check_launch(ctx, "kv_attention_kernel");
+    launch_cluster(ctx, kernel, dim3((unsigned)(items * parts)), 32 * warps, F::smem(warps), a.work ? 1u : (unsigned)parts, a, k_map, v_map);
+    ZB_TRY(check_launch(ctx, "kv_attention_kernel"));
+    if (!a.work) return ZANT_OK;
+    launch(ctx, kv_attention_join_kernel<DP, NT>, dim3((unsigned)items, F::ROWS * (DP / 4) / 256 ? F::ROWS * (DP / 4) / 256 : 1), 256, 0, a);
+    return check_launch(ctx, "kv_attention_join_kernel");
 }
 
 template <int DP, bool SPLIT>

@@ -6,8 +6,9 @@
 // Probabilities are what the program has made of its logits, so that everything here is exact but sums, which are fp64: products of
 // two fp32 numbers and differences fit 53 bits, and the border of a token in the running sum is off by 2^-53 of the whole, 2^29 times less than an fp32 sum's.
 //
-// Bound by memory: a sequence's own two rows are read once, in segments (16 a CTA, up to 8 CTAs a sequence) whose sums every CTA of the cluster gets; the CTA that
-// has the segment in which the border lies reads that one again.
+// Bound by memory: a sequence's own two rows are read once, in segments (16 a CTA, a warp each with 16 loads of a lane under way, up to 8 CTAs a sequence) whose sums every CTA of the
+// cluster gets; the CTA that has the segment in which the border lies reads that one again, each thread some neighbouring probabilities.  Rows start at any address (vocabularies are odd), so loads
+// are of single ones.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -28,10 +29,12 @@ struct VerifyArgs {
 };
 
 struct VerifyShared {
-    static constexpr int THREADS = 512, SEGS = 16;
+    static constexpr int THREADS = 512, SEGS = 16, PARTS = 8;
     double seg[SEGS];                                 // a warp's sums, of this CTA's part of the row
+    double all[SEGS * PARTS];
     double warp_sum[SEGS];
-    int n, begin, end, found, last;
+    double total, before;
+    int n, begin, end, mine, found, last;
 };
 
 template <typename T>
@@ -87,65 +90,94 @@ __global__ void __launch_bounds__(VerifyShared::THREADS) verify_drafts_kernel(co
     const double u = a.sample[s];
     for (int round = 0; round < 2; ++round) {
         const int v0 = seg_begin(part * Sh::SEGS + warp), v1 = seg_begin(part * Sh::SEGS + warp + 1);
+        constexpr int U = 8;
         double sum = 0.0;
-        for (int v = v0 + lane; v < v1; v += 32) sum += mass(v);
+        for (int v = v0 + lane; v < v1; v += 32 * U) {
+            float pv[U], qv[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) pv[i] = v + 32 * i < v1 ? as_float(p[v + 32 * i]) : 0.0f;
+            if (less && q) {
+#pragma unroll
+                for (int i = 0; i < U; ++i) qv[i] = v + 32 * i < v1 ? as_float(q[v + 32 * i]) : 0.0f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < U; ++i) qv[i] = less && v + 32 * i == given ? 1.0f : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const double r = (double)pv[i] - (double)qv[i];
+                sum += r > 0.0 && r < INFINITY ? r : 0.0;
+            }
+        }
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (lane == 0) sh.seg[warp] = sum;
         if (tid == 0) { sh.found = 0x7fffffff; sh.last = -1; }
         __syncthreads();
-        if (P > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); }
-        auto seg_sum = [&](int i) {
-            if (P == 1) return sh.seg[i];
-            double v;
-            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(ptx::cluster_addr(ptx::smem_u32(&sh.seg[i % Sh::SEGS]), (uint32_t)(i / Sh::SEGS))) : "memory");
-            return v;
-        };
-        double total = 0.0;
-        for (int i = 0; i < segs; ++i) total += seg_sum(i);
-        if (total == 0.0 && less && round == 0) {     // nothing is left of the target's row: the row itself
-            less = false;
+        if (P > 1) {
+            ptx::cluster_arrive(); ptx::cluster_wait();
+            if (tid < segs) {
+                double v;
+                asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(ptx::cluster_addr(ptx::smem_u32(&sh.seg[tid % Sh::SEGS]), (uint32_t)(tid / Sh::SEGS))) : "memory");
+                sh.all[tid] = v;
+            }
             __syncwarp();
-            if (P > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); }
-            __syncthreads();
-            continue;
+            ptx::cluster_arrive(); ptx::cluster_wait();       // nobody leaves, or goes on to its next sums, while its sums are read
+        } else if (tid < segs) sh.all[tid] = sh.seg[tid];
+        __syncthreads();
+        if (warp == 0) {
+            // each lane has neighbouring segments: where the running sum passes the border, and the last segment that holds anything
+            const int each = (segs + 31) / 32;
+            double own = 0.0;
+            for (int i = 0; i < each; ++i) own += lane * each + i < segs ? sh.all[lane * each + i] : 0.0;
+            double run = own;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) { const double o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
+            const double total = __shfl_sync(0xffffffffu, run, 31), border = u * total;
+            double sofar = run - own;
+            int mine = 0x7fffffff, filled = -1;
+            double mine_before = 0.0, filled_before = 0.0;
+            for (int i = 0; i < each && lane * each + i < segs; ++i) {
+                const double v = sh.all[lane * each + i];
+                if (v > 0.0) { filled = lane * each + i; filled_before = sofar; }
+                if (mine == 0x7fffffff && v > 0.0 && sofar + v > border) { mine = lane * each + i; mine_before = sofar; }
+                sofar += v;
+            }
+            int best = mine, most = filled;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) { best = min(best, __shfl_xor_sync(0xffffffffu, best, d)); most = max(most, __shfl_xor_sync(0xffffffffu, most, d)); }
+            if (best != 0x7fffffff ? mine == best : (most >= 0 && filled == most)) { sh.mine = best != 0x7fffffff ? best : most; sh.before = best != 0x7fffffff ? mine_before : filled_before; }
+            if (lane == 0) sh.total = total;
         }
-        const double border = u * total;
-        double before = 0.0, sofar = 0.0;
-        int mine = -1, filled = -1;                   // the segment in which the sum passes the border, the last one that holds anything
-        double filled_before = 0.0;
-        for (int i = 0; i < segs; ++i) {
-            const double v = seg_sum(i);
-            if (v > 0.0) { filled = i; filled_before = sofar; }
-            if (mine < 0 && sofar + v > border && v > 0.0) { mine = i; before = sofar; }
-            sofar += v;
-        }
-        if (mine < 0) { mine = filled; before = filled_before; }
-        if (P > 1) { __syncwarp(); ptx::cluster_arrive(); ptx::cluster_wait(); }     // nobody leaves while its sums are read
+        __syncthreads();
+        const double total = sh.total, border = u * total;
         if (total == 0.0) {
+            if (less && round == 0) { less = false; __syncthreads(); continue; }       // nothing is left of the target's row: the row itself
             if (part == 0 && tid == 0) { a.accepted[s] = n; a.next[s] = -1; }
             return;
         }
+        const int mine = sh.mine;
         if (mine / Sh::SEGS != part) return;
-        const int w0 = seg_begin(mine), w1 = seg_begin(mine + 1);
-        for (int v0b = w0; v0b < w1; v0b += Sh::THREADS) {
-            const int v = v0b + tid;
-            const double r = v < w1 ? mass(v) : 0.0;
-            double run = r;
+        const int w0 = seg_begin(mine), w1 = seg_begin(mine + 1), each = (w1 - w0 + Sh::THREADS - 1) / Sh::THREADS;
+        const int from = min(w1, w0 + tid * each), to = min(w1, from + each);
+        double own = 0.0;
+        for (int v = from; v < to; ++v) own += mass(v);
+        double run = own;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) { const double o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
-            if (lane == 31) sh.warp_sum[warp] = run;
-            __syncthreads();
-            double base = before, all = 0.0;
-            for (int i = 0; i < Sh::SEGS; ++i) { if (i < warp) base += sh.warp_sum[i]; all += sh.warp_sum[i]; }
-            if (r > 0.0) {
-                if (base + run > border) atomicMin(&sh.found, v);
-                atomicMax(&sh.last, v);
-            }
-            before += all;
-            __syncthreads();
-            if (sh.found != 0x7fffffff) break;
+        for (int d = 1; d < 32; d <<= 1) { const double o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
+        if (lane == 31) sh.warp_sum[warp] = run;
+        __syncthreads();
+        double sofar = sh.before + (run - own);
+        for (int i = 0; i < warp; ++i) sofar += sh.warp_sum[i];
+        int found = 0x7fffffff, last = -1;
+        for (int v = from; v < to; ++v) {
+            const double r = mass(v);
+            sofar += r;
+            if (r > 0.0) { last = v; if (found == 0x7fffffff && sofar > border) found = v; }
         }
+        if (found != 0x7fffffff) atomicMin(&sh.found, found);
+        if (last >= 0) atomicMax(&sh.last, last);
+        __syncthreads();
         if (tid == 0) { a.accepted[s] = n; a.next[s] = sh.found != 0x7fffffff ? sh.found : sh.last; }
         return;
     }
