@@ -5,7 +5,7 @@
 //   reading   c * s
 //
 // Both are bound by memory.  A CTA has one page of one head, keys or values: the new rows are read once for the maximum, which stays in the
-// CTA, and again from its own L1 for the codes (the first 16 values of each thread wait in registers instead).  Pages, not tokens, are what the grid
+// CTA, and their values wait in registers (kKvHold times 16 a thread, all under way at once; what is beyond is read again).  Pages, not tokens, are what the grid
 // counts, so that no other CTA writes the page or its scale.
 #pragma once
 #include <cuda_runtime.h>
@@ -84,6 +84,9 @@ __device__ __forceinline__ long long kv_page(const KvArgs& a, int s, int at) {
     return id >= 0 && id < a.pages ? id : -1;
 }
 
+// 16 values each that a thread holds of what it reads.
+template <typename T> constexpr int kKvHold = sizeof(T) == 2 ? 4 : 2;
+
 struct KvWriteArgs {
     KvArgs c;
     const void* x[2]; long long stride[2];            // keys, values
@@ -133,22 +136,36 @@ __global__ void __launch_bounds__(256) kv_cache_write_kernel(const __grid_consta
     const int at = (max(q.first, 0) >> c.page_log2) + unit, from = max(q.first, at << c.page_log2);
     const int to = min(q.first + q.n, (at + 1) << c.page_log2);
     if (from < 0 || from >= to) return;
-    const long long page = kv_page(c, q.s, at);
-    if (page < 0) return;
     const int begin = from & (c.page - 1), per_row = c.dim >> 4, units = (to - from) * per_row;
-    int8_t* codes = (kv ? c.v : c.k) + (page * c.heads + h) * c.page * c.dim;
-    float* scale = (kv ? c.v_scale : c.k_scale) + page * c.heads + h;
     const T* x = static_cast<const T*>(a.x[kv]) + (long long)(q.row + from - q.first) * a.stride[kv] + (long long)h * c.dim;
     const bool wide = a.wide[kv];
     auto load = [&](int u, uint32_t (&w)[W]) { const int t = u / per_row; kv_load16(x + t * a.stride[kv] + (u - t * per_row) * 16, wide, w); };
-    const float old = begin == 0 ? 0.0f : *scale;
-    uint32_t mine[W] = {};
+    constexpr int HOLD = kKvHold<T>;
+    uint32_t mine[HOLD][W];
     uint32_t m = 0;
-    for (int u = tid; u < units; u += threads) {
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+        if (tid + i * threads < units) load(tid + i * threads, mine[i]);
+        else {
+#pragma unroll
+            for (int z = 0; z < W; ++z) mine[i][z] = 0;
+        }
+    }
+    // (the page is looked up while the rows are on their way)
+    const long long page = kv_page(c, q.s, at);
+    if (page < 0) return;
+    int8_t* codes = (kv ? c.v : c.k) + (page * c.heads + h) * c.page * c.dim;
+    float* scale = (kv ? c.v_scale : c.k_scale) + page * c.heads + h;
+    const float old = begin == 0 ? 0.0f : *scale;
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i)
+#pragma unroll
+        for (int z = 0; z < W; ++z) m = C::top(m, mine[i][z]);
+    for (int u = tid + HOLD * threads; u < units; u += threads) {
         uint32_t w[W];
         load(u, w);
 #pragma unroll
-        for (int i = 0; i < W; ++i) { m = C::top(m, w[i]); if (u == tid) mine[i] = w[i]; }
+        for (int z = 0; z < W; ++z) m = C::top(m, w[z]);
     }
     m = kv_block_max(__float_as_uint(C::top_value(m)), part);
     const bool finite = m < 0x7f800000u && old == old;
@@ -160,18 +177,21 @@ __global__ void __launch_bounds__(256) kv_cache_write_kernel(const __grid_consta
     const RowScale k(s, big, inv, tiny);
     const bool none = !finite || k.none();
     const bool exactly = tiny || (sizeof(T) == 2 && (__float_as_uint(k.s) & 0xfffu) == 0);
-    for (int u = tid; u < units; u += threads) {
-        uint32_t w[W];
-        if (u == tid) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) w[i] = mine[i];
-        } else load(u, w);
+    auto write = [&](int u, const uint32_t (&w)[W]) {
         uint32_t out[4] = {0, 0, 0, 0};
         if (!none) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T); ++i) codes_of<T>(w + 4 * i, k, exactly, out + i * (4 / (int)sizeof(T)));
         }
         *reinterpret_cast<uint4*>(codes + (long long)begin * c.dim + u * 16) = make_uint4(out[0], out[1], out[2], out[3]);
+    };
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i)
+        if (tid + i * threads < units) write(tid + i * threads, mine[i]);
+    for (int u = tid + HOLD * threads; u < units; u += threads) {
+        uint32_t w[W];
+        load(u, w);
+        write(u, w);
     }
     if (finite && begin > 0 && s > old) {
         // The quotient of 64 bits is right at every border: 2 c s and (2 t + 1) s' are whole multiples of a unit with 33 bits at most.
@@ -217,33 +237,41 @@ __global__ void __launch_bounds__(256) kv_cache_read_kernel(const __grid_constan
     const int8_t* codes = (kv ? c.v : c.k) + block * c.page * c.dim + (long long)begin * c.dim;
     const float s = page < 0 ? 0.0f : (kv ? c.v_scale : c.k_scale)[block];
     T* out = static_cast<T*>(a.out[kv]) + (long long)(q.row + from - q.first) * a.stride[kv] + (long long)h * c.dim;
-    for (int u = tid; u < units; u += threads) {
-        const uint4 v = page < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(codes + u * 16);
-        const int8_t* b = reinterpret_cast<const int8_t*>(&v);
-        const int t = u / per_row;
-        T* to_row = out + t * a.stride[kv] + (u - t * per_row) * 16;
-        alignas(16) T y[16];
+    constexpr int HOLD = 4;
+    for (int u0 = tid; u0 < units; u0 += HOLD * threads) {
+        uint4 v[HOLD];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = kv_round<T>((float)b[i] * s);
-        if (a.wide[kv]) {
+        for (int i = 0; i < HOLD; ++i) v[i] = page >= 0 && u0 + i * threads < units ? *reinterpret_cast<const uint4*>(codes + (u0 + i * threads) * 16) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(to_row)[i] = reinterpret_cast<const uint4*>(y)[i];
-        } else {
+        for (int i = 0; i < HOLD; ++i) {
+            const int u = u0 + i * threads;
+            if (u >= units) break;
+            const int8_t* b = reinterpret_cast<const int8_t*>(&v[i]);
+            const int t = u / per_row;
+            T* to_row = out + t * a.stride[kv] + (u - t * per_row) * 16;
+            alignas(16) T y[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) to_row[i] = y[i];
+            for (int z = 0; z < 16; ++z) y[z] = kv_round<T>((float)b[z] * s);
+            if (a.wide[kv]) {
+#pragma unroll
+                for (int z = 0; z < (int)sizeof(T); ++z) reinterpret_cast<uint4*>(to_row)[z] = reinterpret_cast<const uint4*>(y)[z];
+            } else {
+#pragma unroll
+                for (int z = 0; z < 16; ++z) to_row[z] = y[z];
+            }
         }
     }
 }
 
-// Threads for a page's share of the new tokens, 16 values each.
-inline int kv_threads(const KvArgs& a) {
-    const long long tokens = std::min<long long>(a.page, ((long long)a.rows + a.seqs - 1) / a.seqs), units = tokens * (a.dim / 16);
+// Threads for a page's share of the new tokens, 16 values `hold` times each.
+inline int kv_threads(const KvArgs& a, int hold) {
+    const long long tokens = std::min<long long>(a.page, ((long long)a.rows + a.seqs - 1) / a.seqs), units = (tokens * (a.dim / 16) + hold - 1) / hold;
     return units <= 64 ? 64 : (units <= 128 ? 128 : 256);
 }
 
 inline int32_t run_kv_cache_write(zant_ctx* ctx, int32_t dtype, const KvWriteArgs& a) {
     const dim3 grid((unsigned)kv_units(a.c, 1, a.c.page, 2), (unsigned)a.c.heads, 2);
-    auto go = [&](auto kernel) { launch(ctx, kernel, grid, kv_threads(a.c), 0, a); return check_launch(ctx, "kv_cache_write_kernel"); };
+    auto go = [&](auto kernel) { launch(ctx, kernel, grid, kv_threads(a.c, dtype == ZANT_F32 ? 2 : 4), 0, a); return check_launch(ctx, "kv_cache_write_kernel"); };
     if (dtype == ZANT_F32) return go(kv_cache_write_kernel<float>);
     if (dtype == ZANT_F16) return go(kv_cache_write_kernel<__half>);
     return go(kv_cache_write_kernel<__nv_bfloat16>);
@@ -251,7 +279,7 @@ inline int32_t run_kv_cache_write(zant_ctx* ctx, int32_t dtype, const KvWriteArg
 
 inline int32_t run_kv_cache_read(zant_ctx* ctx, int32_t dtype, const KvReadArgs& a) {
     const dim3 grid((unsigned)kv_units(a.c, 1, a.c.page, 2), (unsigned)a.c.heads, a.out[0] && a.out[1] ? 2 : 1);
-    auto go = [&](auto kernel) { launch(ctx, kernel, grid, kv_threads(a.c), 0, a); return check_launch(ctx, "kv_cache_read_kernel"); };
+    auto go = [&](auto kernel) { launch(ctx, kernel, grid, kv_threads(a.c, 4), 0, a); return check_launch(ctx, "kv_cache_read_kernel"); };
     if (dtype == ZANT_F32) return go(kv_cache_read_kernel<float>);
     if (dtype == ZANT_F16) return go(kv_cache_read_kernel<__half>);
     return go(kv_cache_read_kernel<__nv_bfloat16>);
