@@ -529,3 +529,63 @@ pub fn token_logprobs_lean(comptime T: type, logits: *const Tensor(T), tokens: *
     }
     try check(zant_b200_token_logprobs(context(), rowTypeOf(T), logits.data.ptr, rows, logits.shape[1], 0, tokens.data.ptr, logprob.data.ptr, entropy.data.ptr, @intCast(top), if (top_ids) |t| t.data.ptr else null, if (top_logprobs) |t| t.data.ptr else null));
 }
+
+// ------------------------------------------------------------------------------------------
+// A decoder's key-value cache in 8 bits, attention over it, and the check of drafted tokens.  No reference counterpart; zant_b200.h states them.
+// ------------------------------------------------------------------------------------------
+pub const KvCacheData = extern struct { k: [*]i8, k_scale: [*]f32, v: [*]i8, v_scale: [*]f32, pages: usize, heads: usize, page: usize, dim: usize };
+
+extern fn zant_b200_kv_cache_write(ctx: ?*Ctx, cache: *const KvCacheData, dtype: i32, k: *const anyopaque, k_stride: usize, v: *const anyopaque, v_stride: usize, rows: usize, table: [*]const i32, seqs: usize, width: usize, lengths: [*]const i32, offsets: ?[*]const i32) i32;
+extern fn zant_b200_kv_cache_read(ctx: ?*Ctx, cache: *const KvCacheData, dtype: i32, k: ?*anyopaque, k_stride: usize, v: ?*anyopaque, v_stride: usize, rows: usize, table: [*]const i32, seqs: usize, width: usize, lengths: [*]const i32, offsets: ?[*]const i32) i32;
+extern fn zant_b200_kv_cache_attention(ctx: ?*Ctx, cache: *const KvCacheData, dtype: i32, q: *const anyopaque, q_stride: usize, rows: usize, heads: usize, table: [*]const i32, seqs: usize, width: usize, lengths: [*]const i32, offsets: ?[*]const i32, scale: f32, window: i32, sinks: i32, out: *anyopaque, out_stride: usize, lse: ?[*]f32) i32;
+extern fn zant_b200_verify_drafts(ctx: ?*Ctx, dtype: i32, target: *const anyopaque, target_stride: usize, drafted: ?*const anyopaque, drafted_stride: usize, vocab: usize, tokens: [*]const i32, drafts: usize, offsets: ?[*]const i32, seqs: usize, accept: [*]const f32, sample: [*]const f32, accepted: [*]i32, next: [*]i32) i32;
+
+/// The arrays of a cache: codes [pages, heads, page, dim], scales [pages, heads].
+pub fn kv_cache_of(k: *const Tensor(i8), k_scale: *const Tensor(f32), v: *const Tensor(i8), v_scale: *const Tensor(f32)) !KvCacheData {
+    if (k.shape.len != 4 or v.shape.len != 4) return TensorError.InvalidRank;
+    if (k_scale.size != k.shape[0] * k.shape[1] or v_scale.size != k_scale.size or v.size != k.size) return TensorMathError.InputTensorsWrongShape;
+    return KvCacheData{ .k = k.data.ptr, .k_scale = k_scale.data.ptr, .v = v.data.ptr, .v_scale = v_scale.data.ptr, .pages = k.shape[0], .heads = k.shape[1], .page = k.shape[2], .dim = k.shape[3] };
+}
+
+fn checkSequences(table: *const Tensor(i32), lengths: *const Tensor(i32), offsets: ?*const Tensor(i32)) !void {
+    if (table.shape.len != 2) return TensorError.InvalidRank;
+    if (lengths.size != table.shape[0]) return TensorMathError.InputTensorDifferentSize;
+    if (offsets) |o| if (o.size != table.shape[0] + 1) return TensorMathError.InputTensorDifferentSize;
+}
+
+/// Keys and values of new tokens [rows, heads * dim] into the cache's pages.
+pub fn kv_cache_write_lean(comptime T: type, cache: *const KvCacheData, k: *const Tensor(T), v: *const Tensor(T), table: *const Tensor(i32), lengths: *const Tensor(i32), offsets: ?*const Tensor(i32)) !void {
+    if (k.shape.len != 2 or v.shape.len != 2) return TensorError.InvalidRank;
+    if (k.shape[1] != cache.heads * cache.dim or v.shape[1] != k.shape[1] or v.shape[0] != k.shape[0]) return TensorMathError.InputTensorsWrongShape;
+    try checkSequences(table, lengths, offsets);
+    try check(zant_b200_kv_cache_write(context(), cache, rowTypeOf(T), k.data.ptr, 0, v.data.ptr, 0, k.shape[0], table.data.ptr, table.shape[0], table.shape[1], lengths.data.ptr, if (offsets) |o| o.data.ptr else null));
+}
+
+/// The last cached tokens of each sequence as rows [rows, heads * dim].
+pub fn kv_cache_read_lean(comptime T: type, cache: *const KvCacheData, k: *Tensor(T), v: *Tensor(T), table: *const Tensor(i32), lengths: *const Tensor(i32), offsets: ?*const Tensor(i32)) !void {
+    if (k.shape.len != 2 or v.shape.len != 2) return TensorError.InvalidRank;
+    if (k.shape[1] != cache.heads * cache.dim or v.shape[1] != k.shape[1] or v.shape[0] != k.shape[0]) return TensorMathError.OutputTensorDifferentSize;
+    try checkSequences(table, lengths, offsets);
+    try check(zant_b200_kv_cache_read(context(), cache, rowTypeOf(T), k.data.ptr, 0, v.data.ptr, 0, k.shape[0], table.data.ptr, table.shape[0], table.shape[1], lengths.data.ptr, if (offsets) |o| o.data.ptr else null));
+}
+
+/// Attention of new tokens q [rows, heads * dim] over their sequences; window 0 is none.
+pub fn kv_cache_attention_lean(comptime T: type, cache: *const KvCacheData, q: *const Tensor(T), table: *const Tensor(i32), lengths: *const Tensor(i32), offsets: ?*const Tensor(i32), scale: f32, window: i32, sinks: i32, out: *Tensor(T)) !void {
+    if (q.shape.len != 2 or out.shape.len != 2) return TensorError.InvalidRank;
+    if (out.shape[0] != q.shape[0] or out.shape[1] != q.shape[1]) return TensorMathError.OutputTensorDifferentSize;
+    if (cache.dim == 0 or q.shape[1] % cache.dim != 0) return TensorMathError.InputTensorsWrongShape;
+    try checkSequences(table, lengths, offsets);
+    try check(zant_b200_kv_cache_attention(context(), cache, rowTypeOf(T), q.data.ptr, 0, q.shape[0], q.shape[1] / cache.dim, table.data.ptr, table.shape[0], table.shape[1], lengths.data.ptr, if (offsets) |o| o.data.ptr else null, scale, window, sinks, out.data.ptr, 0, null));
+}
+
+/// How many drafted tokens of each sequence stand, and the token behind them; `drafted` null: the draft model was certain.
+pub fn verify_drafts_lean(comptime T: type, target: *const Tensor(T), drafted: ?*const Tensor(T), tokens: *const Tensor(i32), accept: *const Tensor(f32), sample: *const Tensor(f32), offsets: ?*const Tensor(i32), accepted: *Tensor(i32), next: *Tensor(i32)) !void {
+    if (target.shape.len != 2) return TensorError.InvalidRank;
+    const drafts = tokens.size;
+    const seqs = sample.size;
+    if (target.shape[0] != drafts + seqs or accept.size != drafts) return TensorMathError.InputTensorsWrongShape;
+    if (drafted) |d| if (d.shape.len != 2 or d.shape[0] != drafts or d.shape[1] != target.shape[1]) return TensorMathError.InputTensorsWrongShape;
+    if (offsets) |o| if (o.size != seqs + 1) return TensorMathError.InputTensorDifferentSize;
+    if (accepted.size != seqs or next.size != seqs) return TensorMathError.OutputTensorDifferentSize;
+    try check(zant_b200_verify_drafts(context(), rowTypeOf(T), target.data.ptr, 0, if (drafted) |d| d.data.ptr else null, 0, target.shape[1], tokens.data.ptr, drafts, if (offsets) |o| o.data.ptr else null, seqs, accept.data.ptr, sample.data.ptr, accepted.data.ptr, next.data.ptr));
+}
