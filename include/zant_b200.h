@@ -192,8 +192,8 @@ int32_t zant_b200_measure_int8_peak_sustained(zant_ctx* ctx, double seconds, dou
 int32_t zant_b200_selftest_bounded_wait(zant_ctx* ctx, uint32_t budget_us);
 
 /* Failure-path self test (no reference counterpart).  In the next launch of the kernel that runs an inverted residual
- * block of a plan on bands of rows (few images), or of a tensor-memory kernel of qmatmul_scaled and qmatmul_grouped, CTA
- * `cta`, modulo the launch's CTAs, acts as if its first bounded wait had run out: it fetches no further weights and gives
+ * block of a plan on bands of rows (few images), of a tensor-memory kernel of qmatmul_scaled and qmatmul_grouped,
+ * or of a kernel of kv_cache_attention, CTA `cta`, modulo the launch's CTAs, acts as if its first bounded wait had run out: it fetches no further weights and gives
  * up later waits soon.  That run reports
  * ZANT_E_DEVICE_TIMEOUT as zant_b200_selftest_bounded_wait describes, and the runs after it are right again.
  * A negative `cta` disarms it.  A launch that is being captured counts: each replay of it gives up. */
@@ -627,7 +627,7 @@ int32_t zant_b200_token_logprobs(zant_ctx* ctx, int32_t dtype, const void* logit
  * compute.  The same rules hold (strides, alignment, capture, calls with no rows).
  *
  * The cache is pages of tokens.  Codes are [pages, heads, page, dim], one scale for each page and head is [pages, heads], keys and values alike; a cached value is
- * code * scale.  `page` is 16, 32, 64, 128 or 256 tokens (else InvalidInput), `dim` a multiple of 16 up to 256 (else UnsupportedDimension).  Codes in device memory
+ * code * scale.  Scales are not negative.  `page` is 16, 32, 64, 128 or 256 tokens (else InvalidInput), `dim` a multiple of 16 up to 256 (else UnsupportedDimension).  Codes in device memory
  * start at a multiple of 16 bytes (InvalidInput).
  *
  * The sequences of a call: page i of sequence s is table[s, i] (table [seqs, width], int32); lengths[s] tokens of it are in the cache, the call's new ones

@@ -226,15 +226,16 @@ def test_host_arrays(ctx, zb):
     within(ls.astype(np.float64), lse, lse_off)
 
 
+@pytest.mark.parametrize("new,length", [(300, 600), (2, 600), (1, 20000)])
 @pytest.mark.parametrize("cta", [0, 3, 10007])
-def test_a_prompts_cta_gives_up(ctx, zb, cta):
-    """A CTA whose first wait runs out: every warp of it comes to the kernel's end, the call reports the time-out, and the calls behind it are right."""
+def test_a_cta_gives_up(ctx, zb, new, length, cta):
+    """A CTA whose first wait runs out: every warp of it comes to the kernel's end (and its cluster), the call reports the time-out, and the calls behind it are right."""
     import torch
     rng = np.random.default_rng(8)
-    cache = ref.Cache(20, 2, 64, 128, rng)
-    table = tables(rng, 20, 64, [600, 300])
-    q = as_kind(torch, rng.standard_normal((600, 4, 128)), "bf16")
-    args = (ctx, zb, torch, cache, q, table, [600, 300], [0, 500, 600], "bf16")
+    cache = ref.Cache(2 * (length // 64 + 1), 2, 64, 128, rng)
+    table = tables(rng, cache.pages, 64, [length, length // 2])
+    q = as_kind(torch, rng.standard_normal((2 * new, 4, 128)), "bf16")
+    args = (ctx, zb, torch, cache, q, table, [length, length // 2], None, "bf16")
     want = run(*args)
     ctx.selftest_give_up(cta)
     with pytest.raises(zb.ZantError) as e:

@@ -355,7 +355,8 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
             vsc[z] = z == 0 || two ? __shfl_sync(0xffffffffu, cur.v[z], i & 31) : vsc[0];
             ok[z] = (cur.there[z] >> (i & 31)) & 1u;
         }
-        if (!__all_sync(0xffffffffu, ptx::mbar_wait(full + 8 * stage, phase, abort_flag))) {
+        if (!__all_sync(0xffffffffu, (int)blockIdx.x != a.give_up && ptx::mbar_wait(full + 8 * stage, phase, abort_flag))) {
+            *abort_flag = 1;
             // given up: the copies on their way land before the ring is something else's (or are given up too)
             for (int z = 0; z < D && k + z * stride_k < steps.total; ++z) {
                 volatile int no = 0;
@@ -698,6 +699,8 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     }
     a.parts = parts;
     a.status = ctx->status_word;
+    a.give_up = ctx->give_up_cta < 0 ? -1 : (int)(ctx->give_up_cta % (items * parts));
+    ctx->give_up_cta = -1;
     alignas(64) CUtensorMap k_map{}, v_map{};
     const int box_rows = std::min(a.c.page, F::STEP);
     ZB_TRY(encode_kv_map(&k_map, a.c.k, a.c, F::BOX, box_rows));

@@ -10,7 +10,7 @@
 // lv = log2(vs / VS) in [-24, 0], so that what is rounded to f16 is at most 2^14 (the maximum is raised when one of a warp's rows has grown by 2^8, and then what has been summed is
 // rescaled), and what is lost below f16's least numbers is 2^-31 of the largest weight.  The sum of the weights takes the factor out again, once for 16 tokens.
 //
-//   warps 0 .. 3, 4 .. 7  rows of the first and the second tile      12  TMEM owner, MMA issuer      8 .. 11, 13 .. 15  q and codes to f16, scales
+//   warps 0 .. 3, 4 .. 7  q to f16, rows of the first and the second tile      12  TMEM owner, MMA issuer      8 .. 11, 13 .. 15  codes to f16, scales
 // Registers: 136 for the rows' threads, 120 for others (setmaxnreg; 128 each at launch).
 #pragma once
 #include <cuda_fp16.h>
@@ -147,12 +147,13 @@ template <typename F>
 struct KvConvert {
     static constexpr int WARPS = 7, LPR = F::LPR, GROUPS = 128 / F::TPL, N = (GROUPS + WARPS - 1) / WARPS;
     uint4 w[N];
-    // blocks: where 16 tokens each lie in the cache, in units of 16 tokens (-1: nowhere); mine: the lane's 16 bytes are dimensions of the head
-    __device__ __forceinline__ void load(const int8_t* codes, const int* blocks, int warp, int dim, int in_group, int column, bool mine) {
+    // block_of(i): where the i-th 16 tokens lie in the cache, in units of 16 tokens (-1: nowhere); mine: the lane's 16 bytes are dimensions of the head
+    template <typename B>
+    __device__ __forceinline__ void load(const int8_t* codes, B&& block_of, int warp, int dim, int in_group, int column, bool mine) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int group = i * WARPS + warp, tok = group * F::TPL;
-            const int block = GROUPS % WARPS == 0 || group < GROUPS ? blocks[tok >> 4] : -1;
+            const int block = GROUPS % WARPS == 0 || group < GROUPS ? block_of(tok >> 4) : -1;
             const int8_t* p = codes + (unsigned long long)(unsigned)block * (unsigned)(16 * dim) + (unsigned)(((tok & 15) + in_group) * dim + column);
             w[i] = make_uint4(0, 0, 0, 0);
             if (mine && block >= 0) w[i] = ptx::ld_global_once(reinterpret_cast<const uint4*>(p));     // (past L1)
@@ -192,60 +193,17 @@ __device__ __forceinline__ int kv_prompt_block(const KvArgs& c, const KvPromptTi
     return (int)((((unsigned)page * (unsigned)c.heads + (unsigned)tile.h) << (c.page_log2 - 4)) + (unsigned)((t & (c.page - 1)) >> 4));
 }
 
-// ---- warps 8 .. 11 and 13 .. 15: the largest scale of V; q; K, V and what each step's pages say.  Codes are on their way a step ahead.
+// ---- warps 0 .. 7, while the first codes are on their way: q as f16, a power of two for each row
 template <typename F>
-__device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
+__device__ __forceinline__ void kv_prompt_queries(const KvAttendArgs& a, const KvPromptTile& tile, const KvPromptBars& bar, uint8_t* smem) {
     constexpr int LPR = F::LPR, TPL = F::TPL;
     const KvArgs& c = a.c;
-    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - ((threadIdx.x >> 5) < 12 ? 8 : 9), pl = c.page_log2;
-    float* row_factor = reinterpret_cast<float*>(smem + F::OFF_REST);
-    float* info = reinterpret_cast<float*>(smem + F::OFF_INFO);
-    float* part = reinterpret_cast<float*>(smem + F::OFF_MAX);
-    // the lane's 16 dimensions of a token: their place in its row of codes, and in an operand's
-    const int which = lane % LPR, in_group = lane / LPR, column = which * 16, chunk = (which & 3) * 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, which = lane % LPR, in_group = lane / LPR, column = which * 16, chunk = (which & 3) * 2;
     const bool mine = column < c.dim;
+    float* row_factor = reinterpret_cast<float*>(smem + F::OFF_REST);
     uint8_t* operand = smem + (which >> 2) * F::BLOCK;
-    KvConvert<F> kc, vc;
-    // The last warp (it has the fewest tokens) says what a step's pages are like, two steps before the others ask: in the place of step k - 6 then, whose weights have been taken, or
-    // step k - 1's K would not have had room.
-    int page = -1;
-    float ks = 0.0f, vsc = 0.0f;
-    auto look = [&](int k) {                          // on their way
-        page = kv_prompt_page(a, tile, steps, k);
-        ks = page >= 0 ? c.k_scale[(long long)page * c.heads + tile.h] : 0.0f;
-        vsc = page >= 0 ? c.v_scale[(long long)page * c.heads + tile.h] : 0.0f;
-    };
-    auto tell = [&](int k, float vs) {
-        float* i = info + (k & (F::RING - 1)) * F::INFO;
-        const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
-        const bool k_nan = ks != ks, v_nan = vsc != vsc;
-        const unsigned there = __ballot_sync(0xffffffffu, page >= 0), bad_k = __ballot_sync(0xffffffffu, k_nan), bad_v = __ballot_sync(0xffffffffu, v_nan);
-        if (lane < 8) {
-            i[lane] = k_nan ? 0.0f : fabsf(ks); i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 6.0f);
-            reinterpret_cast<int*>(i)[28 + lane] = kv_prompt_block(c, tile, steps, k, page);
-        }
-        if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8)); }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar.info_full(k & (F::RING - 1)));
-    };
-    auto blocks = [&](int k) { return reinterpret_cast<const int*>(info + (k & (F::RING - 1)) * F::INFO) + 28; };
-    if (warp == 6) look(0);
-
-    float top = 0.0f;
-    if (steps.total > 0) {
-        const int low = tile.low0, high = tile.last(), from = a.window > 0 ? max(low - a.window + 1, 0) >> pl : 0, to = (high >> pl) + 1;
-        const int sink_pages = a.sinks > 0 ? min(((a.sinks - 1) >> pl) + 1, from) : 0;
 #pragma unroll 2
-        for (int i = warp * 32 + lane; i < sink_pages + to - from; i += 224) {
-            const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
-            if (id >= 0) top = fmaxf(top, fabsf(c.v_scale[id * c.heads + tile.h]));
-        }
-    }
-    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-    if (lane == 0) part[warp] = top;
-
-#pragma unroll 1
-    for (int g = warp; g < F::ROWS / TPL; g += 7) {
+    for (int g = warp; g < F::ROWS / TPL; g += 8) {
         const int r = g * TPL + in_group, row = tile.row0 + r;
         const bool there = r < tile.rows && mine;
         float v[16];
@@ -280,6 +238,64 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         *reinterpret_cast<uint4*>(to + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
     }
     kv_written(bar.q_full());
+}
+
+// ---- warps 8 .. 11 and 13 .. 15: the largest scale of V; K, V and what each step's pages say.  Codes are on their way a step ahead.
+template <typename F>
+__device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
+    constexpr int LPR = F::LPR;
+    const KvArgs& c = a.c;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - ((threadIdx.x >> 5) < 12 ? 8 : 9), pl = c.page_log2;
+    float* info = reinterpret_cast<float*>(smem + F::OFF_INFO);
+    float* part = reinterpret_cast<float*>(smem + F::OFF_MAX);
+    // the lane's 16 dimensions of a token: their place in its row of codes, and in an operand's
+    const int which = lane % LPR, in_group = lane / LPR, column = which * 16, chunk = (which & 3) * 2;
+    const bool mine = column < c.dim;
+    uint8_t* operand = smem + (which >> 2) * F::BLOCK;
+    KvConvert<F> kc, vc;
+    // The last warp (it has the fewest tokens) says what a step's pages are like, two steps before the others ask: in the place of step k - 6 then, whose weights have been taken, or
+    // step k - 1's K would not have had room.
+    int page = -1;
+    float ks = 0.0f, vsc = 0.0f;
+    auto look = [&](int k) {                          // on their way
+        page = kv_prompt_page(a, tile, steps, k);
+        ks = page >= 0 ? c.k_scale[(long long)page * c.heads + tile.h] : 0.0f;
+        vsc = page >= 0 ? c.v_scale[(long long)page * c.heads + tile.h] : 0.0f;
+    };
+    auto tell = [&](int k, float vs) {
+        float* i = info + (k & (F::RING - 1)) * F::INFO;
+        const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
+        const bool k_nan = ks != ks, v_nan = vsc != vsc;
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0), bad_k = __ballot_sync(0xffffffffu, k_nan), bad_v = __ballot_sync(0xffffffffu, v_nan);
+        if (lane < 8) {
+            i[lane] = k_nan ? 0.0f : fabsf(ks); i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 6.0f);
+            reinterpret_cast<int*>(i)[28 + lane] = kv_prompt_block(c, tile, steps, k, page);
+        }
+        if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8)); }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar.info_full(k & (F::RING - 1)));
+    };
+    auto blocks = [&](int k) { return [=](int i) { return reinterpret_cast<const int*>(info + (k & (F::RING - 1)) * F::INFO)[28 + i]; }; };
+    // the first step's codes before anything else
+    look(0);
+    const int first = kv_prompt_block(c, tile, steps, 0, page);
+    auto first_block = [&](int i) { return __shfl_sync(0xffffffffu, first, i & 7); };
+    kc.load(c.k, first_block, warp, c.dim, in_group, column, mine);
+    vc.load(c.v, first_block, warp, c.dim, in_group, column, mine);
+
+    float top = 0.0f;
+    if (steps.total > 0) {
+        const int low = tile.low0, high = tile.last(), from = a.window > 0 ? max(low - a.window + 1, 0) >> pl : 0, to = (high >> pl) + 1;
+        const int sink_pages = a.sinks > 0 ? min(((a.sinks - 1) >> pl) + 1, from) : 0;
+#pragma unroll 2
+        for (int i = warp * 32 + lane; i < sink_pages + to - from; i += 224) {
+            const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
+            if (id >= 0) top = fmaxf(top, fabsf(c.v_scale[id * c.heads + tile.h]));
+        }
+    }
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if (lane == 0) part[warp] = top;
+
     ptx::named_barrier_sync(1, 224);                  // (in front of any wait that may be given up)
     const float vs = kv_prompt_top(part);
     if (warp == 6) {
@@ -288,9 +304,6 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         tell(1, vs);
         look(2);
     }
-    if (!kv_wait(a, bar.info_full(0), 0, abort_flag)) return;
-    kc.load(c.k, blocks(0), warp, c.dim, in_group, column, mine);
-    vc.load(c.v, blocks(0), warp, c.dim, in_group, column, mine);
 
 #pragma unroll 1
     for (int k = 0; k < steps.total; ++k) {
@@ -545,7 +558,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
             ptx::mbar_init(bar.pv_done(i), 1); ptx::mbar_init(bar.o_full(i), 1);
         }
         for (int i = 0; i < F::RING; ++i) ptx::mbar_init(bar.info_full(i), 1);
-        ptx::mbar_init(bar.q_full(), 7); ptx::mbar_init(bar.drained(), 1);
+        ptx::mbar_init(bar.q_full(), 8); ptx::mbar_init(bar.drained(), 1);
         ptx::mbar_fence_init();
         *abort_flag = (int)blockIdx.x == a.give_up ? 1 : 0;
     }
@@ -576,6 +589,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
         const KvSteps steps(tile.low0, tile.last(), a.window, a.sinks, 128);
         if (warp < 8) {
             set_registers_up<F::ROWS_REGS>();
+            kv_prompt_queries<F>(a, tile, bar, smem);
             kv_prompt_rows<F>(a, tile, steps, bar, smem, tmem, abort_flag);
         } else {
             set_registers_down<F::OTHER_REGS>();
