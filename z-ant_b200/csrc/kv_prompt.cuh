@@ -202,40 +202,49 @@ __device__ __forceinline__ void kv_prompt_queries(const KvAttendArgs& a, const K
     const bool mine = column < c.dim;
     float* row_factor = reinterpret_cast<float*>(smem + F::OFF_REST);
     uint8_t* operand = smem + (which >> 2) * F::BLOCK;
-#pragma unroll 2
-    for (int g = warp; g < F::ROWS / TPL; g += 8) {
-        const int r = g * TPL + in_group, row = tile.row0 + r;
-        const bool there = r < tile.rows && mine;
-        float v[16];
-        if (there) kv_values16(a.q, a.q_type, a.wide_q, (long long)(tile.row + row / a.group) * a.q_stride + (long long)(tile.h * a.group + row % a.group) * c.dim + column, v);
-        else {
+    constexpr int N = F::ROWS / TPL / 8, U = N < 4 ? N : 4;       // a warp's turns; rows that a lane has under way (one at a time: 14800 clocks for all)
+#pragma unroll 1
+    for (int g0 = 0; g0 < N; g0 += U) {
+        uint32_t raw[U][8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+        for (int i = 0; i < U; ++i) {
+            const int r = ((g0 + i) * 8 + warp) * TPL + in_group, row = tile.row0 + r;
+#pragma unroll
+            for (int z = 0; z < 8; ++z) raw[i][z] = 0;
+            if (r < tile.rows && mine)
+                kv_load16(static_cast<const __half*>(a.q) + (long long)(tile.row + row / a.group) * a.q_stride + (long long)(tile.h * a.group + row % a.group) * c.dim + column, a.wide_q, raw[i]);
         }
-        float big = 0.0f;
-        bool odd = false;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { big = fmaxf(big, fabsf(v[i])); odd |= !(fabsf(v[i]) < INFINITY); }
+        for (int i = 0; i < U; ++i) {
+            const int r = ((g0 + i) * 8 + warp) * TPL + in_group;
+            float v[16];
+            if (a.q_type == ZANT_F16) { RowChunk<__half>::values(raw[i], v); RowChunk<__half>::values(raw[i] + 4, v + 8); }
+            else { RowChunk<__nv_bfloat16>::values(raw[i], v); RowChunk<__nv_bfloat16>::values(raw[i] + 4, v + 8); }
+            float big = 0.0f;
+            bool odd = false;
 #pragma unroll
-        for (int d = LPR / 2; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-        odd = (__ballot_sync(0xffffffffu, odd) >> (lane / LPR * LPR)) & ((1u << LPR) - 1u);
-        const int e = min(max((int)(__float_as_uint(big) >> 23) - 127 - 14, -114), 127);
-        // (a negative scale's sign goes into q: scores are multiplied by positive numbers only)
-        const float down = odd ? 0.0f : copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);
-        const float up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(127 + e, 1) << 23);
-        if (which == 0) row_factor[r] = up * fabsf(a.scale_log2);
-        uint32_t f[8];
+            for (int z = 0; z < 16; ++z) { big = fmaxf(big, fabsf(v[z])); odd |= !(fabsf(v[z]) < INFINITY); }
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-            float x[4];
+            for (int d = LPR / 2; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+            odd = (__ballot_sync(0xffffffffu, odd) >> (lane / LPR * LPR)) & ((1u << LPR) - 1u);
+            const int e = min(max((int)(__float_as_uint(big) >> 23) - 127 - 14, -114), 127);
+            // (a negative scale's sign goes into q: scores are multiplied by positive numbers only)
+            const float down = odd ? 0.0f : copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);
+            const float up = odd ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(127 + e, 1) << 23);
+            if (which == 0) row_factor[r] = up * fabsf(a.scale_log2);
+            uint32_t f[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = odd ? 0.0f : v[4 * z + i] * down;
-            f[2 * z] = pack_f16(x[0], x[2]);
-            f[2 * z + 1] = pack_f16(x[1], x[3]);
+            for (int z = 0; z < 4; ++z) {
+                float x[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) x[y] = odd ? 0.0f : v[4 * z + y] * down;
+                f[2 * z] = pack_f16(x[0], x[2]);
+                f[2 * z + 1] = pack_f16(x[1], x[3]);
+            }
+            uint8_t* to = operand + (r >> 7) * F::OPERAND + (r & 127) * 128;
+            *reinterpret_cast<uint4*>(to + ((chunk ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(to + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
         }
-        uint8_t* to = operand + (r >> 7) * F::OPERAND + (r & 127) * 128;
-        *reinterpret_cast<uint4*>(to + ((chunk ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
-        *reinterpret_cast<uint4*>(to + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
     }
     kv_written(bar.q_full());
 }
