@@ -64,7 +64,8 @@ def test_few_tokens(ctx, zb, new, lengths, heads, kv_heads, dim, page, kind):
 PROMPTS = [
     ([40], [40], 4, 4, 64, 16), ([130], [130], 4, 2, 128, 64), ([100, 1, 0, 29], [400, 1, 10, 30], 6, 2, 96, 32), ([257], [300], 5, 1, 128, 128),
     ([33], [200], 2, 1, 256, 16), ([129, 128, 127], [129, 500, 127], 3, 1, 80, 256), ([1, 300], [600, 300], 8, 2, 128, 64), ([150], [151], 16, 2, 48, 16),
-    ([200, 7], [200, 900], 7, 1, 128, 32), ([64, 64, 64], [64, 128, 1000], 12, 12, 96, 64)]
+    ([200, 7], [200, 900], 7, 1, 128, 32), ([64, 64, 64], [64, 128, 1000], 12, 12, 96, 64),
+    ([150, 1], [900, 200], 4, 2, 256, 32), ([130], [130], 3, 1, 144, 16), ([70, 100, 1], [70, 300, 5], 4, 4, 208, 128), ([257], [1000], 2, 2, 256, 256)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
@@ -75,7 +76,7 @@ def test_prompts(ctx, zb, new, lengths, heads, kv_heads, dim, page, kind):
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 3), (5, 0), (32, 4), (33, 1), (64, 64), (100, 40), (130, 200), (10 ** 6, 4), (2 ** 31 - 1, 2 ** 31 - 1)])
-@pytest.mark.parametrize("new,lengths,heads,kv_heads,dim,page", [([1, 1], [500, 90], 8, 2, 128, 16), ([3, 2, 1], [300, 100, 33], 6, 1, 64, 32), ([150, 20], [400, 20], 4, 2, 96, 64), ([300], [300], 5, 1, 128, 32)])
+@pytest.mark.parametrize("new,lengths,heads,kv_heads,dim,page", [([1, 1], [500, 90], 8, 2, 128, 16), ([3, 2, 1], [300, 100, 33], 6, 1, 64, 32), ([150, 20], [400, 20], 4, 2, 96, 64), ([300], [300], 5, 1, 128, 32), ([140], [500], 2, 1, 256, 16)])
 def test_windows_and_sinks(ctx, zb, new, lengths, heads, kv_heads, dim, page, kind, window, sinks):
     check(ctx, zb, new, lengths, heads, kv_heads, dim, page, kind, window=window, sinks=sinks)
 
@@ -226,15 +227,15 @@ def test_host_arrays(ctx, zb):
     within(ls.astype(np.float64), lse, lse_off)
 
 
-@pytest.mark.parametrize("new,length", [(300, 600), (2, 600), (1, 20000)])
+@pytest.mark.parametrize("new,length,dim", [(300, 600, 128), (2, 600, 128), (1, 20000, 128), (200, 300, 256)])
 @pytest.mark.parametrize("cta", [0, 3, 10007])
-def test_a_cta_gives_up(ctx, zb, new, length, cta):
+def test_a_cta_gives_up(ctx, zb, new, length, dim, cta):
     """A CTA whose first wait runs out: every warp of it comes to the kernel's end (and its cluster), the call reports the time-out, and the calls behind it are right."""
     import torch
     rng = np.random.default_rng(8)
-    cache = ref.Cache(2 * (length // 64 + 1), 2, 64, 128, rng)
+    cache = ref.Cache(2 * (length // 64 + 1), 2, 64, dim, rng)
     table = tables(rng, cache.pages, 64, [length, length // 2])
-    q = as_kind(torch, rng.standard_normal((2 * new, 4, 128)), "bf16")
+    q = as_kind(torch, rng.standard_normal((2 * new, 4, dim)), "bf16")
     args = (ctx, zb, torch, cache, q, table, [length, length // 2], None, "bf16")
     want = run(*args)
     ctx.selftest_give_up(cta)

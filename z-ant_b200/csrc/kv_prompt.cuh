@@ -1,6 +1,6 @@
 // Attention of many new tokens (prompts, parts of them) over the cache of kv_cache.cuh on tcgen05: the formulas and masks of kv_attention.cuh for results in 16 bits.
 //
-// A CTA has 256 rows, (new token, head) pairs that share a key head, as two tiles of 128.  Steps of 128 tokens, whose scores come in halves of 64 with a place each in tensor memory: while a
+// A CTA has 256 rows, (new token, head) pairs that share a key head, as two tiles of 128 (with more than 128 dimensions one tile, whose sums take half of tensor memory).  Steps of 128 tokens, whose scores come in halves of 64 with a place each in tensor memory: while a
 // row's thread takes the exponentials of one half, the tensor core multiplies V with the other half's weights and takes the next step's scores in its place.  (Whole steps with one
 // place: the rows waited 1300 clocks of 4500 for their next scores.)  Codes become f16 (exactly) once for all 256 rows; q is f16 times a power of two for each row, so that its largest value lies in
 // [2^14, 2^15) (f16 and bf16 values lose nothing down to 2^-28 of that one).  Scores are 128 x 64 x dim products into tensor memory; each thread has a row of them, finds its maximum, and
@@ -63,10 +63,12 @@ template <int N> __device__ __forceinline__ void set_registers_down() { asm vola
 
 template <int DP_>
 struct KvPromptCfg {
-    static constexpr int DP = DP_, TILE = 128, ROWS = 2 * TILE, STEP = 128, WARPS = 16, THREADS = 32 * WARPS;
-    static constexpr int BLOCK = TILE * 128;          // 128 rows of 64 f16 numbers
-    static constexpr int OPERAND = BLOCK * (DP / 64); // Q of a tile, K or V of a step
-    static constexpr int OFF_K = 2 * OPERAND, OFF_V = 4 * OPERAND, OFF_REST = 6 * OPERAND;
+    static constexpr int DP = DP_, TILES = DP > 128 ? 1 : 2, ROWS = 128 * TILES, THREADS = 512;
+    // K and V come in units of 128 tokens, of 256 dimensions of 64 (a half of a step); two of each are there
+    static constexpr int UNIT = DP > 128 ? 64 : 128, UNITS = 128 / UNIT;
+    static constexpr int Q_BLOCK = 128 * 128, BLOCK = UNIT * 128;      // rows of 64 f16 numbers: of a tile's q, of a unit
+    static constexpr int Q_OPERAND = Q_BLOCK * (DP / 64), OPERAND = BLOCK * (DP / 64);
+    static constexpr int OFF_K = TILES * Q_OPERAND, OFF_V = OFF_K + 2 * OPERAND, OFF_REST = OFF_V + 2 * OPERAND;
     static constexpr int LPR = DP / 16;               // lanes of a row of codes
     static constexpr int TPL = 32 / LPR;              // tokens of a warp's load
     static constexpr int ROWS_REGS = 136, OTHER_REGS = 120;       // 256 x 136 + 256 x 120 = 512 x 128
@@ -142,10 +144,10 @@ __device__ __forceinline__ bool kv_wait(const KvAttendArgs& a, uint32_t bar, uin
     }
 }
 
-// Codes on their way to f16 operands: warp `warp` of the seven takes every seventh TPL tokens of a step's 128.
+// Codes on their way to f16 operands: warp `warp` of the seven takes every seventh TPL tokens of a unit.
 template <typename F>
 struct KvConvert {
-    static constexpr int WARPS = 7, LPR = F::LPR, GROUPS = 128 / F::TPL, N = (GROUPS + WARPS - 1) / WARPS;
+    static constexpr int WARPS = 7, LPR = F::LPR, GROUPS = F::UNIT / F::TPL, N = (GROUPS + WARPS - 1) / WARPS;
     uint4 w[N];
     // block_of(i): where the i-th 16 tokens lie in the cache, in units of 16 tokens (-1: nowhere); mine: the lane's 16 bytes are dimensions of the head
     template <typename B>
@@ -201,7 +203,7 @@ __device__ __forceinline__ void kv_prompt_queries(const KvAttendArgs& a, const K
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, which = lane % LPR, in_group = lane / LPR, column = which * 16, chunk = (which & 3) * 2;
     const bool mine = column < c.dim;
     float* row_factor = reinterpret_cast<float*>(smem + F::OFF_REST);
-    uint8_t* operand = smem + (which >> 2) * F::BLOCK;
+    uint8_t* operand = smem + (which >> 2) * F::Q_BLOCK;
     constexpr int N = F::ROWS / TPL / 8, U = N < 4 ? N : 4;       // a warp's turns; rows that a lane has under way (one at a time: 14800 clocks for all)
 #pragma unroll 1
     for (int g0 = 0; g0 < N; g0 += U) {
@@ -241,7 +243,7 @@ __device__ __forceinline__ void kv_prompt_queries(const KvAttendArgs& a, const K
                 f[2 * z] = pack_f16(x[0], x[2]);
                 f[2 * z + 1] = pack_f16(x[1], x[3]);
             }
-            uint8_t* to = operand + (r >> 7) * F::OPERAND + (r & 127) * 128;
+            uint8_t* to = operand + (r >> 7) * F::Q_OPERAND + (r & 127) * 128;
             *reinterpret_cast<uint4*>(to + ((chunk ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
             *reinterpret_cast<uint4*>(to + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
         }
@@ -284,8 +286,8 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar.info_full(k & (F::RING - 1)));
     };
-    auto blocks = [&](int k) { return [=](int i) { return reinterpret_cast<const int*>(info + (k & (F::RING - 1)) * F::INFO)[28 + i]; }; };
-    // the first step's codes before anything else
+    auto blocks = [&](int u) { return [=](int i) { return reinterpret_cast<const int*>(info + ((u / F::UNITS) & (F::RING - 1)) * F::INFO)[28 + (u % F::UNITS) * (F::UNIT / 16) + i]; }; };
+    // the first unit's codes before anything else
     look(0);
     const int first = kv_prompt_block(c, tile, steps, 0, page);
     auto first_block = [&](int i) { return __shfl_sync(0xffffffffu, first, i & 7); };
@@ -315,21 +317,22 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
     }
 
 #pragma unroll 1
-    for (int k = 0; k < steps.total; ++k) {
-        const uint32_t free_parity = ((uint32_t)(k >> 1) & 1u) ^ 1u;
+    for (int u = 0; u < steps.total * F::UNITS; ++u) {
+        const int k = u / F::UNITS;
+        const uint32_t free_parity = ((uint32_t)(u >> 1) & 1u) ^ 1u;
         if (!kv_wait(a, bar.info_full((k + 1) & (F::RING - 1)), (uint32_t)((k + 1) / F::RING) & 1u, abort_flag)) return;
-        if (!kv_wait(a, bar.k_empty(k & 1), free_parity, abort_flag)) return;
-        kc.store(operand + F::OFF_K + (k & 1) * F::OPERAND, warp, in_group, chunk);
-        kv_written(bar.k_full(k & 1));
-        kc.load(c.k, blocks(k + 1), warp, c.dim, in_group, column, mine);
-        if (warp == 6) {
+        if (!kv_wait(a, bar.k_empty(u & 1), free_parity, abort_flag)) return;
+        kc.store(operand + F::OFF_K + (u & 1) * F::OPERAND, warp, in_group, chunk);
+        kv_written(bar.k_full(u & 1));
+        kc.load(c.k, blocks(u + 1), warp, c.dim, in_group, column, mine);
+        if (warp == 6 && u % F::UNITS == 0) {
             tell(k + 2, vs);
             look(k + 3);
         }
-        if (!kv_wait(a, bar.v_empty(k & 1), free_parity, abort_flag)) return;
-        vc.store(operand + F::OFF_V + (k & 1) * F::OPERAND, warp, in_group, chunk);
-        kv_written(bar.v_full(k & 1));
-        vc.load(c.v, blocks(k + 1), warp, c.dim, in_group, column, mine);
+        if (!kv_wait(a, bar.v_empty(u & 1), free_parity, abort_flag)) return;
+        vc.store(operand + F::OFF_V + (u & 1) * F::OPERAND, warp, in_group, chunk);
+        kv_written(bar.v_full(u & 1));
+        vc.load(c.v, blocks(u + 1), warp, c.dim, in_group, column, mine);
     }
 }
 
@@ -341,22 +344,55 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
     const uint32_t leader = ptx::elect_one() ? 1u : 0u;
     int count[2] = {0, 0};                            // a tile's steps so far
     const KvPromptSteps mine[2] = {KvPromptSteps(steps, tile.low0, tile.high0, a.window, a.sinks), KvPromptSteps(steps, tile.low1, tile.high1, a.window, a.sinks)};
+    // where the half of a step lies: a part of its unit, or a unit of its own
+    auto unit_at = [&](int k, int b) { return (uint32_t)(F::UNITS == 1 ? (k & 1) * F::OPERAND + b * 64 * 128 : b * F::OPERAND); };
     auto scores = [&](int x, int k, int b) {
-        const uint32_t qa = kv_desc_lo(s0 + x * F::OPERAND, 16), kb = kv_desc_lo(s0 + F::OFF_K + (k & 1) * F::OPERAND + b * 64 * 128, 16);
+        const uint32_t qa = kv_desc_lo(s0 + x * F::Q_OPERAND, 16), kb = kv_desc_lo(s0 + F::OFF_K + unit_at(k, b), 16);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            const uint32_t at = ((i >> 2) * F::BLOCK + (i & 3) * 32) >> 4;
-            mma_f16_ss_if(leader, tmem + x * 128 + b * 64, qa + at, kb + at, idesc_s, i > 0);
-        }
+        for (int i = 0; i < DP / 16; ++i)
+            mma_f16_ss_if(leader, tmem + x * 128 + b * 64, qa + (((i >> 2) * F::Q_BLOCK + (i & 3) * 32) >> 4), kb + (((i >> 2) * F::BLOCK + (i & 3) * 32) >> 4), idesc_s, i > 0);
         ptx::mma_commit_if(leader, bar.s_full(x, b));
     };
     auto values = [&](int x, int k, int b) {
-        const uint32_t vb = kv_desc_lo(s0 + F::OFF_V + (k & 1) * F::OPERAND + b * 64 * 128, F::BLOCK);
+        const uint32_t vb = kv_desc_lo(s0 + F::OFF_V + unit_at(k, b), F::BLOCK);
 #pragma unroll
         for (int i = 0; i < 4; ++i) mma_f16_ts_if(leader, tmem + 256 + x * DP, tmem + x * 128 + b * 64 + i * 8, vb + i * (2048 >> 4), idesc_o, (count[x] | b | i) != 0);
         ptx::mma_commit_if(leader, bar.pv_done(x));
         if (b == 1 && k == mine[x].to - 1) ptx::mma_commit_if(leader, bar.o_full(x));      // its last step
     };
+    if constexpr (F::UNITS == 2) {
+        // one tile; the halves have barriers of their own
+        if (steps.total > 0) {
+            if (!kv_wait(a, bar.q_full(), 0, abort_flag)) return;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (!kv_wait(a, bar.k_full(b), 0, abort_flag)) return;
+                ptx::tc_fence_after();
+                if (mine[0].active(0)) scores(0, 0, b);
+                ptx::mma_commit_if(leader, bar.k_empty(b));
+            }
+        }
+        for (int k = 0; k < steps.total; ++k) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (!kv_wait(a, bar.v_full(b), (uint32_t)k & 1u, abort_flag)) return;
+                if (mine[0].active(k)) {
+                    if (!kv_wait(a, bar.p_full(0, b), (uint32_t)count[0] & 1u, abort_flag)) return;
+                    ptx::tc_fence_after();
+                    values(0, k, b);
+                    count[0] += b;
+                }
+                ptx::mma_commit_if(leader, bar.v_empty(b));
+                if (k + 1 < steps.total) {
+                    if (!kv_wait(a, bar.k_full(b), (uint32_t)(k + 1) & 1u, abort_flag)) return;
+                    ptx::tc_fence_after();
+                    if (mine[0].active(k + 1)) scores(0, k + 1, b);
+                    ptx::mma_commit_if(leader, bar.k_empty(b));
+                }
+            }
+        }
+        return;
+    }
     if (steps.total > 0) {
         if (!kv_wait(a, bar.q_full(), 0, abort_flag) || !kv_wait(a, bar.k_full(0), 0, abort_flag)) return;
         ptx::tc_fence_after();
@@ -592,7 +628,7 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
     if (tile.rows > 0) {                              // (the same for the whole CTA)
         tile.s = q.s; tile.row = q.row; tile.first = q.first;
         tile.low0 = max(q.first + tile.row0 / a.group, -1);
-        tile.high0 = max(q.first + (tile.row0 + min(tile.rows, 128) - 1) / a.group, -1);
+        tile.high0 = max(q.first + (tile.row0 + min(tile.rows, 128) - 1) / a.group, -1);      // (of 256 dimensions all of them)
         tile.low1 = max(q.first + (tile.row0 + 128) / a.group, -1);
         tile.high1 = tile.rows <= 128 ? -1 : max(q.first + (tile.row0 + tile.rows - 1) / a.group, -1);
         const KvSteps steps(tile.low0, tile.last(), a.window, a.sinks, 128);
@@ -642,14 +678,14 @@ constexpr int kPromptRows = 64;
 
 inline int32_t run_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     a.more_rows_than = 0; a.rows_up_to = 0x7fffffff;
-    if (a.q_type == ZANT_F32 || a.c.dim > 128) return run_kv_few(ctx, a);
+    if (a.q_type == ZANT_F32) return run_kv_few(ctx, a);
     // Which sequences have many rows is known on the device only, unless all have the same number: both kernels run then, and each takes its own.
     const bool uniform = !a.c.offsets;
     const long long most = uniform ? (long long)a.c.per * a.group : (long long)a.c.rows * a.group;
     if (most > kPromptRows) {
         KvAttendArgs p = a;
         p.more_rows_than = kPromptRows;
-        ZB_TRY(a.c.dim <= 64 ? launch_kv_prompt<64>(ctx, p) : launch_kv_prompt<128>(ctx, p));
+        ZB_TRY(a.c.dim <= 64 ? launch_kv_prompt<64>(ctx, p) : (a.c.dim <= 128 ? launch_kv_prompt<128>(ctx, p) : launch_kv_prompt<256>(ctx, p)));
         if (uniform) return ZANT_OK;
         a.rows_up_to = kPromptRows;
     }
