@@ -673,8 +673,14 @@ inline int32_t launch_kv_prompt(zant_ctx* ctx, KvAttendArgs a) {
     return check_launch(ctx, "kv_prompt_kernel");
 }
 
-// Rows of a key head from which on a sequence is a prompt.
-constexpr int kPromptRows = 64;
+// A sequence with more rows of a key head than this is a prompt.  Where prompts' tiles fill half of the SMs, 30 rows take as long here as in kv_attention_kernel (16 x 6 tokens of 5 heads
+// over 6000: 164 us both; 12 tokens 168, 282 there; 3 tokens 164, 82); fewer tiles leave SMs idle that kv_attention_kernel's clusters use (2 x 6 over 6000: 125 us here, 55
+// there; 2 x 48 140, 127; over 500 2 x 12 25 both).
+inline int kv_prompt_from(const zant_ctx* ctx, const KvAttendArgs& a) {
+    const long long tiles = kv_units(a.c, a.group, a.c.dim > 128 ? 128 : 256, 1) * a.c.heads;
+    const long long reach = std::min((long long)a.c.width << a.c.page_log2, a.window > 0 ? (long long)a.window + a.sinks : 0x7fffffffffLL);
+    return tiles * 2 >= ctx->sm_count ? 28 : (reach >= 2048 ? 192 : 64);
+}
 
 inline int32_t run_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     a.more_rows_than = 0; a.rows_up_to = 0x7fffffff;
@@ -682,12 +688,13 @@ inline int32_t run_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     // Which sequences have many rows is known on the device only, unless all have the same number: both kernels run then, and each takes its own.
     const bool uniform = !a.c.offsets;
     const long long most = uniform ? (long long)a.c.per * a.group : (long long)a.c.rows * a.group;
-    if (most > kPromptRows) {
+    const int from = kv_prompt_from(ctx, a);
+    if (most > from) {
         KvAttendArgs p = a;
-        p.more_rows_than = kPromptRows;
+        p.more_rows_than = from;
         ZB_TRY(a.c.dim <= 64 ? launch_kv_prompt<64>(ctx, p) : (a.c.dim <= 128 ? launch_kv_prompt<128>(ctx, p) : launch_kv_prompt<256>(ctx, p)));
         if (uniform) return ZANT_OK;
-        a.rows_up_to = kPromptRows;
+        a.rows_up_to = from;
     }
     return run_kv_few(ctx, a);
 }
