@@ -81,6 +81,25 @@ def test_windows_and_sinks(ctx, zb, new, lengths, heads, kv_heads, dim, page, ki
     check(ctx, zb, new, lengths, heads, kv_heads, dim, page, kind, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [2, 90])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1.0, 1e-20])
+def test_scales(ctx, zb, new, scale, kind):
+    check(ctx, zb, [new, new], [new, 300], 4, 2, 64, 16, kind, scale=scale, q_size=0.3)
+
+
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32 + 5, 2 ** 40])
+def test_windows_beyond_int32_are_none(ctx, zb, window):
+    check(ctx, zb, [2], [300], 2, 1, 64, 16, "bf16", window=window, sinks=window)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_decoding_and_prompts_in_one_call(ctx, zb, kind):
+    """Both kernels run, each takes its sequences; rows of none are left as they were."""
+    check(ctx, zb, [1, 300, 0, 2, 5, 130, 1, 40], [700, 300, 50, 90, 2000, 131, 1, 41], 10, 2, 128, 32, kind, spare=3)
+    check(ctx, zb, [1] * 30 + [400], [100 + 7 * i for i in range(30)] + [400], 8, 4, 64, 16, kind)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("new", [1, 3, 70])
 def test_equal_shares_without_offsets(ctx, zb, new, kind):

@@ -1028,7 +1028,7 @@ class Context:
         keep, tp, seqs, width, lp, op = self._sequences(table, lengths, offsets)
         sp = None if lse is None else _values(lse, rows * heads, F32, "lse", True)[1]
         check(lib().zant_b200_kv_cache_attention(self._h, cache._at, code, qp, q_stride, rows, heads, tp, seqs, width, lp, op,
-                                                 cache.dim ** -0.5 if scale is None else scale, window, sinks, yp, y_stride, sp))
+                                                 cache.dim ** -0.5 if scale is None else scale, max(-1, min(window, 2 ** 31 - 1)), max(-1, min(sinks, 2 ** 31 - 1)), yp, y_stride, sp))
         return out
 
     def verify_drafts(self, target, drafted, tokens, accept, sample, offsets=None, out=None):

@@ -722,8 +722,9 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
 
 template <int DP, bool SPLIT>
 inline int32_t choose_kv_attention(zant_ctx* ctx, const KvAttendArgs& a) {
-    // (where others take the sequences with many rows, what is left has a token or a few)
-    const long long rows = a.rows_up_to < 0x7fffffff ? a.group : ((long long)a.c.rows + a.c.seqs - 1) / a.c.seqs * a.group;
+    // (where others take the sequences with many rows and these are most, what is left has a token or a few)
+    long long rows = ((long long)a.c.rows + a.c.seqs - 1) / a.c.seqs * a.group;
+    if (rows > a.rows_up_to) rows = a.group;
     if (rows <= 8) return launch_kv_attention<DP, 1, SPLIT>(ctx, a);
     if constexpr (DP <= 128 && !SPLIT)
         if (rows > 16) return launch_kv_attention<DP, 4, SPLIT>(ctx, a);
