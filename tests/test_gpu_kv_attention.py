@@ -81,6 +81,16 @@ def test_windows_and_sinks(ctx, zb, new, lengths, heads, kv_heads, dim, page, ki
     check(ctx, zb, new, lengths, heads, kv_heads, dim, page, kind, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("seqs,kv_heads,new", [(100, 5, 1), (128, 8, 1), (129, 4, 1), (70, 8, 3), (60, 4, 12)])
+def test_more_sequences_than_there_is_room_for(ctx, zb, seqs, kv_heads, new):
+    """The longest go first; equal lengths, lengths of zero."""
+    rng = np.random.default_rng(seqs)
+    lengths = rng.integers(0, 200, seqs)
+    lengths[::7] = 64
+    lengths[5:9] = 0
+    check(ctx, zb, [new] * seqs, list(lengths), kv_heads * 2, kv_heads, 64, 16, "bf16", uniform=True)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("new", [2, 90])
 @pytest.mark.parametrize("scale", [0.0, -0.125, 1.0, 1e-20])

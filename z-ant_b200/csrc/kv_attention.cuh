@@ -42,6 +42,7 @@ struct KvAttendArgs {
     bool wide_q, wide_out;                            // q, out in whole 16-byte blocks
     int more_rows_than, rows_up_to;                   // sequences with more rows of a key head than the first, up to the second, are the kernel's
     int parts, tiles_each;                            // CTAs of a tile; tiles of each sequence (0: by its rows)
+    bool by_length;                                   // the longest sequences first (as many as a CTA has threads at most)
     float* work; size_t work_bytes;                   // a workspace, if there is one: a tile's CTAs leave their sums there, and need not be a cluster
     int* status; long long wait_budget; int give_up;  // give_up: self test, a CTA whose first wait counts as run out (-1: none)
 };
@@ -191,6 +192,22 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         unit = work / c.heads % a.tiles_each;
         q = kv_seq(c, min(work / c.heads / a.tiles_each, c.seqs - 1));
         any = q.n > 0;
+    } else if (a.by_length) {
+        // the sequence whose length has the wanted place among all
+        int* lengths = reinterpret_cast<int*>(smem);
+        const int tid = threadIdx.x, each = (int)(((long long)c.per * a.group + F::ROWS - 1) / F::ROWS), want = work / c.heads / each;
+        const int mine = tid < c.seqs ? c.lengths[tid] : 0;
+        if (tid < c.seqs) lengths[tid] = mine;
+        __syncthreads();
+        int place = 0;
+        for (int i = 0; i < c.seqs; ++i) place += lengths[i] > mine || (lengths[i] == mine && i < tid);
+        if (tid < c.seqs && place == want) lengths[128] = tid;
+        __syncthreads();
+        const int s = lengths[128];
+        __syncthreads();                              // (the ring is used from here on)
+        unit = work / c.heads % each;
+        q = kv_seq(c, s);
+        any = true;
     } else any = kv_locate(c, work / c.heads, a.group, F::ROWS, 1, q, unit);
     const int row0 = unit * F::ROWS, rows = any && q.n * a.group > a.more_rows_than && q.n * a.group <= a.rows_up_to ? min(F::ROWS, q.n * a.group - row0) : 0;
     if (rows <= 0) return;                            // (all CTAs of a cluster)
@@ -698,6 +715,8 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
         else a.work = nullptr;
     }
     a.parts = parts;
+    // more CTAs than there is room for at once: the longest sequences first, so that the last ones are short
+    a.by_length = !a.c.offsets && !a.tiles_each && a.c.seqs > 1 && a.c.seqs <= 32 * warps && items * parts > slots;
     a.status = ctx->status_word;
     a.give_up = ctx->give_up_cta < 0 ? -1 : (int)(ctx->give_up_cta % (items * parts));
     ctx->give_up_cta = -1;

@@ -426,14 +426,15 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
 // Weights of a row's 64 scores in tensor memory at `ts` (minus infinity: not seen), in pairs, under the base `base` (log2): p, their sum with each page's factor taken out, and
 // the largest exponent.
 __device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* info, float factor, float base, uint32_t (&p)[32], float& sum) {
-    uint32_t v[2][16];
+    uint32_t v[64];
     float top = -INFINITY;
     sum = 0.0f;
-    ptx::tmem_ld16(ts, v[0]);
+    ptx::tmem_ld32(ts, v);
+    ptx::tmem_ld32(ts + 32, v + 32);
+    ptx::tmem_wait_ld32(v);
+    ptx::tmem_wait_ld32(v + 32);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {                     // 16 tokens, which are on one page
-        tmem_wait_ld16(v[g & 1]);
-        if (g < 3) ptx::tmem_ld16(ts + 16 * (g + 1), v[(g + 1) & 1]);
         float f = factor * info[g];
         f = f == 0.0f ? 1e-38f : f;                   // (minus infinity stays what it is)
         const float lv = info[8 + g], b = lv + 6.0f - base;
@@ -442,7 +443,7 @@ __device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* inf
         float most = -INFINITY;
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
-            const float2 e = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(v[g & 1][2 * y]), __uint_as_float(v[g & 1][2 * y + 1])), f2, b2));
+            const float2 e = ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(v[16 * g + 2 * y]), __uint_as_float(v[16 * g + 2 * y + 1])), f2, b2));
             most = fmaxf(most, fmaxf(e.x, e.y));
             const float2 w = make_float2(ex2(e.x), ex2(e.y));
             s2 = ptx::add2(s2, ptx::pack2(w.x, w.y));
