@@ -388,8 +388,8 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         float x[H][NT][4];
 #pragma unroll
         for (int half = 0; half < H; ++half) {
-            // (16 rows at a time, for the registers' sake; K is read again for others)
-            constexpr int NG = NT < 2 ? NT : 2;
+            // (8 or 16 rows at a time, for the registers' sake; K is read again for others)
+            constexpr int NG = NT % 2 ? 1 : 2;
 #pragma unroll
             for (int n0 = 0; n0 < NT; n0 += NG) {
                 int sum[NG][DIG][4];
@@ -705,7 +705,7 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     const long long steps = (reach + F::STEP - 1) / F::STEP;
     const long long slots = (long long)ctx->sm_count * (F::MOST_WARPS / 4);
     int warps = 4, parts = 1;
-    while (parts < 16 && ((items * parts * 2 <= slots && steps >= 8LL * parts) || (items * parts * 2 <= 3 * slots && steps >= 64LL * parts))) parts *= 2;
+    while (parts < 16 && ((items * parts * 2 <= slots && steps > 4LL * parts) || (items * parts * 2 <= 3 * slots && steps >= 64LL * parts))) parts *= 2;
     if (items * parts <= ctx->sm_count && parts < 16 && steps >= (long long)parts * F::MOST_WARPS) warps = F::MOST_WARPS;
     // Few tiles of long contexts: clusters of 16 leave most of the GPU idle (8 of them, one sequence of 131072: 113 us), so as many CTAs as it holds share a tile through the workspace and
     // a second kernel joins them.
@@ -746,7 +746,7 @@ inline int32_t choose_kv_attention(zant_ctx* ctx, const KvAttendArgs& a) {
     if (rows > a.rows_up_to) rows = a.group;
     if (rows <= 8) return launch_kv_attention<DP, 1, SPLIT>(ctx, a);
     if constexpr (DP <= 128 && !SPLIT)
-        if (rows > 16) return launch_kv_attention<DP, 4, SPLIT>(ctx, a);
+        if (rows > 16) return rows <= 24 ? launch_kv_attention<DP, 3, SPLIT>(ctx, a) : launch_kv_attention<DP, 4, SPLIT>(ctx, a);
     return launch_kv_attention<DP, 2, SPLIT>(ctx, a);
 }
 
