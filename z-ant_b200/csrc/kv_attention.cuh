@@ -739,7 +739,7 @@ inline int32_t launch_kv_attention(zant_ctx* ctx, KvAttendArgs a) {
     launch_cluster(ctx, kernel, dim3((unsigned)(items * parts)), 32 * warps, F::smem(warps), a.work ? 1u : (unsigned)parts, a, k_map, v_map);
     ZB_TRY(check_launch(ctx, "kv_attention_kernel"));
     if (!a.work) return ZANT_OK;
-    launch(ctx, kv_attention_join_kernel<DP, NT>, dim3((unsigned)items, F::ROWS * (DP / 4) / 256 ? F::ROWS * (DP / 4) / 256 : 1), 256, 0, a);
+    launch(ctx, kv_attention_join_kernel<DP, NT>, dim3((unsigned)items, (F::ROWS * (DP / 4) + 255) / 256), 256, 0, a);
     return check_launch(ctx, "kv_attention_join_kernel");
 }
 
