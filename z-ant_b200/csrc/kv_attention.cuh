@@ -122,6 +122,11 @@ struct KvSteps {
     }
     __device__ __forceinline__ int at(int k, int S) const { return (k < sink ? k : k - sink + first) * S; }
 };
+// The rows of a key head that the kernel has to do with in a sequence of n new tokens: all, or none where they are another kernel's.
+__device__ __forceinline__ int kv_rows_of(const KvAttendArgs& a, int n) {
+    const int rows = n * a.group;
+    return rows > a.more_rows_than && rows <= a.rows_up_to ? rows : 0;
+}
 // Some row at positions [low, high] sees one of the 16 tokens from t on.  (What the table says of others, and their pages' scales, is nobody's business.)
 __device__ __forceinline__ bool kv_seen16(int t, int low, int high, int window, int sinks) { return t <= high && (window == 0 || t + 15 > low - window || t < sinks); }
 
@@ -210,7 +215,7 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         q = kv_seq(c, s);
         any = true;
     } else any = kv_locate(c, work / c.heads, a.group, F::ROWS, 1, q, unit);
-    const int row0 = unit * F::ROWS, rows = any && q.n * a.group > a.more_rows_than && q.n * a.group <= a.rows_up_to ? min(F::ROWS, q.n * a.group - row0) : 0;
+    const int row0 = unit * F::ROWS, rows = any ? min(F::ROWS, kv_rows_of(a, q.n) - row0) : 0;
     if (rows <= 0) {                                  // (all CTAs of a cluster)
         if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, (int)DEV_ERR_WAIT_TIMEOUT);
         return;
@@ -640,7 +645,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const __grid_con
     const int h = blockIdx.x % c.heads;
     KvSeq q; int unit;
     if (!kv_locate(c, blockIdx.x / c.heads, a.group, ROWS, 1, q, unit)) return;
-    const int row0 = unit * ROWS, rows = min(ROWS, q.n * a.group - row0);
+    const int row0 = unit * ROWS, rows = min(ROWS, kv_rows_of(a, q.n) - row0);      // (no more than the CTAs that left sums here)
     const int e = blockIdx.y * 256 + threadIdx.x, r = e / QUADS, d = (e % QUADS) * 4;
     if (r >= rows || d >= c.dim) return;
     const float* part = a.work + (size_t)blockIdx.x * a.parts * (ROWS * (DP + 2));
