@@ -115,7 +115,7 @@ struct KvSteps {
         if (high < 0) { total = 0; return; }
         if (window > 0 && low - window + 1 > 0) {
             first = (low - window + 1) / S;
-            sink = min((sinks + S - 1) / S, high / S + 1);
+            sink = min(sinks / S + (sinks % S != 0), high / S + 1);      // (sinks up to the end of int)
             if (sink >= first) sink = first = 0;
         }
         total = sink + high / S + 1 - first;
