@@ -199,8 +199,10 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         q = kv_seq(c, min(work / c.heads / a.tiles_each, c.seqs - 1));
         any = q.n > 0;
     } else if (a.by_length) {
-        // the sequence whose length has the wanted place among all
-        int* lengths = reinterpret_cast<int*>(smem);
+        // the sequence whose length has the wanted place among all.  (They lie where q's digits come later: the ring is written by TMA alone until its copies have landed, plain stores there would
+        // need a fence of proxies in front of the first copy.)
+        static_assert(F::Q_BYTES >= (32 * 4 + 1) * 4, "lengths of 128 sequences and a place");
+        int* lengths = reinterpret_cast<int*>(qs);
         const int tid = threadIdx.x, each = (int)(((long long)c.per * a.group + F::ROWS - 1) / F::ROWS), want = work / c.heads / each;
         const int mine = tid < c.seqs ? c.lengths[tid] : 0;
         if (tid < c.seqs) lengths[tid] = mine;
@@ -210,7 +212,7 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         if (tid < c.seqs && place == want) lengths[128] = tid;
         __syncthreads();
         const int s = lengths[128];
-        __syncthreads();                              // (the ring is used from here on)
+        __syncthreads();                              // (q's digits are written from here on)
         unit = work / c.heads % each;
         q = kv_seq(c, s);
         any = true;
