@@ -310,6 +310,7 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
     if (lane == 0) part[warp] = top;
 
+    __syncwarp();
     ptx::named_barrier_sync(1, 224);                  // (in front of any wait that may be given up)
     const float vs = kv_prompt_top(part);
     if (warp == 6) {
@@ -558,6 +559,7 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
 #pragma unroll
     for (int g = 0; g < DP / 16; ++g) {
         uint32_t v[16];
+        __syncwarp();                                 // (lanes that have stored and lanes without a row load together)
         if (count > 0) {                              // (the same for the whole warp)
             ptx::tmem_ld16(to + g * 16, v);
             tmem_wait_ld16(v);
