@@ -6,9 +6,11 @@
 // [2^14, 2^15) (f16 and bf16 values lose nothing down to 2^-28 of that one).  Scores are 128 x 64 x dim products into tensor memory; each thread has a row of them, finds its maximum, and
 // writes the weights back over them as f16, where they are the next product's operand.
 //
-// A page's scale of K multiplies its columns' scores; its scale of V, over the largest of the pages that the CTA sees, goes into the exponent: weights are 2^(x - m + lv + 6) with
-// lv = log2(vs / VS) in [-24, 0], so that what is rounded to f16 is at most 2^14 (the maximum is raised when one of a warp's rows has grown by 2^8, and then what has been summed is
-// rescaled), and what is lost below f16's least numbers is 2^-31 of the largest weight.  The sum of the weights takes the factor out again, once for 16 tokens.
+// A page's scale of K multiplies its columns' scores; its scale of V, over the largest VS of the pages that the CTA sees, goes into the exponent: weights are 2^(x + lv - M + 6) with
+// lv = log2(vs / VS) and M a row's own largest x + lv, so that what is rounded to f16 is at most 2^14 (M is raised when one of a warp's rows has grown by 2^8, and then what has been summed is
+// rescaled), and what is lost below f16's least numbers is 2^-31 of the row's largest weight times scale, wherever the scales of pages that other rows see lie.  The sum of the weights takes a page's
+// factor out again, once for 16 tokens: it is one of 2^(x - M), and in range while scales lie within 2^80 of one another.  CTAs that see others, or a scale of 0, have a form of the rows' code for themselves
+// (DEEP) that keeps a second maximum, of x, for it.
 //
 // A prompt of 8192 tokens, 40 over 8 heads of 128: 803 us (856 TFLOP/s, causal; 53 % of what cuBLAS reaches).  Exponentials and the tensor core are busy 40 % of the time each; a thread's chain of
 // loads from tensor memory, exponentials, packing and stores takes 1400 clocks a half step, waits, votes and addresses around it 900.
@@ -75,9 +77,9 @@ struct KvPromptCfg {
     static constexpr int LPR = DP / 16;               // lanes of a row of codes
     static constexpr int TPL = 32 / LPR;              // tokens of a warp's load
     static constexpr int ROWS_REGS = 136, OTHER_REGS = 120;       // 256 x 136 + 256 x 120 = 512 x 128
-    static constexpr int INFO = 36, RING = 8;         // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN; where they lie
-    // factors of rows, info of RING steps, maxima of scales, barriers, address of TMEM, flag
-    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + RING * INFO * 4, OFF_BAR = OFF_MAX + 32, OFF_TMEM = OFF_BAR + 30 * 8, SMEM = OFF_TMEM + 16;
+    static constexpr int INFO = 36, RING = 8;         // words of a step: scales of K, lv, 2^-(lv + 6) of 16 tokens each, which of them there are, which have scales of NaN or far below VS; where they lie
+    // factors of rows, info of RING steps, maxima and minima of scales, barriers, address of TMEM, flag
+    static constexpr int OFF_INFO = OFF_REST + ROWS * 4, OFF_MAX = OFF_INFO + RING * INFO * 4, OFF_BAR = OFF_MAX + 64, OFF_TMEM = OFF_BAR + 30 * 8, SMEM = OFF_TMEM + 16;
 };
 struct KvPromptBars {
     uint32_t at;
@@ -119,6 +121,11 @@ struct KvPromptSteps {
     __device__ __forceinline__ bool active(int k) const { return k < to && (k < sink || k >= from); }
     __device__ __forceinline__ bool whole(int k) const { return k >= whole_from && k < whole_to; }
 };
+
+// lv of a page whose scale of V is 0: below all others' by more than a weight can make up for.
+constexpr float kKvNoScale = -400.0f;
+// Pages whose scale is below this part of the largest are far below it.
+constexpr float kKvFar = 0x1p-80f;
 
 // The largest of the seven warps' numbers.
 __device__ __forceinline__ float kv_prompt_top(const float* part) {
@@ -198,9 +205,10 @@ __device__ __forceinline__ int kv_prompt_block(const KvArgs& c, const KvPromptTi
     return (int)((((unsigned)page * (unsigned)c.heads + (unsigned)tile.h) << (c.page_log2 - 4)) + (unsigned)((t & (c.page - 1)) >> 4));
 }
 
-// ---- warps 0 .. 7, while the first codes are on their way: q as f16, a power of two for each row
+// ---- warps 0 .. 7, while the first codes are on their way: q as f16, a power of two for each row.  Says whether the CTA sees scales far below the largest (1, or 0; -1: given up), which it reads before q counts as
+// written: the steps' information is not written anew until then.
 template <typename F>
-__device__ __forceinline__ void kv_prompt_queries(const KvAttendArgs& a, const KvPromptTile& tile, const KvPromptBars& bar, uint8_t* smem) {
+__device__ __forceinline__ int kv_prompt_queries(const KvAttendArgs& a, const KvPromptTile& tile, const KvPromptBars& bar, uint8_t* smem, volatile int* abort_flag) {
     constexpr int LPR = F::LPR, TPL = F::TPL;
     const KvArgs& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, which = lane % LPR, in_group = lane / LPR, column = which * 16, chunk = (which & 3) * 2;
@@ -251,7 +259,10 @@ __device__ __forceinline__ void kv_prompt_queries(const KvAttendArgs& a, const K
             *reinterpret_cast<uint4*>(to + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
         }
     }
+    if (!kv_wait(a, bar.info_full(0), 0, abort_flag)) return -1;
+    const int any_far = (reinterpret_cast<const volatile int*>(smem + F::OFF_INFO)[25] >> 24) & 1;
     kv_written(bar.q_full());
+    return any_far;
 }
 
 // ---- warps 8 .. 11 and 13 .. 15: the largest scale of V; K, V and what each step's pages say.  Codes are on their way a step ahead.
@@ -276,16 +287,18 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         ks = page >= 0 ? c.k_scale[(long long)page * c.heads + tile.h] : 0.0f;
         vsc = page >= 0 ? c.v_scale[(long long)page * c.heads + tile.h] : 0.0f;
     };
-    auto tell = [&](int k, float vs) {
+    auto tell = [&](int k, float vs, bool any_far) {
         float* i = info + (k & (F::RING - 1)) * F::INFO;
-        const float lv = fminf(fmaxf(vs > 0.0f ? __log2f(fabsf(vsc) / vs) : 0.0f, -24.0f), 0.0f);      // (of NaN -24)
         const bool k_nan = ks != ks, v_nan = vsc != vsc;
-        const unsigned there = __ballot_sync(0xffffffffu, page >= 0), bad_k = __ballot_sync(0xffffffffu, k_nan), bad_v = __ballot_sync(0xffffffffu, v_nan);
+        const float ratio = page >= 0 && vs > 0.0f && !v_nan ? fabsf(vsc) / vs : 1.0f;
+        const bool deep = ratio < kKvFar;             // (where the quotient may be below the least number, the logarithms are not: 2^-277 at the least, and for 0 something less)
+        const float lv = deep ? fmaxf(__log2f(fabsf(vsc) * 0x1p64f) - 64.0f - __log2f(vs), kKvNoScale) : fminf(__log2f(ratio), 0.0f);
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0), bad_k = __ballot_sync(0xffffffffu, k_nan), bad_v = __ballot_sync(0xffffffffu, v_nan), far = __ballot_sync(0xffffffffu, deep);
         if (lane < 8) {
-            i[lane] = k_nan ? 0.0f : fabsf(ks); i[8 + lane] = lv; i[16 + lane] = ex2(-lv - 6.0f);
+            i[lane] = k_nan ? 0.0f : fabsf(ks); i[8 + lane] = lv; i[16 + lane] = deep ? 0.0f : ex2(-lv - 6.0f);
             reinterpret_cast<int*>(i)[28 + lane] = kv_prompt_block(c, tile, steps, k, page);
         }
-        if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8)); }
+        if (lane == 0) { reinterpret_cast<int*>(i)[24] = (int)(there & 255u); reinterpret_cast<int*>(i)[25] = (int)((bad_k & 255u) | ((bad_v & 255u) << 8) | ((far & 255u) << 16) | (any_far ? 1u << 24 : 0u)); }
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar.info_full(k & (F::RING - 1)));
     };
@@ -297,26 +310,32 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
     kc.load(c.k, first_block, warp, c.dim, in_group, column, mine);
     vc.load(c.v, first_block, warp, c.dim, in_group, column, mine);
 
-    float top = 0.0f;
+    float top = 0.0f, least = INFINITY;
     if (steps.total > 0) {
         const int low = tile.low0, high = tile.last(), from = a.window > 0 ? max(low - a.window + 1, 0) >> pl : 0, to = (high >> pl) + 1;
         const int sink_pages = a.sinks > 0 ? min(((a.sinks - 1) >> pl) + 1, from) : 0;
 #pragma unroll 2
         for (int i = warp * 32 + lane; i < sink_pages + to - from; i += 224) {
             const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
-            if (id >= 0) top = fmaxf(top, fabsf(c.v_scale[id * c.heads + tile.h]));
+            if (id >= 0) {
+                const float scale = fabsf(c.v_scale[id * c.heads + tile.h]);
+                top = fmaxf(top, scale);
+                least = fminf(least, scale);
+            }
         }
     }
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-    if (lane == 0) part[warp] = top;
+    least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
+    if (lane == 0) { part[warp] = top; part[8 + warp] = -least; }
 
     __syncwarp();
     ptx::named_barrier_sync(1, 224);                  // (in front of any wait that may be given up)
     const float vs = kv_prompt_top(part);
+    const bool any_far = -kv_prompt_top(part + 8) * (1.0f / kKvFar) < vs;
     if (warp == 6) {
-        tell(0, vs);
+        tell(0, vs, any_far);
         look(1);
-        tell(1, vs);
+        tell(1, vs, false);
         look(2);
     }
 
@@ -330,7 +349,7 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         kv_written(bar.k_full(u & 1));
         kc.load(c.k, blocks(u + 1), warp, c.dim, in_group, column, mine);
         if (warp == 6 && u % F::UNITS == 0) {
-            tell(k + 2, vs);
+            tell(k + 2, vs, false);
             look(k + 3);
         }
         if (!kv_wait(a, bar.v_empty(u & 1), free_parity, abort_flag)) return;
@@ -427,11 +446,15 @@ __device__ __forceinline__ void kv_prompt_mma(const KvAttendArgs& a, const KvPro
     }
 }
 
-// Weights of a row's 64 scores in tensor memory at `ts` (minus infinity: not seen), in pairs, under the base `base` (log2): p, their sum with each page's factor taken out, and
-// the largest exponent.
-__device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* info, float factor, float base, uint32_t (&p)[32], float& sum) {
+// What scores are multiplied with: not 0, so that minus infinity stays what it is.
+__device__ __forceinline__ float kv_prompt_factor(float f) { return f == 0.0f ? 1e-38f : f; }
+
+// Weights of a row's 64 scores in tensor memory at `ts` (minus infinity: not seen), in pairs, under the base `base` (log2): p, their sum with each page's factor taken out (without pages far below VS, whose
+// factor is none), and the largest exponents over the base, with the pages' scales (the result) and, of DEEP, without (`top_x`).
+template <bool DEEP>
+__device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* info, float factor, float base, uint32_t (&p)[32], float& sum, float& top_x) {
     uint32_t v[64];
-    float top = -INFINITY;
+    float top = -INFINITY, plain = -INFINITY;
     sum = 0.0f;
     ptx::tmem_ld32(ts, v);
     ptx::tmem_ld32(ts + 32, v + 32);
@@ -439,8 +462,7 @@ __device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* inf
     ptx::tmem_wait_ld32(v + 32);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {                     // 16 tokens, which are on one page
-        float f = factor * info[g];
-        f = f == 0.0f ? 1e-38f : f;                   // (minus infinity stays what it is)
+        const float f = kv_prompt_factor(factor * info[g]);
         const float lv = info[8 + g], b = lv + 6.0f - base;
         const unsigned long long f2 = ptx::pack2(f, f), b2 = ptx::pack2(b, b);
         unsigned long long s2 = 0;
@@ -453,10 +475,12 @@ __device__ __forceinline__ float kv_prompt_weights(uint32_t ts, const float* inf
             s2 = ptx::add2(s2, ptx::pack2(w.x, w.y));
             p[8 * g + y] = pack_f16(w.x, w.y);
         }
-        top = fmaxf(top, most - lv);
+        top = fmaxf(top, most);
+        if (DEEP) plain = fmaxf(plain, most - lv);
         const float2 s1 = ptx::unpack2(s2);
         sum = fmaf(s1.x + s1.y, info[16 + g], sum);
     }
+    top_x = plain - 6.0f;
     return top - 6.0f;
 }
 // The first n of 32 columns.
@@ -468,7 +492,7 @@ __device__ __forceinline__ uint32_t first_columns(int n) { return n >= 32 ? 0xff
 // others) it is taken again.  (A pass for the maximum in front: twice the time.)  Steps that a row sees in part have minus infinity written over the other scores first, so that there is one
 // form of the pass, which is what the instruction cache has to hold (with a second form for such steps beside it: 7000 clocks a step where this one takes 3300).  Pages with a scale of NaN count as
 // zeros; the rows that see them are noted and get their NaN at the end.
-template <typename F>
+template <typename F, bool DEEP>
 __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, uint32_t tmem, volatile int* abort_flag) {
     constexpr int DP = F::DP;
     const KvArgs& c = a.c;
@@ -476,7 +500,8 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, to = tmem + 256 + x * DP + lanes;
     const float* all_info = reinterpret_cast<const float*>(smem + F::OFF_INFO);
     const int row = tile.row0 + min(mine, tile.rows - 1), pos = max(tile.first + row / a.group, -1);
-    float factor = 0.0f, m = -INFINITY, l = 0.0f;
+    float factor = 0.0f, M = -INFINITY, l = 0.0f;       // l: the sum of 2^(x - M), of DEEP of 2^(x - m)
+    float m = -INFINITY;
     const KvPromptSteps own(steps, tile.low(x), tile.high(x), a.window, a.sinks);
     int count = 0, spoilt = 0;                        // halves so far; 1: by a page's scale of K, 2: of V
     if (own.to > 0) {
@@ -492,7 +517,7 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
         // (what the step's pages say was said before its K was there)
         const float* info = all_info + (k & (F::RING - 1)) * F::INFO;
         const int2 pages = *reinterpret_cast<const int2*>(info + 24);
-        if (pages.x != 255 || pages.y != 0 || !own.whole(k)) {
+        if (pages.x != 255 || (pages.y & 0xffff) != 0 || !own.whole(k)) {
             const int there = pages.x >> (4 * b), k_nan = pages.y >> (4 * b), v_nan = pages.y >> (8 + 4 * b);       // of the half's four 16 tokens
             const int t = steps.at(k, 128) + 64 * b, upto = pos - t, behind = (a.window == 0 ? -1 : max(pos - a.window, -1)) - t, sunk = a.sinks - t;       // columns seen: <= upto, and > behind or < sunk
 #pragma unroll 1
@@ -516,12 +541,18 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
         float sum;
 #pragma unroll 1
         for (int again = 0; again < 2; ++again) {
-            const float base = m == -INFINITY ? 0.0f : m, top = kv_prompt_weights(ts, info + 4 * b, factor, base, p, sum);
-            const bool raise = m == -INFINITY ? top > -INFINITY : top > 8.0f;
+            float top_x;
+            const float base = M == -INFINITY ? 0.0f : M, top = kv_prompt_weights<DEEP>(ts, info + 4 * b, factor, base, p, sum, top_x);
+            const bool raise = M == -INFINITY ? top > -INFINITY : (top > 8.0f || (DEEP && base + top_x > m + 60.0f));       // (m only keeps the sum in range)
             if (again || !__any_sync(0xffffffffu, raise)) break;
-            const bool more = raise || top > 0.0f;    // (a row that has grown at all goes along)
-            const float to_m = base + top, f = more ? (m == -INFINITY ? 0.0f : ex2(m - to_m)) : 1.0f;
-            if (more) { l *= f; m = to_m; }
+            // rows that have grown at all go along
+            const float M_now = fmaxf(M, base + top), f = M_now == M ? 1.0f : ex2(M - M_now);
+            M = M_now;
+            if (DEEP) {
+                const float m_now = fmaxf(m, base + top_x);
+                l *= m_now == m ? 1.0f : ex2(m - m_now);
+                m = m_now;
+            } else l *= f;
             if (count > 0) {
                 // the half before is in the sums (the one before that was, or this one's scores would not have had room)
                 if (!kv_wait(a, bar.pv_done(x), (uint32_t)(count - 1) & 1u, abort_flag)) return;
@@ -537,7 +568,22 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
                 }
             }
         }
-        l += sum;
+        if (!DEEP) l += sum;
+        else {
+            const float over = M == -INFINITY ? 1.0f : ex2(0.5f * (M - m)), bx = m == -INFINITY ? 0.0f : m;       // (its square may be too small where the product is not)
+            l = fmaf(sum * over, over, l);
+            int far = (reinterpret_cast<const volatile int*>(info)[25] >> (16 + 4 * b)) & 15;       // (the same for all rows) pages far below VS: their weights by themselves
+#pragma unroll 1
+            for (int g = 0; far != 0; ++g, far >>= 1) {
+                if (!(far & 1)) continue;
+                uint32_t v[16];
+                ptx::tmem_ld16(ts + g * 16, v);
+                tmem_wait_ld16(v);
+                const float f = kv_prompt_factor(factor * info[4 * b + g]);
+#pragma unroll
+                for (int y = 0; y < 16; ++y) l += ex2(fmaf(__uint_as_float(v[y]), f, -bx));
+            }
+        }
 #pragma unroll
         for (int g = 0; g < 2; ++g) tmem_st16(ts + g * 16, p + 16 * g);
         tmem_wait_st();
@@ -554,7 +600,12 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     const float vs = count > 0 ? kv_prompt_top(part) : 0.0f;
     const bool mine_there = mine < tile.rows;
     if (spoilt & 1) l = __uint_as_float(0x7fffffffu);
-    const float out_scale = spoilt ? __uint_as_float(0x7fffffffu) : (l == 0.0f ? 0.0f : vs * (1.0f / 64.0f) / l);
+    float out_scale = l == 0.0f ? 0.0f : vs * (1.0f / 64.0f) / l;
+    if (DEEP) {                                       // VS 2^(M - m) is a scale that the row has seen, or more than a weight below one: the power in four factors, none of which is too small
+        const float quarter = l == 0.0f ? 0.0f : ex2(0.25f * (M - m));
+        out_scale = out_scale * quarter * quarter * quarter * quarter;
+    }
+    if (spoilt) out_scale = __uint_as_float(0x7fffffffu);
     const long long token = tile.row + row / a.group, head = tile.h * a.group + row % a.group, at = token * a.out_stride + head * c.dim;
 #pragma unroll
     for (int g = 0; g < DP / 16; ++g) {
@@ -589,7 +640,7 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
             }
         }
     }
-    if (a.lse && mine_there) a.lse[token * a.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    if (a.lse && mine_there) a.lse[token * a.heads + head] = l == 0.0f ? -INFINITY : ((DEEP ? m : M) + log2f(l)) * kLn2;
 }
 
 template <int DP>
@@ -640,8 +691,9 @@ __global__ void __launch_bounds__(KvPromptCfg<DP>::THREADS, 1) kv_prompt_kernel(
         const KvSteps steps(tile.low0, tile.last(), a.window, a.sinks, 128);
         if (warp < 8) {
             set_registers_up<F::ROWS_REGS>();
-            kv_prompt_queries<F>(a, tile, bar, smem);
-            kv_prompt_rows<F>(a, tile, steps, bar, smem, tmem, abort_flag);
+            const int far = kv_prompt_queries<F>(a, tile, bar, smem, abort_flag);
+            if (far == 0) kv_prompt_rows<F, false>(a, tile, steps, bar, smem, tmem, abort_flag);
+            else if (far == 1) kv_prompt_rows<F, true>(a, tile, steps, bar, smem, tmem, abort_flag);
         } else {
             set_registers_down<F::OTHER_REGS>();
             if (warp != 12) kv_prompt_convert<F>(a, tile, steps, bar, smem, abort_flag);
