@@ -18,7 +18,7 @@ def test_lanes_come_together_in_front_of_instructions_of_the_whole_warp():
     """tcgen05.ld and bar.sync are executed by all lanes of a warp at once: behind stores of single lanes stands a warp barrier."""
     text = source("kv_prompt.cuh")
     rows = text[text.index("void kv_prompt_rows("):text.index("kv_prompt_kernel(const __grid_constant__")]
-    end = rows[rows.index("const float out_scale"):]
+    end = rows[rows.index("float out_scale"):]
     assert re.search(r"uint32_t v\[16\];\s*__syncwarp\(\);\s*if \(count > 0\) \{\s*ptx::tmem_ld16\(", end) and end.count("tmem_ld16(") == 1
     for m in re.finditer(r"named_barrier_sync\(", text):
         assert re.search(r"__syncwarp\(\);\s*ptx::$", text[:m.start()])
