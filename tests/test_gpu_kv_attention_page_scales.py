@@ -68,9 +68,9 @@ def times(cache, pages, bits):
     cache.scales[1][pages] = np.ldexp(cache.scales[1][pages], bits)
 
 
-@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("bits", [10, 20, 24, 30, 40, 80, 99, 120, 150])
-@pytest.mark.parametrize("new,length,dim,page,window", [(160, 160, 64, 16, 0), (160, 160, 128, 16, 0), (200, 250, 128, 64, 60), (150, 150, 256, 32, 0)])
+@pytest.mark.parametrize("new,length,dim,page,window", [(160, 160, 64, 16, 0), (160, 160, 128, 16, 0), (200, 250, 128, 64, 60), (150, 150, 256, 32, 0), (5, 69, 64, 64, 0), (6, 122, 128, 16, 40)])
 def test_quiet_pages_beside_loud_ones(ctx, zb, new, length, dim, page, window, bits, kind):
     """Quiet pages first, or loud ones that a window leaves behind: some rows see quiet ones alone."""
     pages = -(-length // page)
@@ -83,8 +83,8 @@ def test_quiet_pages_beside_loud_ones(ctx, zb, new, length, dim, page, window, b
     compare(ctx, zb, new, length, 4, 2, dim, page, kind, change, window=window)
 
 
-@pytest.mark.parametrize("kind", ["bf16"])
-@pytest.mark.parametrize("new", [140])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("new", [1, 140])
 @pytest.mark.parametrize("bits", [20, 40, 70, 110])
 @pytest.mark.parametrize("first", [True, False])
 def test_a_loud_page_that_nobody_attends_to(ctx, zb, new, bits, first, kind):
@@ -100,15 +100,15 @@ def test_a_loud_page_that_nobody_attends_to(ctx, zb, new, bits, first, kind):
     compare(ctx, zb, new, length, 4, 2, 64, page, kind, change, scale=1.0)
 
 
-@pytest.mark.parametrize("kind", ["bf16"])
-@pytest.mark.parametrize("new", [140])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("new", [1, 5, 140])
 @pytest.mark.parametrize("bits", [-116, -110, -60, 60, 110])
 def test_all_pages_alike(ctx, zb, new, bits, kind):
     compare(ctx, zb, new, 200, 4, 2, 64, 16, kind, lambda cache, pages, q: times(cache, pages, bits))
 
 
-@pytest.mark.parametrize("kind", ["f16", "bf16"])
-@pytest.mark.parametrize("new", [140])
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("new", [1, 140])
 @pytest.mark.parametrize("page", [16, 64])
 def test_scales_of_zero(ctx, zb, new, page, kind):
     """Their codes count as zeros, whatever they are, and their weights are in the sum."""
@@ -117,11 +117,11 @@ def test_scales_of_zero(ctx, zb, new, page, kind):
     compare(ctx, zb, new, 260, 4, 2, 128, page, kind, change)
 
 
-@pytest.mark.parametrize("new", [140])
+@pytest.mark.parametrize("new", [1, 140])
 def test_every_page_its_own(ctx, zb, new):
     """Scales over the whole range of fp32, sums across pages of all of them."""
     def change(cache, pages, q):
         for i, p in enumerate(pages):
             times(cache, [p], -100 + (i * 37) % 200)
-    for kind in ("bf16",):
+    for kind in ("bf16", "f32"):
         compare(ctx, zb, new, 400, 4, 2, 64, 16, kind, change)

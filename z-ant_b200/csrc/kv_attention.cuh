@@ -10,8 +10,9 @@
 //
 // K stays int8: q goes in as whole numbers whose largest in a row is about 2^20 (of F32 2^27), in 3 (4) digits of 7 bits, whose products are int8 products with exact
 // sums; a value of q loses 2^-20 of the largest of its row at most (2^-27).  K in f16 took 96 more ALU instructions of 510 for a step, and ALU is the busiest pipe.
-// V becomes f16 on the way (exactly) and P is rounded to f16 (2^-11 relative, for results in 16 bits; of F32 the sum of two f16 numbers), each weight times its page's scale
-// over the largest scale so far, times 2^14, so that what is rounded is at most 2^14 and weights down to 2^-28 keep their 11 bits.  Statistics and sums are fp32.
+// V becomes f16 on the way (exactly) and P is rounded to f16 (2^-11 relative, for results in 16 bits; of F32 the sum of two f16 numbers): each weight times its page's scale, over the largest such
+// product M of its row, times 2^9 to 2^15 (M is raised when it has grown by 2^6), so that 2^-23 of a row's largest keeps its 11 bits whatever the scales of pages are that only other rows see.  Statistics and
+// sums are fp32; scales below 2^-104 keep fewer bits.
 //
 // Memory is the bound (a cached token of 128 dimensions is 256 bytes for 4 x 8 x 128 operations of 8 rows).  Each warp takes every so many'th step of 32 tokens (16 of
 // 256 dimensions), which its first lane brings by TMA into a ring of the warp's own, swizzled so that the lanes' 16-byte reads meet no bank twice.  No warp waits for
@@ -129,6 +130,9 @@ __device__ __forceinline__ int kv_rows_of(const KvAttendArgs& a, int n) {
 }
 // Some row at positions [low, high] sees one of the 16 tokens from t on.  (What the table says of others, and their pages' scales, is nobody's business.)
 __device__ __forceinline__ bool kv_seen16(int t, int low, int high, int window, int sinks) { return t <= high && (window == 0 || t + 15 > low - window || t < sinks); }
+
+// The maximum of a row that has seen nothing: a number, so that differences are numbers, and below all scores.
+constexpr float kKvNothing = -1e30f;
 
 template <int DP_, int NT_, bool SPLIT_>
 struct KvAttendCfg {
@@ -347,11 +351,24 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         }
 
     float o[MT][NT][4];
-    float m[NT][2], l[NT][2], vs = 0.0f, over = 0.0f;     // over: 2^14 / vs
+    // A row's M is its largest x + log2(scale of V), as of when that had last grown by 2^6, and o the sum of 2^(x - M + 9) times the scale times codes: in factors 2^(x - m), which l sums, and the scale times
+    // `up`, 2^(9 + m - M).  m is the largest x of that time; it only keeps the factors in range.
+    float m[NT][2], M[NT][2], l[NT][2], up_top = 0.0f, up_low = INFINITY;       // (the largest and the least up of the lane's rows)
+    // (of 32 rows taken anew each time, for the registers' sake)
+    constexpr bool KEEP_UP = NT < 4;
+    float kept[KEEP_UP ? NT : 1][2];
+    auto up_of = [&](int n, int i) { return KEEP_UP ? kept[KEEP_UP ? n : 0][i] : ex2(9.0f + m[n][i] - M[n][i]); };
+    auto set_up = [&](int n, int i) {
+        const float up = ex2(9.0f + m[n][i] - M[n][i]);
+        if (KEEP_UP) kept[KEEP_UP ? n : 0][i] = up;
+        up_top = fmaxf(up_top, up);
+        up_low = fminf(up_low, up);
+    };
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        m[n][0] = m[n][1] = -INFINITY;
+        m[n][0] = m[n][1] = M[n][0] = M[n][1] = kKvNothing;
         l[n][0] = l[n][1] = 0.0f;
+        if (KEEP_UP) kept[KEEP_UP ? n : 0][0] = kept[KEEP_UP ? n : 0][1] = 0.0f;
 #pragma unroll
         for (int j = 0; j < MT; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
     }
@@ -438,56 +455,84 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
                         if (!seen) x[half][n][i] = -INFINITY;
                     }
         }
-        // the running maximum of each row, and the largest scale of V
+        // the largest x + log2(scale of V) of each row
+        float lv[H], va[H];
+#pragma unroll
+        for (int half = 0; half < H; ++half) {
+            va[half] = half == 0 || two ? fmaxf(fabsf(vsc[half]), 0.0f) : va[0];       // (of NaN 0)
+            lv[half] = half == 0 || two ? __log2f(va[half]) : lv[0];       // (of 0 minus infinity)
+        }
+        const float v_top = fmaxf(ok[0] ? va[0] : 0.0f, ok[H - 1] ? va[H - 1] : 0.0f), v_low = fminf(ok[0] ? va[0] : INFINITY, ok[H - 1] ? va[H - 1] : INFINITY);
+        // (no factor leaves the numbers: of a row that is not raised x + lv is at most M + 6, and 2^(x - m) at most 2^15 over the other factor, 2^27)
         float to[NT][2];
-        bool raise = false;
+        bool raise = !(v_top * up_top <= 0x1p110f && v_low * up_low >= 0x1p-12f);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float v = fmaxf(x[0][n][i], x[0][n][i + 2]);
-                if (H > 1) v = fmaxf(v, fmaxf(x[H - 1][n][i], x[H - 1][n][i + 2]));
+                float v = fmaxf(x[0][n][i], x[0][n][i + 2]) + lv[0];
+                if (H > 1) v = fmaxf(v, fmaxf(x[H - 1][n][i], x[H - 1][n][i + 2]) + lv[H - 1]);
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-                to[n][i] = fmaxf(m[n][i], v);
-                raise |= to[n][i] > m[n][i];
+                to[n][i] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                raise |= to[n][i] > M[n][i] + 6.0f;
             }
-        const float vs_to = fmaxf(vs, fmaxf(fabsf(vsc[0]), fabsf(vsc[H - 1])));
-        if (__any_sync(0xffffffffu, raise || vs_to > vs)) {
-            const float fv = vs_to > 0.0f ? vs / vs_to : 1.0f;
+        bool odd = false;                             // weights below 2^-170 at the most: none
+        if (__any_sync(0xffffffffu, raise)) {
+            up_top = 0.0f; up_low = INFINITY;
+            const float lv_top = __log2f(v_top);
+            const bool near = v_top > 0.0f && v_top <= 16.0f * v_low;       // of the step's pages: the largest x is found from x + lv, or 4 more
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float f = m[n][i] == to[n][i] ? 1.0f : ex2(m[n][i] - to[n][i]);
-                    l[n][i] *= f;
-                    m[n][i] = to[n][i];
+                    float v = to[n][i] - lv_top;
+                    if (!near) {
+                        v = fmaxf(x[0][n][i], x[0][n][i + 2]);
+                        if (H > 1) v = fmaxf(v, fmaxf(x[H - 1][n][i], x[H - 1][n][i + 2]));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                    }
+                    const float m_now = fmaxf(m[n][i], v), M_now = fmaxf(fmaxf(M[n][i], to[n][i]), m_now - 104.0f);       // (scales below 2^-104 have no say in M: up is a number)
+                    const float f = ex2(M[n][i] - M_now);
+                    l[n][i] *= ex2(m[n][i] - m_now);
+                    m[n][i] = m_now;
+                    M[n][i] = M_now;
+                    set_up(n, i);
 #pragma unroll
-                    for (int j = 0; j < MT; ++j) { o[j][n][i] *= f * fv; o[j][n][i + 2] *= f * fv; }
+                    for (int j = 0; j < MT; ++j) { o[j][n][i] *= f; o[j][n][i + 2] *= f; }
                 }
-            vs = vs_to;
-            over = vs > 0.0f ? 16384.0f / vs : 0.0f;
+            // A scale 2^80 above those that a row's M is made of, so that its weights, if any, are below 2^-74 there: m goes down for them, but l stays in range.
+            if (__any_sync(0xffffffffu, v_top * up_top > 0x1p100f)) {
+                up_top = 0.0f; up_low = INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float m_now = fminf(m[n][i], fmaxf(M[n][i] + 80.0f - lv_top, m[n][i] - 60.0f));
+                        l[n][i] *= ex2(m[n][i] - m_now);
+                        m[n][i] = m_now;
+                        set_up(n, i);
+                    }
+                odd = __any_sync(0xffffffffu, v_top * up_top > 0x1p126f);
+            }
         }
-        float base[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) base[n][i] = m[n][i] == -INFINITY ? 0.0f : m[n][i];
 #pragma unroll
         for (int half = 0; half < H; ++half) {
-            const float vf = vsc[half] * over;
-            const bool plain = vf == vf;              // (a scale of NaN: only of what is seen)
+            const float scale = ok[half] ? vsc[half] : 0.0f;
+            const bool plain = scale == scale && !odd;       // (a scale of NaN: only of what is seen)
             uint32_t b[NT][2], d[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float p[4];
+                const float factors[2] = {scale * up_of(n, 0), scale * up_of(n, 1)};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = ex2(x[half][n][i] - base[n][i & 1]);
+                    const float e = ex2(x[half][n][i] - m[n][i & 1]);
                     l[n][i & 1] += e;
-                    p[i] = e * vf;
-                    if (!plain) p[i] = e == 0.0f ? 0.0f : p[i];
+                    p[i] = e * factors[i & 1];
+                    if (!plain) p[i] = e == 0.0f || factors[i & 1] > 0x1p126f ? 0.0f : p[i];
                 }
                 b[n][0] = pack_f16(p[0], p[1]);
                 b[n][1] = pack_f16(p[2], p[3]);
@@ -546,7 +591,10 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
             v += __shfl_xor_sync(0xffffffffu, v, 16);
             if (l4 == 0) {
                 float* s = stat + (warp * F::ROWS + r) * 3;
-                s[0] = m[n][i]; s[1] = v; s[2] = vs * (1.0f / 16384.0f);
+                // (m becomes what l is next to)
+                const int e = v > 0.0f && v < INFINITY ? min((int)(__float_as_uint(v) >> 23) - 127, 126) : 0;
+                const float u = up_of(n, i), down = __uint_as_float((uint32_t)(127 - e) << 23);
+                s[0] = m[n][i] == kKvNothing ? -INFINITY : m[n][i] + (float)e; s[1] = v * down; s[2] = u > 0.0f ? __fdividef(down, u) : 0.0f;
             }
             float* to = sums + (warp * F::ROWS + r) * F::PITCH;
 #pragma unroll
