@@ -108,6 +108,9 @@ __device__ __forceinline__ void kv_values16(const void* p, int type, bool wide, 
     for (int i = 0; i < 16; ++i) f[i] = kv_value(p, type, at + i);
 }
 
+// A page's scale; one that is no finite number is NaN.
+__device__ __forceinline__ float kv_scale(float s) { return fabsf(s) < INFINITY ? s : __uint_as_float(0x7fffffffu); }
+
 // The tokens that a tile of rows at positions [low, high] sees, in steps of S tokens: sinks first, then the window (or all).
 struct KvSteps {
     int sink, first, total;                           // steps of sinks alone, the first step behind them, all
@@ -251,6 +254,11 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
         }
         return b;
     };
+    // (when they are needed: as they come they would be waited for)
+    auto settle = [&](Batch& b) {
+#pragma unroll
+        for (int z = 0; z < H; ++z) { b.k[z] = kv_scale(b.k[z]); b.v[z] = kv_scale(b.v[z]); }
+    };
     Batch cur = batch_of(0), nxt;
     // Step i of the warp goes into the ring, by its first lane.
     auto issue = [&](int i, int stage, const Batch& b) {
@@ -388,6 +396,7 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
     for (int k = k0, i = 0; k < steps.total; k += stride_k, ++i) {
         if ((i & 31) == 0) {
             if (i > 0) cur = nxt;
+            settle(cur);
             nxt = batch_of(i + 32);
         }
         __syncwarp();                                 // the warp has read the stage that is filled now
@@ -521,7 +530,7 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
 #pragma unroll
         for (int half = 0; half < H; ++half) {
             const float scale = ok[half] ? vsc[half] : 0.0f;
-            const bool plain = scale == scale && !odd;       // (a scale of NaN: only of what is seen)
+            const bool plain = scale == scale && !odd;       // (a scale of NaN: of all that is seen, also with a weight of nothing)
             uint32_t b[NT][2], d[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -532,7 +541,7 @@ kv_attention_kernel(const __grid_constant__ KvAttendArgs a, const __grid_constan
                     const float e = ex2(x[half][n][i] - m[n][i & 1]);
                     l[n][i & 1] += e;
                     p[i] = e * factors[i & 1];
-                    if (!plain) p[i] = e == 0.0f || factors[i & 1] > 0x1p126f ? 0.0f : p[i];
+                    if (!plain) p[i] = x[half][n][i] == -INFINITY || factors[i & 1] > 0x1p126f ? 0.0f : p[i];
                 }
                 b[n][0] = pack_f16(p[0], p[1]);
                 b[n][1] = pack_f16(p[2], p[3]);

@@ -289,7 +289,7 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
     };
     auto tell = [&](int k, float vs, bool any_far) {
         float* i = info + (k & (F::RING - 1)) * F::INFO;
-        const bool k_nan = ks != ks, v_nan = vsc != vsc;
+        const bool k_nan = !(fabsf(ks) < INFINITY), v_nan = !(fabsf(vsc) < INFINITY);
         const float ratio = page >= 0 && vs > 0.0f && !v_nan ? fabsf(vsc) / vs : 1.0f;
         const bool deep = ratio < kKvFar;             // (where the quotient may be below the least number, the logarithms are not: 2^-277 at the least, and for 0 something less)
         const float lv = deep ? fmaxf(__log2f(fabsf(vsc) * 0x1p64f) - 64.0f - __log2f(vs), kKvNoScale) : fminf(__log2f(ratio), 0.0f);
@@ -318,7 +318,7 @@ __device__ __forceinline__ void kv_prompt_convert(const KvAttendArgs& a, const K
         for (int i = warp * 32 + lane; i < sink_pages + to - from; i += 224) {
             const long long id = kv_page(c, tile.s, i < sink_pages ? i : i - sink_pages + from);
             if (id >= 0) {
-                const float scale = fabsf(c.v_scale[id * c.heads + tile.h]);
+                const float scale = fabsf(kv_scale(c.v_scale[id * c.heads + tile.h]));       // (NaN is neither the largest nor the least)
                 top = fmaxf(top, scale);
                 least = fminf(least, scale);
             }
@@ -491,7 +491,7 @@ __device__ __forceinline__ uint32_t first_columns(int n) { return n >= 32 ? 0xff
 // The base of the exponents is the maximum of earlier steps: one pass over the scores gives weights and their maximum, and only where that has grown by 2^8 (a row's first step, and few
 // others) it is taken again.  (A pass for the maximum in front: twice the time.)  Steps that a row sees in part have minus infinity written over the other scores first, so that there is one
 // form of the pass, which is what the instruction cache has to hold (with a second form for such steps beside it: 7000 clocks a step where this one takes 3300).  Pages with a scale of NaN count as
-// zeros; the rows that see them are noted and get their NaN at the end.
+// zeros, and so do rows of q with one; the rows that see such a page, or anything, are noted and get their NaN at the end.
 template <typename F, bool DEEP>
 __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPromptTile& tile, const KvSteps& steps, const KvPromptBars& bar, uint8_t* smem, uint32_t tmem, volatile int* abort_flag) {
     constexpr int DP = F::DP;
@@ -503,10 +503,11 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     float factor = 0.0f, M = -INFINITY, l = 0.0f;       // l: the sum of 2^(x - M), of DEEP of 2^(x - m)
     float m = -INFINITY;
     const KvPromptSteps own(steps, tile.low(x), tile.high(x), a.window, a.sinks);
-    int count = 0, spoilt = 0;                        // halves so far; 1: by a page's scale of K, 2: of V
+    int count = 0, spoilt = 0;                        // halves so far; 1: by a page's scale of K, or by q, 2: of V
     if (own.to > 0) {
         if (!kv_wait(a, bar.q_full(), 0, abort_flag)) return;
         factor = reinterpret_cast<const float*>(smem + F::OFF_REST)[mine];
+        if (!(factor < INFINITY)) { factor = 0.0f; spoilt = 1; }
     }
     for (int j = 0; j < 2 * own.to; ++j) {            // halves of steps
         const int k = j >> 1, b = j & 1;
@@ -599,6 +600,7 @@ __device__ __forceinline__ void kv_prompt_rows(const KvAttendArgs& a, const KvPr
     const float* part = reinterpret_cast<const float*>(smem + F::OFF_MAX);
     const float vs = count > 0 ? kv_prompt_top(part) : 0.0f;
     const bool mine_there = mine < tile.rows;
+    if (l == 0.0f) spoilt = 0;                        // (sees nothing)
     if (spoilt & 1) l = __uint_as_float(0x7fffffffu);
     float out_scale = l == 0.0f ? 0.0f : vs * (1.0f / 64.0f) / l;
     if (DEEP) {                                       // VS 2^(M - m) is a scale that the row has seen, or more than a weight below one: the power in four factors, none of which is too small
