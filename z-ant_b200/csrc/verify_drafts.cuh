@@ -37,6 +37,9 @@ struct VerifyShared {
     int n, begin, end, mine, found, last;
 };
 
+// A probability; what is none (NaN, negative, infinite) counts as 0.
+__device__ __forceinline__ float verify_number(float v) { return v > 0.0f && v < INFINITY ? v : 0.0f; }
+
 template <typename T>
 __global__ void __launch_bounds__(VerifyShared::THREADS) verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
     using Sh = VerifyShared;
@@ -80,9 +83,8 @@ __global__ void __launch_bounds__(VerifyShared::THREADS) verify_drafts_kernel(co
     const T* q = less && drafted ? drafted + (long long)at * a.drafted_stride : nullptr;
     const int given = less && !drafted ? a.tokens[at] : -1;
     auto mass = [&](int v) -> double {
-        double r = as_float(p[v]);
-        if (less) r -= q ? (double)as_float(q[v]) : (v == given ? 1.0 : 0.0);
-        return r > 0.0 && r < INFINITY ? r : 0.0;
+        const float pv = verify_number(as_float(p[v])), qv = !less ? 0.0f : (q ? verify_number(as_float(q[v])) : (v == given ? 1.0f : 0.0f));
+        return pv > qv ? (double)pv - (double)qv : 0.0;
     };
     // segments in order: warp w of part i has the (16 i + w)-th
     const int segs = P * Sh::SEGS;
@@ -106,8 +108,9 @@ __global__ void __launch_bounds__(VerifyShared::THREADS) verify_drafts_kernel(co
 #pragma unroll
             for (int i = 0; i < U; ++i) {
                 // (compared in fp32, which is exact: comparisons of 64 bits were the busiest instructions)
-                const bool keep = pv[i] > qv[i] && pv[i] < INFINITY && qv[i] > -INFINITY;
-                sum += (double)(keep ? pv[i] : 0.0f) - (double)(keep ? qv[i] : 0.0f);
+                const float less_by = verify_number(qv[i]);
+                const bool keep = pv[i] > less_by && pv[i] < INFINITY;
+                sum += (double)(keep ? pv[i] : 0.0f) - (double)(keep ? less_by : 0.0f);
             }
         }
 #pragma unroll
