@@ -37,8 +37,8 @@ struct VerifyShared {
     int n, begin, end, mine, found, last;
 };
 
-// A probability; what is none (NaN, negative, infinite) counts as 0.
-__device__ __forceinline__ float verify_number(float v) { return v > 0.0f && v < INFINITY ? v : 0.0f; }
+// A probability; what is none (NaN, negative, infinite) counts as 0.  (One comparison: the others' bits are not below infinity's.)
+__device__ __forceinline__ float verify_number(float v) { return __float_as_uint(v) < 0x7f800000u ? v : 0.0f; }
 
 template <typename T>
 __global__ void __launch_bounds__(VerifyShared::THREADS) verify_drafts_kernel(const __grid_constant__ VerifyArgs a) {
