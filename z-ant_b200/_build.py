@@ -17,7 +17,7 @@ NVCC_FLAGS = [
 
 
 def _newest_source():
-    newest = 0.0
+    newest = os.path.getmtime(os.path.abspath(__file__))       # the flags are in here
     for root, _dirs, files in os.walk(CSRC):
         for f in files:
             newest = max(newest, os.path.getmtime(os.path.join(root, f)))
@@ -26,11 +26,11 @@ def _newest_source():
 
 
 def _stale(target, depfile):
-    """`target` is missing or older than a file that went into it (`depfile`, as nvcc wrote it)."""
+    """`target` is missing or older than a file that went into it (`depfile`, as nvcc wrote it), or than this one, which has the flags."""
     if not os.path.exists(target) or not os.path.exists(depfile):
         return True
     with open(depfile) as f:
-        parts = f.read().replace("\\\n", " ").split(":", 1)[1].split()
+        parts = f.read().replace("\\\n", " ").split(":", 1)[1].split() + [os.path.abspath(__file__)]
     made = os.path.getmtime(target)
     return any(not os.path.exists(p) or os.path.getmtime(p) > made for p in parts)
 
