@@ -543,7 +543,8 @@ extern fn zant_b200_verify_drafts(ctx: ?*Ctx, dtype: i32, target: *const anyopaq
 /// The arrays of a cache: codes [pages, heads, page, dim], scales [pages, heads].
 pub fn kv_cache_of(k: *const Tensor(i8), k_scale: *const Tensor(f32), v: *const Tensor(i8), v_scale: *const Tensor(f32)) !KvCacheData {
     if (k.shape.len != 4 or v.shape.len != 4) return TensorError.InvalidRank;
-    if (k_scale.size != k.shape[0] * k.shape[1] or v_scale.size != k_scale.size or v.size != k.size) return TensorMathError.InputTensorsWrongShape;
+    for (k.shape, v.shape) |a, b| if (a != b) return TensorMathError.InputTensorsWrongShape;
+    if (k_scale.size != k.shape[0] * k.shape[1] or v_scale.size != k_scale.size) return TensorMathError.InputTensorsWrongShape;
     return KvCacheData{ .k = k.data.ptr, .k_scale = k_scale.data.ptr, .v = v.data.ptr, .v_scale = v_scale.data.ptr, .pages = k.shape[0], .heads = k.shape[1], .page = k.shape[2], .dim = k.shape[3] };
 }
 
