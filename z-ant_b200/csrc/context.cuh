@@ -347,9 +347,10 @@ class Stager {
     // tried then.  (Anything else that is wrong with the buffers is left to commit.)
     bool room() {
         if (foreign_ || stream_capturing(ctx_)) return true;
-        const int32_t st = arena_reserve(ctx_, layout());
-        return st != ZANT_E_ARENA_EXHAUSTED && st != ZANT_E_MEM_ERROR;
+        return reserved(layout());
     }
+    // The same of `more` bytes on top, a workspace that the call can do without (in a capture it does).
+    bool room_for(size_t more) { return !foreign_ && !stream_capturing(ctx_) && reserved(layout() + more + kArenaAlign); }
 
     // Allocates arena space for every staged slot and issues the H2D copies.
     int32_t commit() {
@@ -398,6 +399,10 @@ class Stager {
     }
 
   private:
+    bool reserved(size_t total) {
+        const int32_t st = arena_reserve(ctx_, total);
+        return st != ZANT_E_ARENA_EXHAUSTED && st != ZANT_E_MEM_ERROR;
+    }
     size_t layout() {
         size_t total = 0;
         for (int rest = 0; rest < 2; ++rest)

@@ -158,9 +158,9 @@ int32_t zant_b200_kv_cache_attention(zant_ctx* ctx, const zant_kv_cache* cache, 
         KvAttendArgs a{};
         a.c = slots.args(s, cache, rows, seqs, width);       // (sizes; pointers again when all is in place)
         a.heads = (int)heads; a.group = (int)group; a.q_type = dtype; a.window = window; a.sinks = sinks;
-        // a workspace in the arena, unless the call is captured or the arena must not grow that far
+        // a workspace in the arena, unless the call is captured or the arena may not or cannot grow that far
         size_t work = kv_work_bytes(ctx, a);
-        if (work && (stream_capturing(ctx) || (ctx->arena_limit && !s.holds(work + kArenaAlign)))) work = 0;
+        if (work && !s.room_for(work)) work = 0;
         const int iw = work ? s.scratch(work) : -1;
         ZB_TRY(s.commit());
         a.c = slots.args(s, cache, rows, seqs, width);
