@@ -668,8 +668,8 @@ int32_t zant_b200_kv_cache_read(zant_ctx* ctx, const zant_kv_cache* cache, int32
  * The token at position i sees position j where j <= i and, with window > 0, j > i - window or j < sinks; window 0 is none.  A query that sees nothing has the result 0.
  * lse [rows, heads] fp32, may be NULL: the logarithm of the sum of exp(scale * q . k_j), minus infinity where nothing is seen.
  * Weights and sums are fp32; weights are rounded to f16 in front of the product with v where the result has 16 bits, and to 22 bits where it is F32: relative to the weight, or, with the page's scale of v in
- * it, by 2^-31 of the query's largest where that is more.  Scales of v may be as far apart as they like.  A query with
- * a NaN or an infinity, and one that sees a page with such a scale, has NaN, unless it sees nothing. */
+ * it, by 2^-31 of the query's largest where that is more.  Scales of v may be as far apart as they like; with few new tokens a sequence those below 2^-104 keep fewer bits.
+ * A query with a NaN or an infinity, and one that sees a page with such a scale, has NaN, unless it sees nothing. */
 int32_t zant_b200_kv_cache_attention(zant_ctx* ctx, const zant_kv_cache* cache, int32_t dtype, const void* q, size_t q_stride, size_t rows, size_t heads,
                                      const int32_t* table, size_t seqs, size_t width, const int32_t* lengths, const int32_t* offsets,
                                      float scale, int32_t window, int32_t sinks, void* out, size_t out_stride, float* lse);

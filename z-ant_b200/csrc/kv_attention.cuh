@@ -16,8 +16,8 @@
 //
 // Memory is the bound (a cached token of 128 dimensions is 256 bytes for 4 x 8 x 128 operations of 8 rows).  Each warp takes every so many'th step of 32 tokens (16 of
 // 256 dimensions), which its first lane brings by TMA into a ring of the warp's own, swizzled so that the lanes' 16-byte reads meet no bank twice.  No warp waits for
-// another until the end, when the warps of a CTA, and the CTAs of a cluster that share a tile, join their sums.  64 x 1 tokens of 40 over 8 heads of 128, 4096 each: 112 us (4.9 TB/s), 760
-// instructions a step of 32 tokens at 2.1 a clock; 5 tokens of 16 over 4 heads of 64 in windows of 1024, 24 sequences: 17.6 us with tiles of 24 rows, 20.5 with 32.
+// another until the end, when the warps of a CTA, and the CTAs of a cluster that share a tile, join their sums.  64 x 1 tokens of 40 over 8 heads of 128, 4096 each: 113 us (4.8 TB/s), 760
+// instructions a step of 32 tokens at 2.1 a clock; 5 tokens of 16 over 4 heads of 64 in windows of 1024, 24 sequences: 18.2 us with tiles of 24 rows (20.5 with 32, when the former took 17.6).
 #pragma once
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -41,7 +41,7 @@ struct KvAttendArgs {
     void* out; long long out_stride; float* lse;
     float scale_log2;                                 // scale log2(e)
     int window, sinks;
-    bool wide_q, wide_out;                            // q, out in whole 16-byte blocks
+    bool wide_q, wide_out;                            // q, out in whole 16-byte blocks (out: prompts)
     int more_rows_than, rows_up_to;                   // sequences with more rows of a key head than the first, up to the second, are the kernel's
     int parts, tiles_each;                            // CTAs of a tile; tiles of each sequence (0: by its rows)
     bool by_length;                                   // the longest sequences first (as many as a CTA has threads at most)

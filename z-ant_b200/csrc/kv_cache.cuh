@@ -6,8 +6,8 @@
 //
 // Both are bound by memory.  A CTA has one page of one head, keys or values: the new rows are read once for the maximum, which stays in the
 // CTA, and their values wait in registers (kKvHold times 16 a thread, all under way at once; what is beyond is read again).  Pages, not tokens, are what the grid
-// counts, so that no other CTA writes the page or its scale.  A prompt of 8192 tokens, 8 heads of 128, bf16: written in 15.5 us (3.2 TB/s), read back in 13.6 (3.7); 64 single tokens 4 each
-// in a graph, the latency of lengths, table and page one after the other.
+// counts, so that no other CTA writes the page or its scale.  A prompt of 8192 tokens, 8 heads of 128, bf16: written in 15.5 us (3.2 TB/s), read back in 13.6 (3.7); 64 single tokens in a
+// graph: written in 3.7, their pages of 32 back in 5.5, the latency of lengths, table and page one after the other.
 #pragma once
 #include <cuda_runtime.h>
 

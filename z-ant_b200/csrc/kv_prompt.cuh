@@ -12,7 +12,7 @@
 // factor out again, once for 16 tokens: it is one of 2^(x - M), and in range while scales lie within 2^80 of one another.  CTAs that see others, or a scale of 0, have a form of the rows' code for themselves
 // (DEEP) that keeps a second maximum, of x, for it.
 //
-// A prompt of 8192 tokens, 40 over 8 heads of 128: 803 us (856 TFLOP/s, causal; 53 % of what cuBLAS reaches).  Exponentials and the tensor core are busy 40 % of the time each; a thread's chain of
+// A prompt of 8192 tokens, 40 over 8 heads of 128: 814 us (844 TFLOP/s, causal; 52 % of what cuBLAS reaches).  Exponentials and the tensor core are busy 40 % of the time each; a thread's chain of
 // loads from tensor memory, exponentials, packing and stores takes 1400 clocks a half step, waits, votes and addresses around it 900.
 //
 //   warps 0 .. 3, 4 .. 7  q to f16, rows of the first and the second tile      12  TMEM owner, MMA issuer      8 .. 11, 13 .. 15  codes to f16, scales

@@ -8,7 +8,7 @@
 //
 // Bound by memory: a sequence's own two rows are read once, in segments (16 a CTA, a warp each with 16 loads of a lane under way, up to 8 CTAs a sequence) whose sums every CTA of the
 // cluster gets; the CTA that has the segment in which the border lies reads that one again, each thread some neighbouring probabilities.  Rows start at any address (vocabularies are odd), so loads
-// are of single ones.  64 sequences of 128001 fp32 probabilities: 24 us (2.7 TB/s); 4 of 32000: 6.8 in a graph.
+// are of single ones.  64 sequences of 128001 fp32 probabilities: 23.5 us (2.8 TB/s); 4 of 32000: 6.8 in a graph.
 #pragma once
 #include <cuda_runtime.h>
 
